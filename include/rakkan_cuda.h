@@ -76,6 +76,7 @@ typedef struct rk_model rk_model;
 typedef struct rk_group rk_group;
 typedef struct rk_pipeline rk_pipeline;
 typedef struct rk_tensors rk_tensors;
+typedef struct rk_w4 rk_w4;
 
 /* gpu.Info (device.go:21-47). */
 typedef struct {
@@ -471,6 +472,135 @@ int rk_matrix_download(rk_matrix *m, void *w, float *scales);
 int rk_generate_normal(rk_device *d, uint64_t seed, uint64_t tid, int64_t offset, int64_t n, float scale, float *out);
 /* num.QuantizeQ8 / QuantizeQ4 of host floats, computed on the device. */
 int rk_quantize(rk_device *d, int fmt, const float *w, int64_t n, void *q, float *scales);
+
+/* ---- Serving operators on the caller's device buffers ----
+ * No counterpart in the reference: the pieces of a decode step that serves
+ * many sequences from one paged 8-bit cache with 8-bit activations and 4-bit
+ * weights. Their results are not the reference's bits (it has no such
+ * formats); each comment states what is computed.
+ *
+ * All of them take device buffers that the caller owns, enqueue their work
+ * on `stream` (a cudaStream_t; NULL: the device's own stream) and return
+ * without waiting; they allocate nothing, hold no state between calls and
+ * can be captured into a CUDA graph. The calling thread's current device is
+ * left as it was. Buffers must not overlap unless a comment says so, and
+ * need the alignment of their element type only, unless it says more.
+ * Wrong arguments return RK_ERR_ARGS before anything is enqueued. An index
+ * read on the device (a page, a slot) that lies outside the cache is never
+ * followed: what it names is left out, and the device's error word is set,
+ * which rk_device_check reports. */
+#define RK_ACT_F32 0
+#define RK_ACT_F16 1
+#define RK_ACT_BF16 2
+/* Waits for `stream` and returns RK_OK, or the status of what a kernel on
+ * this device has recorded since the word was last read (RK_ERR_ARGS: an
+ * index out of range; RK_ERR_TIMEOUT: a bounded wait), clearing it. */
+int rk_device_check(rk_device *d, void *stream);
+
+/* Block tables, slots and positions from request lengths, on the GPU.
+ * Request i holds ctx_lens[i] tokens and takes new_lens[i] more in this step
+ * (below zero: zero). table is [n][max_blocks]: entry j of a row is the page
+ * with the request's tokens [j*block, (j+1)*block). Pages for the new tokens
+ * come from free_pages[head ..  n_free) in order, request by request
+ * (head = *free_head, 0 if NULL); they are written to the row behind its
+ * ceil(ctx_lens / block) first entries, which are read and stay, as do the
+ * entries behind the new ones.
+ * Rows of the step's tokens lie request after request: request i's are
+ * [q_start[i], q_start[i+1]) (q_start: n + 1 values, none above max_tokens).
+ * slots[t] = page * block + offset and positions[t] (2^31 - 1 at most) for row t; behind the
+ * last row up to max_tokens, -1 and 0. lens[i] = ctx + new.
+ * A request is refused when its rows pass max_tokens, its tokens pass
+ * max_blocks * block, or the free pages do not suffice for it and those
+ * before it: it takes no page, its slots are -1 and its lens is 0, so that
+ * the append skips it and the attention gives zeros for its rows.
+ * info: {rows, pages taken, requests refused, head + pages taken}.
+ * n <= RK_MAX_REQUESTS; block is 16, 32, 64 or 128. */
+#define RK_MAX_REQUESTS 16384
+int rk_page_tables(rk_device *d, int n, int block, const int32_t *ctx_lens, const int32_t *new_lens,
+                   const int32_t *free_pages, const int32_t *free_head, int n_free, int32_t *table, int max_blocks,
+                   int32_t *lens, int32_t *q_start, int32_t *slots, int32_t *positions, int max_tokens, int32_t *info,
+                   void *stream);
+
+/* One layer's paged cache in 8 bits: token o of page p has, for kv head h,
+ * the key k[p][h][o][head_size] * k_scale[p][h] and the value
+ * v[p][h][head_size][o] * v_scale[p][h] (values are transposed within a
+ * page). block is 16, 32, 64 or 128 tokens, head_size a multiple of 16 up to
+ * 128, or 256; blocks * block fits in 31 bits. k and v are 16-byte aligned. */
+typedef struct {
+    int8_t *k, *v;          /* [blocks][kv_heads][block][head_size], [blocks][kv_heads][head_size][block] */
+    float *k_scale, *v_scale; /* [blocks][kv_heads] */
+    int blocks, block, kv_heads, head_size;
+} rk_kv8;
+/* Stores rows t < tokens of k and v ([kv_heads][head_size] each, rows
+ * k_stride and v_stride elements apart, of type RK_ACT_*) at slots[t]
+ * (below zero: the row is skipped). The rows of one page are consecutive in
+ * the call, in ascending slots, and a page is in one such run only; what a
+ * page below its run's first slot holds are earlier tokens, and what lies
+ * behind the run is left as it is. For each page and head, with m the
+ * largest finite magnitude of the run:
+ *   scale = max(the page's scale if it holds earlier tokens, m * fl(1/127)),
+ *           zero when below 2^-120;
+ *   new values: clamp(RoundToEven(x * fl(1/scale)), +-127), NaN as 0;
+ *   earlier ones, when the scale grew: RoundToEven(q * fl(old / scale)). */
+int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const void *k, int64_t k_stride, const void *v,
+                  int64_t v_stride, const int32_t *slots, void *stream);
+
+/* Attention over the cache. Request i < n holds lens[i] tokens, in the pages
+ * of row i of table ([n][max_blocks]); its queries are the rows
+ * [q_start[i], q_start[i+1]) of q (NULL: row i alone), the last of them the
+ * token lens[i] - 1. Query head h reads kv head h / (heads / kv_heads).
+ *   out = sum_t softmax_t(scale * q.k_t) v_t
+ * over the tokens t up to the query's own position and, when window > 0, the
+ * last `window` of those (its own among them); scale 0 is 1/sqrt(head_size).
+ * A query that sees no token gives zeros; one with a NaN or infinity gives
+ * NaN. q and out are [tokens][heads][head_size] of `type`, rows q_stride and
+ * out_stride elements apart; rows of no request are neither read nor
+ * written. Scores, sums and weighted values are held in float32; the keys
+ * and values enter exactly, the queries and softmax weights as float16
+ * (a query scaled by a power of two first), in one term for 16-bit types
+ * and in two (22 bits) for float32.
+ * workspace: rk_kv8_attention_workspace() bytes, 16-byte aligned, used during the
+ * call's kernels only; calls that may run at once need one each. */
+int64_t rk_kv8_attention_workspace(rk_device *d, const rk_kv8 *c, int heads);
+int rk_kv8_attention(rk_device *d, const rk_kv8 *c, int type, int n, int heads, int tokens, const void *q,
+                     int64_t q_stride, const int32_t *q_start, const int32_t *lens, const int32_t *table,
+                     int max_blocks, float scale, int window, void *out, int64_t out_stride, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+
+/* h = x + residual (residual NULL: x), and the root-mean-square norm
+ * y = h * weight / sqrt(mean(h^2) + eps) of each row in 8 bits: value j of a
+ * row is q[j] * scales[j / group]. sum_out (may be NULL) receives h rounded
+ * to `type`; the norm takes h before that rounding. sum_out may be residual
+ * or x (same stride). group divides cols (0: cols, one scale a row).
+ * The quotient y / (max|y| / 127) does not depend on the row's norm, so with
+ * u = fl(h * weight) and base = fl(max|u| * fl(1/127)) of a group (zero when
+ * below 2^-120), q = clamp(RoundToEven(u * fl(1/base)), +-127), NaN as 0, and
+ * scale = base / sqrt(mean(h^2) + eps). Rows of x, residual and sum_out are
+ * x_stride, r_stride and s_stride elements apart, of type RK_ACT_* as
+ * weight; q is [rows][cols], scales [rows][cols / group]. */
+int rk_add_rmsnorm_q8(rk_device *d, int type, int rows, int cols, int group, const void *x, int64_t x_stride,
+                      const void *residual, int64_t r_stride, const void *weight, float eps, void *sum_out,
+                      int64_t s_stride, int8_t *q, float *scales, void *stream);
+
+/* A matrix of 4-bit weights with a scale, and optionally a zero point, for
+ * each `group` columns of a row: weight = (u - zero) * scale, zero 8 when
+ * zeros is NULL. Host buffers: w is [rows][cols/2], packed as Q4_0 packs a
+ * block (byte j of 16 holds columns j and j + 16 of a block of 32, low and
+ * high half); scales [rows][cols/group] of type scale_type (RK_ACT_*), kept
+ * in it; zeros [rows][cols/group] of 0..15. group is a multiple of 32 that
+ * divides cols. */
+int rk_w4_upload(rk_device *d, int rows, int cols, int group, int scale_type, const uint8_t *w, const void *scales,
+                 const uint8_t *zeros, rk_w4 **out);
+void rk_w4_free(rk_w4 *m);
+int64_t rk_w4_bytes(const rk_w4 *m);
+/* out[t][rows] = m . (x[t] * x_scales[t]) for t < n: 8-bit vectors x
+ * [n][cols] (16-byte aligned) with a scale for each x_group columns (a
+ * multiple of 32 that divides cols; 0: cols), as rk_add_rmsnorm_q8 makes
+ * them. Products are exact integers within a run of columns that shares both
+ * scales; the runs are added in float32, and out (rows out_stride elements
+ * apart) is rounded to `type` once. */
+int rk_w4_mulvec(rk_w4 *m, int n, const int8_t *x, const float *x_scales, int x_group, int type, void *out,
+                 int64_t out_stride, void *stream);
 
 /* ---- Measurement helpers (device buffers, device stream, CUDA events) ---- */
 /* Times `iters` launches of the matvec of m on device-resident input and

@@ -32,6 +32,7 @@
 #include "rk_gen.cuh"
 #include "rk_layer.cuh"
 #include "rk_matvec.cuh"
+#include "rk_serve.cuh"
 #include "rk_tensor.cuh"
 
 using namespace rk;
@@ -192,6 +193,7 @@ extern "C" int rk_device_open(int index, rk_device **out) {
   if (e == cudaSuccess) e = init_layer_attributes();
   if (e == cudaSuccess) e = init_tensor_attributes();
   if (e == cudaSuccess) e = init_mvmany_attributes();
+  if (e == cudaSuccess) e = init_serve_attributes();
   if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&d->st, cudaStreamNonBlocking);
   if (e == cudaSuccess) e = cudaMalloc(&d->err_dev, 2 * sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(d->err_dev, 0, 2 * sizeof(int));
@@ -3808,6 +3810,25 @@ void internal_device_unlock(const rk_matrix *m) { m->d->mu.unlock(); }
 // Reads and clears the device error word, with check_dev_err's mapping of
 // the word to a status (call with the device mutex held, after a sync).
 int internal_check_dev_err(const rk_matrix *m) { return check_dev_err(m->d); }
+
+// What the operators on the caller's device buffers need of a device.
+void internal_device_view(const rk_device *d, int *ordinal, int *sms, void **stream, int **err_word) {
+  *ordinal = d->ordinal;
+  *sms = d->sms;
+  *stream = d->st;
+  *err_word = d->err_dev;
+}
+
+// Counts device memory that a handle holds (rk_device_used).
+void internal_device_count(rk_device *d, int64_t bytes) {
+  Guard g(d);
+  d->used += bytes;
+}
+
+int internal_device_check(rk_device *d) {
+  Guard g(d);
+  return check_dev_err(d);
+}
 }  // namespace rk
 
 extern "C" int rk_sample_argmax(rk_device *d, const float *logits, int n, int *index) {

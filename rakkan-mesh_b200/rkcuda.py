@@ -21,6 +21,8 @@ TENSOR_F32, TENSOR_I8, TENSOR_I32 = 0, 1, 2
 RK_BENCH_FLUSH, RK_BENCH_FUSED = 1, 2
 MAX_COLS, MAX_ROWS = 1 << 18, 1 << 20
 NOALLOC_MAX_COLS = 32768
+ACT_F32, ACT_F16, ACT_BF16 = 0, 1, 2
+MAX_REQUESTS = 16384
 
 # Every symbol include/rakkan_cuda.h declares.
 EXPORTS = [
@@ -43,6 +45,8 @@ EXPORTS = [
     "rk_tensors_new", "rk_tensors_free", "rk_tensors_used", "rk_tensors_from_memory", "rk_tensors_from_blob",
     "rk_tensors_to_memory", "rk_tensors_dim", "rk_tensors_release", "rk_tensors_matmul", "rk_tensors_add",
     "rk_tensors_scale", "rk_tensors_relu", "rk_tensors_softmax", "rk_tensors_quantize", "rk_tensors_argmax",
+    "rk_device_check", "rk_page_tables", "rk_kv8_append", "rk_kv8_attention_workspace", "rk_kv8_attention",
+    "rk_add_rmsnorm_q8", "rk_w4_upload", "rk_w4_free", "rk_w4_bytes", "rk_w4_mulvec",
 ]
 
 
@@ -78,6 +82,11 @@ class HostLayer(C.Structure):
     _fields_ = [("rms_att", C.c_void_p), ("rms_ffn", C.c_void_p), ("bq", C.c_void_p), ("bk", C.c_void_p),
                 ("bv", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)] + [
                    (n, HostMatrix) for n in ("wq", "wk", "wv", "wo", "w1", "w2", "w3")]
+
+
+class KV8(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("blocks", C.c_int), ("block", C.c_int), ("kv_heads", C.c_int), ("head_size", C.c_int)]
 
 
 _lib = None
@@ -150,6 +159,14 @@ def lib():
             "rk_layer_load_part": (i, [vp, vp, vp, i64, vp]), "rk_embed_load_part": (i, [vp, vp, vp, i64, vp]),
             "rk_head_load_part": (i, [vp, vp, vp, i64, vp, vp, vp]),
             "rk_matmul_bf16": (i, [vp, i, vp, vp]), "rk_measure_speed": (i, [vp, vp]),
+            "rk_device_check": (i, [vp, vp]),
+            "rk_page_tables": (i, [vp, i, i, vp, vp, vp, vp, i, vp, i, vp, vp, vp, vp, i, vp, vp]),
+            "rk_kv8_append": (i, [vp, vp, i, i, vp, i64, vp, i64, vp, vp]),
+            "rk_kv8_attention_workspace": (i64, [vp, vp, i]),
+            "rk_kv8_attention": (i, [vp, vp, i, i, i, i, vp, i64, vp, vp, vp, i, f, i, vp, i64, vp, i64, vp]),
+            "rk_add_rmsnorm_q8": (i, [vp, i, i, i, i, vp, i64, vp, i64, vp, f, vp, i64, vp, vp, vp]),
+            "rk_w4_upload": (i, [vp, i, i, i, i, vp, vp, vp, vp]), "rk_w4_free": (None, [vp]),
+            "rk_w4_bytes": (i64, [vp]), "rk_w4_mulvec": (i, [vp, i, vp, vp, i, i, vp, i64, vp]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -815,4 +832,268 @@ class Tensors:
     def free(self):
         if self.h:
             lib().rk_tensors_free(self.h)
+            self.h = C.c_void_p()
+
+
+# ---------------------------------------------------------------------------
+# Serving operators over torch tensors on the device (rk_page_tables,
+# rk_kv8_*, rk_add_rmsnorm_q8, rk_w4_*). They run on torch's current stream of
+# the device, do not wait, and can be captured into a torch CUDA graph. Wrong
+# tensors raise RkError(RK_ERR_ARGS) before anything runs.
+# ---------------------------------------------------------------------------
+_t = None
+
+
+def _torch():
+    """torch, imported by the first use of an operator that takes tensors."""
+    global _t
+    if _t is None:
+        import types
+
+        import torch
+        # Handle 0 is torch's name for the legacy default stream; the C ABI
+        # reads NULL as the device's own, so the legacy stream's handle is passed.
+        _t = types.SimpleNamespace(
+            torch=torch, stream=lambda index: torch._C._cuda_getCurrentRawStream(index) or 1,
+            act={torch.float32: ACT_F32, torch.float16: ACT_F16, torch.bfloat16: ACT_BF16},
+            f32=torch.float32, i32=torch.int32, i8=torch.int8, u8=torch.uint8)
+    return _t
+
+
+def _refuse(msg):
+    raise RkError(RK_ERR_ARGS, msg)
+
+
+def _tensor(x, index, dtype, what, shape=None):
+    """A contiguous tensor of the dtype on the device (and of the shape): its address."""
+    if not x.is_cuda or x.get_device() != index:
+        _refuse(f"{what}: a tensor on {x.device}, not on cuda:{index}")
+    if x.dtype is not dtype:
+        _refuse(f"{what}: a tensor of {x.dtype}, not of {dtype}")
+    if shape is not None and x.shape != shape:
+        _refuse(f"{what}: shape {tuple(x.shape)}, not {tuple(shape)}")
+    if not x.is_contiguous():
+        _refuse(f"{what}: not contiguous")
+    return x.data_ptr()
+
+
+def _rows(x, index, dtype, what, shape):
+    """A tensor of rows that are contiguous inside and lie a stride apart: its address and that stride."""
+    if not x.is_cuda or x.get_device() != index:
+        _refuse(f"{what}: a tensor on {x.device}, not on cuda:{index}")
+    if x.dtype is not dtype:
+        _refuse(f"{what}: a tensor of {x.dtype}, not of {dtype}")
+    if x.shape != shape:
+        _refuse(f"{what}: shape {tuple(x.shape)}, not {tuple(shape)}")
+    if not x.is_contiguous():
+        want = 1
+        for size, stride in zip(reversed(shape[1:]), reversed(x.stride()[1:])):
+            if size != 1 and stride != want:
+                _refuse(f"{what}: rows that are not contiguous inside (strides {x.stride()})")
+            want *= size
+        if shape[0] > 1:
+            return x.data_ptr(), x.stride(0)
+    width = 1
+    for size in shape[1:]:
+        width *= size
+    return x.data_ptr(), width
+
+
+def device_check(dev):
+    """Waits for torch's current stream of the device; raises what a kernel on it has recorded."""
+    _check(lib().rk_device_check(dev.h, _torch().stream(dev.info.index)))
+
+
+class PageTables:
+    """The block tables, slots and positions of a scheduler's steps
+    (rk_page_tables), in tensors kept from step to step: table [n][max_blocks],
+    lens [n], q_start [n + 1], slots and positions [max_tokens], info [4] (rows,
+    pages taken, requests refused, the free list's next head)."""
+
+    def __init__(self, dev, n, max_blocks, block, max_tokens, table=None):
+        t = _torch()
+        self.dev, self.index, self.n, self.max_blocks, self.block, self.max_tokens = dev, dev.info.index, n, max_blocks, block, max_tokens
+
+        def ints(*shape):
+            return t.torch.zeros(shape, dtype=t.i32, device=f"cuda:{self.index}")
+        self.table = ints(n, max_blocks) if table is None else table
+        _tensor(self.table, self.index, t.i32, "page tables: table", (n, max_blocks))
+        self.lens, self.q_start, self.info = ints(n), ints(n + 1), ints(4)
+        self.slots, self.positions = ints(max_tokens), ints(max_tokens)
+        self._out = [x.data_ptr() for x in (self.table, self.lens, self.q_start, self.slots, self.positions, self.info)]
+
+    def build(self, ctx_lens, new_lens, free_pages, free_head=None):
+        """One step: int32 tensors ctx_lens and new_lens [n], free_pages [any] and free_head [1] (None: 0)."""
+        t, i = _torch(), self.index
+        ctx = _tensor(ctx_lens, i, t.i32, "page tables: ctx_lens", (self.n,))
+        new = _tensor(new_lens, i, t.i32, "page tables: new_lens", (self.n,))
+        free = _tensor(free_pages, i, t.i32, "page tables: free_pages")
+        head = None if free_head is None else _tensor(free_head, i, t.i32, "page tables: free_head", (1,))
+        table, lens, q_start, slots, positions, info = self._out
+        rc = _lib.rk_page_tables(self.dev.h, self.n, self.block, ctx, new, free, head, free_pages.numel(), table,
+                                 self.max_blocks, lens, q_start, slots, positions, self.max_tokens, info, t.stream(i))
+        if rc:
+            _check(rc)
+
+
+class PagedKV8:
+    """One layer's paged cache in 8 bits (rk_kv8) over four tensors: k
+    [blocks][kv_heads][block][head_size] and v [blocks][kv_heads][head_size][block]
+    int8, k_scale and v_scale [blocks][kv_heads] float32."""
+
+    def __init__(self, dev, k, v, k_scale, v_scale):
+        t = _torch()
+        self.dev, self.index = dev, dev.info.index
+        if k.dim() != 4:
+            _refuse(f"kv8: keys of {k.dim()} dimensions, not 4")
+        blocks, kv_heads, block, hs = k.shape
+        self.blocks, self.kv_heads, self.block, self.head_size = blocks, kv_heads, block, hs
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.c = KV8(_tensor(k, self.index, t.i8, "kv8: k"), _tensor(v, self.index, t.i8, "kv8: v", (blocks, kv_heads, hs, block)),
+                     _tensor(k_scale, self.index, t.f32, "kv8: k_scale", (blocks, kv_heads)),
+                     _tensor(v_scale, self.index, t.f32, "kv8: v_scale", (blocks, kv_heads)), blocks, block, kv_heads, hs)
+        self.at = C.addressof(self.c)
+        self._ws = {}  # workspace bytes by the number of query heads
+
+    @classmethod
+    def new(cls, dev, blocks, kv_heads, block, head_size):
+        """An empty cache."""
+        t = _torch()
+
+        def zeros(dtype, *shape):
+            return t.torch.zeros(shape, dtype=dtype, device=f"cuda:{dev.info.index}")
+        return cls(dev, zeros(t.i8, blocks, kv_heads, block, head_size), zeros(t.i8, blocks, kv_heads, head_size, block),
+                   zeros(t.f32, blocks, kv_heads), zeros(t.f32, blocks, kv_heads))
+
+    def append(self, k, v, slots):
+        """Stores rows k and v [tokens][kv_heads][head_size] (float32, float16 or
+        bfloat16; rows may lie a stride apart) at slots [tokens]."""
+        t, i = _torch(), self.index
+        act = t.act.get(k.dtype)
+        if act is None:
+            _refuse(f"kv8 append: keys of {k.dtype}")
+        n = slots.numel()
+        shape = (n, self.kv_heads, self.head_size)
+        kp, ks = _rows(k, i, k.dtype, "kv8 append: k", shape)
+        vp, vs = _rows(v, i, k.dtype, "kv8 append: v", shape)
+        sp = _tensor(slots, i, t.i32, "kv8 append: slots", (n,))
+        rc = _lib.rk_kv8_append(self.dev.h, self.at, act, n, kp, ks, vp, vs, sp, t.stream(i))
+        if rc:
+            _check(rc)
+
+    def attention(self, q, table, lens, q_start=None, scale=0.0, window=0, out=None):
+        """Attention of q [tokens][heads][head_size] (rows may lie a stride apart)
+        over the cache: requests of lens [n] tokens in the pages of table
+        [n][max_blocks], their queries at rows q_start [n + 1] (None: row i is
+        request i's). Rows of no request are left as out has them (out=None:
+        undefined). Returns out."""
+        t, i = _torch(), self.index
+        act = t.act.get(q.dtype)
+        if act is None:
+            _refuse(f"kv8 attention: queries of {q.dtype}")
+        if q.dim() != 3 or q.shape[2] != self.head_size:
+            _refuse(f"kv8 attention: queries of shape {tuple(q.shape)}, head size {self.head_size}")
+        shape = q.shape
+        tokens, heads = shape[0], shape[1]
+        n, max_blocks = table.shape
+        qp, qs = _rows(q, i, q.dtype, "kv8 attention: q", shape)
+        if out is None:
+            out = t.torch.empty(shape, dtype=q.dtype, device=q.device)
+        op, os_ = _rows(out, i, q.dtype, "kv8 attention: out", shape)
+        tp = _tensor(table, i, t.i32, "kv8 attention: table")
+        lp = _tensor(lens, i, t.i32, "kv8 attention: lens", (n,))
+        sp = None if q_start is None else _tensor(q_start, i, t.i32, "kv8 attention: q_start", (n + 1,))
+        need = self._ws.get(heads)
+        if need is None:
+            need = _lib.rk_kv8_attention_workspace(self.dev.h, self.at, heads)
+            if need < 0:
+                _check(need)
+            self._ws[heads] = need
+        # A workspace of each call's own, from torch's allocator: it belongs to
+        # the stream (or to the graph being captured) that uses it.
+        ws = t.torch.empty(need, dtype=t.u8, device=q.device) if need else None
+        rc = _lib.rk_kv8_attention(self.dev.h, self.at, act, n, heads, tokens, qp, qs, sp, lp, tp, max_blocks, scale, window,
+                                   op, os_, ws.data_ptr() if need else None, need, t.stream(i))
+        if rc:
+            _check(rc)
+        return out
+
+
+def add_rmsnorm_q8(dev, x, weight, eps, group=32, residual=None, sum_out=None):
+    """h = x + residual and its RMSNorm in 8 bits (rk_add_rmsnorm_q8): x and
+    residual [rows][cols] (rows may lie a stride apart), weight [cols]; group 0
+    is one scale a row. Returns (q int8 [rows][cols], scales [rows][cols / group],
+    h), h in sum_out if given, in a new tensor if there is a residual, else None."""
+    t, i = _torch(), dev.info.index
+    act = t.act.get(x.dtype)
+    if act is None or x.dim() != 2:
+        _refuse(f"norm q8: x of {x.dtype} and {x.dim()} dimensions")
+    shape = x.shape
+    rows, cols = shape
+    xp, xs = _rows(x, i, x.dtype, "norm q8: x", shape)
+    wp = _tensor(weight, i, x.dtype, "norm q8: weight", (cols,))
+    rp, rs = (None, cols) if residual is None else _rows(residual, i, x.dtype, "norm q8: residual", shape)
+    if sum_out is None and residual is not None:
+        sum_out = t.torch.empty(shape, dtype=x.dtype, device=x.device)
+    sp, ss = (None, cols) if sum_out is None else _rows(sum_out, i, x.dtype, "norm q8: sum_out", shape)
+    if group < 0 or group and cols % group:
+        _refuse(f"norm q8: groups of {group} in {cols} columns")
+    q = t.torch.empty(shape, dtype=t.i8, device=x.device)
+    scales = t.torch.empty((rows, cols // (group or cols)), dtype=t.f32, device=x.device)
+    rc = lib().rk_add_rmsnorm_q8(dev.h, act, rows, cols, group, xp, xs, rp, rs, wp, eps, sp, ss, q.data_ptr(), scales.data_ptr(),
+                                 t.stream(i))
+    if rc:
+        _check(rc)
+    return q, scales, sum_out
+
+
+class W4Matrix:
+    """A matrix of 4-bit weights with group scales on the device (rk_w4): host
+    tensors w [rows][cols / 2] uint8 (Q4_0's packing of a block of 32), scales
+    [rows][cols / group] (float32, float16 or bfloat16) and zeros (uint8, None: 8)."""
+
+    def __init__(self, dev, w, scales, zeros=None):
+        t = _torch()
+        self.dev, self.index = dev, dev.info.index
+        if w.dim() != 2 or scales.dim() != 2 or w.dtype is not t.u8 or scales.dtype not in t.act:
+            _refuse(f"w4: weights of {w.dtype}, scales of {scales.dtype}")
+        self.rows, self.cols = w.shape[0], 2 * w.shape[1]
+        if scales.shape[0] != self.rows or scales.shape[1] < 1 or self.cols % scales.shape[1]:
+            _refuse(f"w4: scales of shape {tuple(scales.shape)} for {self.rows}x{self.cols} weights")
+        if zeros is not None and (zeros.dtype is not t.u8 or zeros.shape != scales.shape):
+            _refuse("w4: zero points are uint8, one for each scale")
+        self.group = self.cols // scales.shape[1]
+        w, scales = w.cpu().contiguous(), scales.cpu().contiguous()
+        zeros = None if zeros is None else zeros.cpu().contiguous()
+        self.h = C.c_void_p()
+        _check(lib().rk_w4_upload(dev.h, self.rows, self.cols, self.group, t.act[scales.dtype], w.data_ptr(), scales.data_ptr(),
+                                  None if zeros is None else zeros.data_ptr(), C.byref(self.h)))
+
+    def mulvec(self, x, x_scales, dtype=None, out=None):
+        """W.(x * x_scales) for each row of x int8 [n][cols], x_scales float32
+        [n][cols / x_group]; returns [n][rows] of dtype (float32 by default), or out."""
+        t, i = _torch(), self.index
+        n = x.shape[0]
+        xp = _tensor(x, i, t.i8, "w4: x", (n, self.cols))
+        groups = x_scales.shape[-1]
+        sp = _tensor(x_scales, i, t.f32, "w4: x_scales", (n, groups))
+        if groups < 1 or self.cols % groups:
+            _refuse(f"w4: {groups} scales a vector for {self.cols} columns")
+        if out is None:
+            out = t.torch.empty((n, self.rows), dtype=t.f32 if dtype is None else dtype, device=x.device)
+        act = t.act.get(out.dtype)
+        if act is None:
+            _refuse(f"w4: an output of {out.dtype}")
+        op, os_ = _rows(out, i, out.dtype, "w4: out", (n, self.rows))
+        rc = _lib.rk_w4_mulvec(self.h, n, xp, sp, self.cols // groups, act, op, os_, t.stream(i))
+        if rc:
+            _check(rc)
+        return out
+
+    def bytes(self):
+        return lib().rk_w4_bytes(self.h)
+
+    def free(self):
+        if self.h:
+            lib().rk_w4_free(self.h)
             self.h = C.c_void_p()
