@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "librakkan_cuda.so")
 SOURCES = ["rk_matvec.cu", "rk_layer.cu", "rk_tensor.cu", "rk_gen.cu", "rk_capi.cu", "rk_noalloc.cu", "rk_mvmany.cu",
-           "rk_serve.cu", "rk_paged.cu", "rk_attn8.cu", "rk_attn8_f32.cu",
+           "rk_serve.cu", "rk_paged.cu", "rk_attn8.cu", "rk_attn8_two.cu",
            "rk_norm8.cu", "rk_w4.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 

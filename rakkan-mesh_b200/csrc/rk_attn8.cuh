@@ -11,28 +11,30 @@
 // warp streams its own tiles from global memory into the registers that the
 // products read.
 //
-// Fragments. A 16-column step of a product may take its columns in any order
-// as long as both operands agree. Lane (r, c) = (lane / 4, lane % 4) holds
-// columns {2c, 2c+1, 2c+8, 2c+9} of a step; they are given to four
-// neighbouring bytes, so that a lane's bytes of several steps are one 16-, 8-
-// or 4-byte load: of a key row, dimensions; of a transposed value row,
-// tokens. The scores' columns (tokens) land where the second product wants
-// its rows, which fixes the token of a key row (token_of).
+// Fragments. Keys and transposed values are the 16-row operand, queries and
+// weights the 8-column one: a tile of 8 query rows then fills the columns,
+// and half as many products and registers do as with queries in the rows
+// (91 us that way). A 16-long step of a product may
+// take its terms in any order as long as both operands agree. Lane
+// (r, c) = (lane / 4, lane % 4) holds terms {2c, 2c+1, 2c+8, 2c+9} of a step;
+// they are given to four neighbouring bytes, so that a lane's bytes of
+// several steps are one 16-, 8- or 4-byte load: of a key row, dimensions; of a
+// transposed value row, tokens. The scores come out as (token, query); a
+// transposing move of 8x8 registers makes them the second product's column
+// operand, which fixes the token of each key row.
 //
 // Precision. A float32 row of queries is scaled by a power of two to a
-// largest magnitude near 2^13 and split into two float16 terms (22 bits)
-// that fill both halves of the 16 rows (8 query rows, high and low terms);
-// 16-bit queries are one exact term (16 query rows). The softmax weights
-// likewise, with the value scale in the weight: w_t = 2^(s_t + E - M + 14)·f
-// for vs = f·2^E, with M the running maximum of s_t + E + 1 and so
-// w_t <= 2^14. The denominator has a running maximum of its own (m), so
-// that pages of any two scales are weighed rightly. 16-bit types round a
-// weight once to float16 (2^-12 of itself, an eighth of bfloat16's own
-// rounding of the result, and half of float16's on average over tokens).
+// largest magnitude near 2^13 and split into two float16 terms (22 bits);
+// 16-bit queries are one exact term. The softmax weights likewise, with the
+// value scale in the weight: w_t = 2^(s_t - M + E + 14) f for vs = f 2^E, M
+// within a power of two of the running maximum of s_t + E + 1 and so
+// w_t < 2^16. The denominator has a reference of its own (m), so that pages
+// of any two scales are weighed rightly. 16-bit types round a weight once to
+// float16 (2^-12 of itself, an eighth of bfloat16's own rounding of the
+// result, and half of float16's on average over tokens).
 //
 // Work. A unit is a request's kv head and up to four tiles of query rows; its
-// keys are cut into tiles of 32 tokens (16 at head size 256). The tiles of all
-// units in a row are dealt out in equal runs, one to a CTA, so that lengths
+// keys are cut into tiles of 32 tokens. The tiles of all units in a row are dealt out in equal runs, one to a CTA, so that lengths
 // need not be alike and one long request fills the GPU as well as many short
 // ones. Within a CTA the warps take different row tiles of the same tokens
 // (their loads meet in L1) or, where there are fewer, different tokens. A unit
@@ -48,15 +50,21 @@ namespace rk {
 constexpr int kA8Warps = 4;
 constexpr int kA8Threads = 32 * kA8Warps;
 
+constexpr int kA8Tile = 32;  // tokens
 template <int HS>
 struct A8Shape {
-  static constexpr int TT = HS > 128 ? 16 : 32;  // tokens of a tile
-  static constexpr int CTAS = HS > 128 ? 1 : HS > 64 ? 2 : HS > 32 ? 3 : 4;  // of an SM, by their registers
-  static constexpr int KS = HS / 16;             // 16-column steps over a head
-  static constexpr int PITCH = HS + 8;           // floats between rows of a merge buffer
+  static constexpr int KS = HS / 16;        // 16-long steps over a head
+  static constexpr int PITCH = HS + 4;      // floats between rows of a merge buffer
+  static constexpr int KBYTES = kA8Tile * HS, TILE = 2 * KBYTES;  // of a tile: keys [32][HS], values [HS][32]
+  static constexpr int RING = 4 * 2 * TILE; // of a CTA: two tiles a warp
 };
+// CTAs of an SM, by their registers and shared memory (TERMS float16 terms,
+// NT tiles of 8 rows a warp).
+__host__ __device__ constexpr int a8_ctas(int hs, int terms, int nt) {
+  return hs > 128 ? 1 : nt > 1 ? (hs > 64 ? 2 : 3) : hs > 64 ? 3 : 4;
+}
 
-// A part's place in the workspace: 4 row tiles of 16 rows, each HS sums and
+// A part's place in the workspace: up to 64 rows, each HS sums and
 // (m, M, l), behind the records of all CTAs.
 struct A8Record {
   int first, last;       // CTAs of the unit (first < 0: no unit crosses into this CTA)
@@ -69,7 +77,8 @@ __host__ __device__ inline int64_t a8_part_floats(int hs) { return 64LL * (hs + 
 
 struct A8Grid {
   int ctas;       // CTAs of the main kernel
-  int min_tiles;  // fewest tiles worth a CTA
+  int min_tiles;  // fewest tiles worth a CTA; 0: a CTA takes whole units
+  int log_block;  // of the page's tokens
 };
 
 RK_DEV uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
@@ -89,7 +98,7 @@ RK_DEV void i8_to_h2(uint32_t w, uint32_t &p01, uint32_t &p23) {
   p23 = *reinterpret_cast<uint32_t *>(&hb);
 }
 
-RK_DEV void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+RK_DEV void mma16816(float *c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -106,28 +115,45 @@ RK_DEV uint32_t pack_h2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
+// An 8x8 tile of 16-bit values, a pair of neighbours a lane, transposed.
+RK_DEV uint32_t transpose_h2(uint32_t v) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
 // The part of (a, b) that pack_h2 left.
 RK_DEV uint32_t pack_rest(float a, float b, uint32_t p) {
   const __half2 h = *reinterpret_cast<const __half2 *>(&p);
   return pack_h2(a - __low2float(h), b - __high2float(h));
 }
 
-// A lane's words of one row of HS bytes: word s is step s's four bytes.
-// Whole 64-byte stretches as 16 bytes a lane, then 32 as 8, then 16 as 4.
+RK_DEV void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+RK_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+RK_DEV void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Key rows of 128 and 256 bytes would meet in the same banks; the 64-byte
+// stretches of odd rows change places in pairs.
 template <int HS>
-RK_DEV void load_row(const int8_t *row, int c, uint32_t *w) {
+RK_DEV int key_swizzle(int row) { return HS % 128 == 0 ? (row & 1) << 6 : 0; }
+
+// A lane's words of one key row: word s is step s's four bytes. Whole 64-byte
+// stretches as 16 bytes a lane, then 32 as 8, then 16 as 4.
+template <int HS>
+RK_DEV void load_row(const char *row, int swizzle, int c, uint32_t *w) {
   constexpr int N64 = HS / 64, R = HS % 64;
 #pragma unroll
   for (int i = 0; i < N64; i++) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(row + 64 * i + 16 * c));
+    const uint4 v = *reinterpret_cast<const uint4 *>(row + ((64 * i) ^ swizzle) + 16 * c);
     w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
   }
   if constexpr (R >= 32) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(row + 64 * N64 + 8 * c));
+    const uint2 v = *reinterpret_cast<const uint2 *>(row + 64 * N64 + 8 * c);
     w[4 * N64] = v.x, w[4 * N64 + 1] = v.y;
   }
-  if constexpr (R % 32 != 0)
-    w[HS / 16 - 1] = __ldg(reinterpret_cast<const uint32_t *>(row + HS - 16 + 4 * c));
+  if constexpr (R % 32 != 0) w[HS / 16 - 1] = *reinterpret_cast<const uint32_t *>(row + HS - 16 + 4 * c);
 }
 // The dimension of byte b (0..3) of lane c's word s.
 template <int HS>
@@ -159,9 +185,9 @@ struct A8Req {
   int rw;          // row tiles of a unit (1, 2 or 4)
 };
 
-template <int HS, bool SPLIT>
+template <int HS, int R>
 RK_DEV A8Req a8_req(const Attn8Args &a, int i) {
-  constexpr int TT = A8Shape<HS>::TT, R = SPLIT ? 8 : 16;
+  constexpr int TT = kA8Tile;
   A8Req q;
   if (a.q_start) {
     q.q0 = min(max(a.q_start[i], 0), a.tokens);
@@ -176,35 +202,36 @@ RK_DEV A8Req a8_req(const Attn8Args &a, int i) {
   const long long from = a.window > 0 ? max(0LL, q.last - (q.nq - 1) + 1 - a.window) : 0;
   q.tile0 = (int)min((long long)q.len, from) / TT;
   q.tiles = max(1, (q.len + TT - 1) / TT - q.tile0);
-  const int rts = (int)(((long long)q.nq * (a.heads / a.c.kv_heads) + R - 1) / R);
+  const long long rows = (long long)q.nq * (a.heads / a.c.kv_heads);
+  const int rts = (int)((rows + R - 1) / R);
   q.rw = rts >= 4 ? 4 : rts >= 2 ? 2 : 1;
   q.units = (rts + q.rw - 1) / q.rw;
   return q;
 }
 
-template <int HS, bool SPLIT, bool WIDE>
-__global__ void __launch_bounds__(kA8Threads, A8Shape<HS>::CTAS) k_attn8(Attn8Args a, int type, A8Grid grid) {
+template <int HS, int TERMS, int NT>
+__global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(Attn8Args a, int type, A8Grid grid) {
   using Shape = A8Shape<HS>;
-  constexpr int TT = Shape::TT, KS = Shape::KS, PITCH = Shape::PITCH, R = SPLIT ? 8 : 16;
-  constexpr int NH = TT / 16, ND = HS / 8;  // 16-token halves of a tile; 8-dimension columns of the output
-  extern __shared__ __align__(16) float sm[];
-  float *s_o = sm;                                     // [warps][16][PITCH]
-  float *s_st = sm + kA8Warps * 16 * PITCH;            // [warps][16][4]
+  constexpr int TT = kA8Tile, KS = Shape::KS, PITCH = Shape::PITCH, R = 8 * NT, ND = HS / 8;
+  static_assert(kA8Warps * R * (PITCH + 4) * 4 <= Shape::RING, "the merge buffers fit the rings");
+  extern __shared__ __align__(128) char sm[];
+  // The rings; between two units, the merge buffers [warps][R][PITCH] and [warps][R][4].
+  float *s_o = reinterpret_cast<float *>(sm), *s_st = s_o + kA8Warps * R * PITCH;
   __shared__ long long s_scan[kA8Warps + 1];
   __shared__ long long s_before;
   __shared__ int s_req;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
-  const int G = a.heads / a.c.kv_heads, H = a.c.kv_heads, B = a.c.block;
+  const int G = a.heads / a.c.kv_heads, H = a.c.kv_heads, lb = grid.log_block;
   griddep_trigger();
 
-  // The run of tiles of this CTA: a scan over the requests' tiles.
+  // The run of tiles (or of whole units) of this CTA: a scan over the
+  // requests' sizes.
+  const bool by_unit = grid.min_tiles == 0;
   const int per_t = (a.n + kA8Threads - 1) / kA8Threads;
   const int i0 = min(a.n, tid * per_t), i1 = min(a.n, i0 + per_t);
+  auto size_of = [&](const A8Req &q) { return (long long)H * q.units * (by_unit ? 1 : q.tiles); };
   long long mine = 0;
-  for (int i = i0; i < i1; i++) {
-    const A8Req q = a8_req<HS, SPLIT>(a, i);
-    mine += (long long)H * q.units * q.tiles;
-  }
+  for (int i = i0; i < i1; i++) mine += size_of(a8_req<HS, R>(a, i));
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -218,19 +245,18 @@ __global__ void __launch_bounds__(kA8Threads, A8Shape<HS>::CTAS) k_attn8(Attn8Ar
     if (w < warp) excl += s_scan[w];
     total += s_scan[w];
   }
-  const long long per = max((long long)grid.min_tiles, (total + grid.ctas - 1) / grid.ctas);
+  const long long per = max((long long)max(grid.min_tiles, 1), (total + grid.ctas - 1) / grid.ctas);
   const long long begin = per * blockIdx.x, end = min(total, begin + per);
   A8Record *records = static_cast<A8Record *>(a.ws);
   float *parts = reinterpret_cast<float *>(records + grid.ctas);
   if (begin >= end) {
-    if (tid == 0) records[blockIdx.x].first = -1;
+    if (tid == 0 && !by_unit) records[blockIdx.x].first = -1;
     return;
   }
   if (begin >= excl && begin < excl + mine) {
     long long p = excl;
     for (int i = i0; i < i1; i++) {
-      const A8Req q = a8_req<HS, SPLIT>(a, i);
-      const long long size = (long long)H * q.units * q.tiles;
+      const long long size = size_of(a8_req<HS, R>(a, i));
       if (begin < p + size) {
         s_req = i;
         s_before = p;
@@ -241,63 +267,128 @@ __global__ void __launch_bounds__(kA8Threads, A8Shape<HS>::CTAS) k_attn8(Attn8Ar
   }
   __syncthreads();
   int req = s_req;
-  long long base = s_before;  // where the request's tiles begin
-  A8Req q = a8_req<HS, SPLIT>(a, req);
+  long long base = s_before;  // where the request's run begins
+  A8Req q = a8_req<HS, R>(a, req);
 
   for (long long at = begin; at < end;) {
     // The unit at `at`, and this CTA's tiles of it.
-    while (at >= base + (long long)H * q.units * q.tiles) {
-      base += (long long)H * q.units * q.tiles;
-      q = a8_req<HS, SPLIT>(a, ++req);
+    while (at >= base + size_of(q)) {
+      base += size_of(q);
+      q = a8_req<HS, R>(a, ++req);
     }
-    const int u = (int)((at - base) / q.tiles);
+    const int step = by_unit ? 1 : q.tiles;
+    const int u = (int)(at - base) / step;
     const int head = u / q.units, rg = u % q.units;
-    const long long u0 = base + (long long)u * q.tiles, u1 = u0 + q.tiles;
-    const int t0 = (int)(at - u0), t1 = (int)(min(end, u1) - u0);
+    const long long u0 = base + (long long)u * step, u1 = u0 + step;
+    const int t0 = (int)(at - u0), t1 = by_unit ? q.tiles : (int)(min(end, u1) - u0);
     const int rw = q.rw, tw = kA8Warps / rw, wr = warp % rw, wt = warp / rw;
     const int row0 = (rg * rw + wr) * R;        // of the request's nq·G rows (token-major)
     const int all_rows = q.nq * G;
 
-    // Limits of this lane's rows: visible tokens are (low, high]. Rows past
-    // the last see all (their queries are zeros, their sums are not stored).
-    int high[2], low[2], high_max = -1;
-    float f[2];
+    const int unit_row0 = rg * rw * R, unit_rows = min(rw * R, all_rows - unit_row0);
+
+    // Limits of this lane's query columns: visible tokens are (low, high].
+    // Columns past the last row see all (their queries are zeros, their sums
+    // are not stored).
+    const long long pos0 = q.last - (q.nq - 1);
+    int high[NT][2], low[NT][2], high_max = -1, high_min = 0x7fffffff, low_max = -1;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const int row = row0 + r + 8 * (SPLIT ? 0 : j);
-      const long long pos = q.last - (q.nq - 1) + row / G;
-      high[j] = 0x7fffffff;
-      low[j] = -1;
-      if (row < all_rows) {
-        high[j] = (int)max(-1LL, min(pos, (long long)q.len - 1));
-        if (a.window > 0) low[j] = (int)max(-1LL, min(pos - a.window, (long long)q.len));
-        high_max = max(high_max, high[j]);
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int row = row0 + 8 * n + 2 * c + e;
+        high[n][e] = 0x7fffffff;
+        low[n][e] = -1;
+        if (row < all_rows) {
+          const long long pos = pos0 + row / G;
+          high[n][e] = (int)max(-1LL, min(pos, (long long)q.len - 1));
+          if (a.window > 0) low[n][e] = (int)max(-1LL, min(pos - a.window, (long long)q.len));
+          high_max = max(high_max, high[n][e]);
+        }
+        high_min = min(high_min, high[n][e]);
+        low_max = max(low_max, low[n][e]);
       }
-    }
-    int high_min = min(high[0], high[1]), low_max = max(low[0], low[1]);
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
+    for (int o = 1; o < 4; o <<= 1) {
       high_max = max(high_max, __shfl_xor_sync(0xffffffffu, high_max, o));
       high_min = min(high_min, __shfl_xor_sync(0xffffffffu, high_min, o));
       low_max = max(low_max, __shfl_xor_sync(0xffffffffu, low_max, o));
     }
+    // The same of the whole unit: the tiles that its warps go through together.
+    const int reach = (int)max(-1LL, min(pos0 + (unit_row0 + unit_rows - 1) / G, (long long)q.len - 1));
+    const long long under = a.window > 0 ? pos0 + unit_row0 / G - a.window + 1 : 0;  // its first visible token
+    const int t_first = max(t0, (int)(max(0LL, min(under, (long long)q.len)) / TT) - q.tile0);
+    const int t_end = min(t1, reach / TT + (reach >= 0) - q.tile0);
+
+    // A group of rw warps shares the tiles t_first + wt, + tw, ..., and copies
+    // each together while it works on the one before. page[h] is the page of
+    // the copied tile's tokens 16h.. (one page from 32 tokens on). A page
+    // outside the cache is left out: page 0 is copied in its place, and masked.
+    char *ring = sm + wt * 2 * Shape::TILE;
+    const int *table = a.table + (int64_t)req * a.max_blocks;
+    int page[2];
+    float ks = 0.0f, vs = 0.0f;  // scales of the next tile, of the page of this lane's tokens
+    bool live = false;
+    auto usable = [&](int p) { return p >= 0 && p < a.c.blocks; };
+    auto look_up = [&](int t) {
+      page[0] = page[1] = -1;
+      if (t < t_end) {
+        const int tok = (q.tile0 + t) * TT;
+        page[0] = __ldg(table + (tok >> lb));
+        page[1] = lb >= 5 ? page[0] : tok + 16 <= reach ? __ldg(table + (tok >> lb) + 1) : -1;
+        if (!usable(page[0]) || (tok + 16 <= reach && !usable(page[1]))) atomicExch(a.err, DEV_ERR_RANGE);
+      }
+    };
+    auto copy_tile = [&](int t, int stage) {  // page[] is the tile's
+      if (t < t_end) {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + stage * Shape::TILE);
+        const int tok = (q.tile0 + t) * TT, in_page = tok & ((1 << lb) - 1);
+        const int64_t unit = (int64_t)HS << lb;
+        const int64_t p0 = usable(page[0]) ? ((int64_t)page[0] * H + head) * unit : 0;
+        const int64_t p1 = usable(page[1]) ? ((int64_t)page[1] * H + head) * unit : 0;
+        const int8_t *k0 = a.c.k + p0 + (int64_t)in_page * HS, *k1 = lb >= 5 ? k0 + 16 * HS : a.c.k + p1;
+        const int8_t *v0 = a.c.v + (lane & 1 ? (lb >= 5 ? p0 + in_page + 16 : p1) : p0 + in_page) + ((int64_t)(lane >> 1) << lb);
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+          if (rw > 1 && i % rw != wr) continue;
+          const int at = 16 * (32 * i + lane);  // of the tile's keys
+          const int row = at / HS;
+          copy16(dst + (at ^ key_swizzle<HS>(row)), (at < 16 * HS ? k0 : k1 - 16 * HS) + at);
+          copy16(dst + Shape::KBYTES + at, v0 + ((int64_t)(16 * i) << lb));
+        }
+      }
+      copy_commit();
+    };
+    auto load_scales = [&](int t) {
+      const int p = page[r >> 2];
+      live = t < t_end && usable(p);
+      const int64_t ph = live ? (int64_t)p * H + head : 0;
+      ks = live ? __ldg(a.c.k_scale + ph) : 0.0f;
+      vs = live ? __ldg(a.c.v_scale + ph) : 0.0f;
+    };
+    int t = t_first + wt;
+    look_up(t);
+    load_scales(t);
+    copy_tile(t, 0);
+    look_up(t + tw);
 
     // Query fragments.
-    uint32_t qa[KS][4];
+    uint32_t qb[NT][TERMS][KS][2];
+    float f[NT][2];
 #pragma unroll
-    for (int j = 0; j < (SPLIT ? 1 : 2); j++) {
-      const int row = row0 + r + 8 * j;
+    for (int n = 0; n < NT; n++) {
+      const int row = row0 + 8 * n + r;
       const bool have = row < all_rows;
       const int64_t qi = have ? (int64_t)(q.q0 + row / G) * a.q_stride + (int64_t)(head * G + row % G) * HS : 0;
-      float top = 0.0f;
+      float top = 0.0f, v[KS][4];
       bool wrong = false;
 #pragma unroll
       for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-          const float v = have ? fabsf(q_load(a.q, type, qi + dim_of<HS>(s, c, b))) : 0.0f;
-          top = fmaxf(top, v);
-          wrong |= !(v < INFINITY);
+          v[s][b] = have ? q_load(a.q, type, qi + dim_of<HS>(s, c, b)) : 0.0f;
+          top = fmaxf(top, fabsf(v[s][b]));
+          wrong |= !(fabsf(v[s][b]) < INFINITY);
         }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -306,263 +397,209 @@ __global__ void __launch_bounds__(kA8Threads, A8Shape<HS>::CTAS) k_attn8(Attn8Ar
       int e = top > 0.0f && !wrong ? int(f2u(top) >> 23) - 127 - 13 : 0;
       e = max(e, -112);
       const float down = u2f(uint32_t(127 - e) << 23);
-      f[j] = wrong ? u2f(kCanonNaN) : u2f(uint32_t(127 + e) << 23) * (a.scale * 1.44269504088896f);
+      const float fr = wrong ? u2f(kCanonNaN) : u2f(uint32_t(127 + e) << 23) * (a.scale * 1.44269504088896f);
+      f[n][0] = __shfl_sync(0xffffffffu, fr, 8 * c);
+      f[n][1] = __shfl_sync(0xffffffffu, fr, 8 * c + 4);
 #pragma unroll
       for (int s = 0; s < KS; s++) {
-        float v[4];
 #pragma unroll
-        for (int b = 0; b < 4; b++)
-          v[b] = have && !wrong ? q_load(a.q, type, qi + dim_of<HS>(s, c, b)) * down : 0.0f;
-        qa[s][j] = pack_h2(v[0], v[1]);
-        qa[s][2 + j] = pack_h2(v[2], v[3]);
-        if constexpr (SPLIT) {
-          qa[s][1] = pack_rest(v[0], v[1], qa[s][0]);
-          qa[s][3] = pack_rest(v[2], v[3], qa[s][2]);
+        for (int b = 0; b < 4; b++) v[s][b] = wrong ? 0.0f : v[s][b] * down;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          qb[n][0][s][h] = pack_h2(v[s][2 * h], v[s][2 * h + 1]);
+          if constexpr (TERMS == 2) qb[n][1][s][h] = pack_rest(v[s][2 * h], v[s][2 * h + 1], qb[n][0][s][h]);
         }
       }
     }
-    if (SPLIT) f[1] = f[0];
 
-    float o[ND][4], m[2] = {-INFINITY, -INFINITY}, M[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float o[NT][ND / 2][4], m[NT][2], M[NT][2], l[NT][2];
 #pragma unroll
-    for (int d = 0; d < ND; d++) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
-
-    // One tile: where its halves lie, and their scales.
-    const int *table = a.table + (int64_t)req * a.max_blocks;
-    int64_t ph[NH];
-    uint32_t kw[NH][2][KS], vw[NH][ND];
-    float ks[NH], vs[NH];
-    bool live[NH];
-    auto place = [&](int t) {
+    for (int n = 0; n < NT; n++) {
 #pragma unroll
-      for (int s = 0; s < NH; s++) {
-        if (WIDE && s > 0) {
-          ph[s] = ph[0];
-          live[s] = live[0];
-          continue;
-        }
-        const int tok = (q.tile0 + t) * TT + 16 * s;
-        int page = tok <= high_max ? __ldg(table + tok / B) : -1;
-        live[s] = page >= 0 && page < a.c.blocks;
-        if (tok <= high_max && !live[s]) atomicExch(a.err, DEV_ERR_RANGE);
-        ph[s] = live[s] ? (int64_t)page * H + head : 0;
-      }
-    };
-    auto load_k = [&](int t) {
-#pragma unroll
-      for (int s = 0; s < NH; s++) {
-        const int o0 = ((q.tile0 + t) * TT + (WIDE ? 0 : 16 * s)) % B;
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const int tok = o0 + (WIDE ? 8 * (r >> 1) + 4 * s : 4 * (r >> 1)) + 2 * j + (r & 1);
-          load_row<HS>(a.c.k + (ph[s] * B + tok) * HS, c, kw[s][j]);
-        }
-        ks[s] = live[s] ? __ldg(a.c.k_scale + ph[s]) : 0.0f;
-        vs[s] = live[s] ? __ldg(a.c.v_scale + ph[s]) : 0.0f;
-      }
-    };
-    auto load_v = [&](int t) {
-      if constexpr (WIDE) {
-        const int8_t *v = a.c.v + (ph[0] * HS + r) * B + ((q.tile0 + t) * TT) % B + 8 * c;
-#pragma unroll
-        for (int d = 0; d < ND; d++) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2 *>(v + (int64_t)8 * d * B));
-          vw[0][d] = w.x;
-          vw[1][d] = w.y;
-        }
-      } else {
-#pragma unroll
-        for (int s = 0; s < NH; s++) {
-          const int8_t *v = a.c.v + (ph[s] * HS + r) * B + ((q.tile0 + t) * TT + 16 * s) % B + 4 * c;
-#pragma unroll
-          for (int d = 0; d < ND; d++) vw[s][d] = __ldg(reinterpret_cast<const uint32_t *>(v + (int64_t)8 * d * B));
-        }
-      }
-    };
-    auto in_reach = [&](int t) {  // of any row of the warp
-      return t < t1 && (q.tile0 + t) * TT <= high_max;
-    };
-
-    int t = t0 + wt;
-    if (in_reach(t)) {
-      place(t);
-      load_k(t);
-      load_v(t);
+      for (int d = 0; d < ND / 2; d++) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.0f;
+      m[n][0] = m[n][1] = M[n][0] = M[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
     }
-    for (; in_reach(t); t += tw) {
+    for (int it = 0; t < t_end; t += tw, it ^= 1) {
+      copy_wait<0>();
+      if (rw == 1) __syncwarp();
+      else asm volatile("bar.sync %0, %1;" ::"r"(1 + wt), "r"(32 * rw) : "memory");
+      const float cks = ks, cvs = vs;
+      const bool clive = live;
+      load_scales(t + tw);
+      copy_tile(t + tw, it ^ 1);
+      look_up(t + 2 * tw);
       const int tok0 = (q.tile0 + t) * TT;
-      float sc[NH][2][4];
-#pragma unroll
-      for (int s = 0; s < NH; s++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          sc[s][j][0] = sc[s][j][1] = sc[s][j][2] = sc[s][j][3] = 0.0f;
-#pragma unroll
-          for (int k = 0; k < KS; k++) {
-            uint32_t b0, b1;
-            i8_to_h2(kw[s][j][k], b0, b1);
-            mma16816(sc[s][j], qa[k], b0, b1);
-          }
-        }
-      float cks[NH], cvs[NH];
-      bool whole = tok0 + TT - 1 <= high_min && tok0 > low_max, clive[NH];
-#pragma unroll
-      for (int s = 0; s < NH; s++) {
-        cks[s] = ks[s];
-        cvs[s] = vs[s];
-        clive[s] = live[s];
-        whole &= live[s];
-      }
-      const bool more = in_reach(t + tw);
-      if (more) {
-        place(t + tw);
-        load_k(t + tw);
-      }
+      if (tok0 > high_max) continue;  // in reach of other warps' rows only
 
-      // Scores in powers of two, their maxima, and the tile's weights.
-      float mx[NH][2];
+      const char *kt = ring + it * Shape::TILE, *vt = kt + Shape::KBYTES;
+      float sc[2][NT][4];
 #pragma unroll
-      for (int s = 0; s < NH; s++) {
-        const float f0 = f[0] * cks[s], f1 = f[1] * cks[s];
+      for (int s = 0; s < 2; s++) {
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          if constexpr (SPLIT) {
-            sc[s][j][0] = (sc[s][j][0] + sc[s][j][2]) * f0;
-            sc[s][j][1] = (sc[s][j][1] + sc[s][j][3]) * f0;
-          } else {
-            sc[s][j][0] *= f0;
-            sc[s][j][1] *= f0;
-            sc[s][j][2] *= f1;
-            sc[s][j][3] *= f1;
-          }
+        for (int n = 0; n < NT; n++) sc[s][n][0] = sc[s][n][1] = sc[s][n][2] = sc[s][n][3] = 0.0f;
+        // Token of row r (and r + 8) of the 16: 8 (r/2) + 4s + r%2 (and + 2).
+        uint32_t kw[2][KS];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          load_row<HS>(kt + (8 * (r >> 1) + 4 * s + 2 * j + (r & 1)) * HS, key_swizzle<HS>(r), c, kw[j]);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          uint32_t ka[4];
+          i8_to_h2(kw[0][k], ka[0], ka[2]);
+          i8_to_h2(kw[1][k], ka[1], ka[3]);
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int x = TERMS - 1; x >= 0; x--) mma16816(sc[s][n], ka, qb[n][x][k][0], qb[n][x][k][1]);
+        }
+      }
+      // vs = vf · 2^ve; a scale of zero: weights of zero.
+      const int ex = max(int(f2u(cvs) >> 23) - 127, -126);
+      const float ve = cvs > 0.0f ? (float)ex : -1e30f;
+      const float vf = cvs * u2f(uint32_t(127 - min(ex, 126)) << 23) * (ex > 126 ? 0.5f : 1.0f);
+      const bool whole = __all_sync(0xffffffffu, clive) && tok0 + TT - 1 <= high_min && tok0 > low_max;
+
+      // Scores in powers of two. m and M are references that stay while no
+      // score passes them by much, so that most tiles need no exchange
+      // between lanes.
+      bool grew = false;
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const float f0 = f[n][0] * cks, f1 = f[n][1] * cks;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          sc[s][n][0] *= f0;
+          sc[s][n][1] *= f1;
+          sc[s][n][2] *= f0;
+          sc[s][n][3] *= f1;
           if (!whole) {
-            const int tok = tok0 + (WIDE ? 8 * c + 4 * s : 16 * s + 4 * c) + 2 * j;
+            const int tok = tok0 + 8 * (r >> 1) + 4 * s + (r & 1);
 #pragma unroll
-            for (int e = 0; e < (SPLIT ? 2 : 4); e++) {
-              const int k = tok + (e & 1);
-              if (!clive[s] || k > high[e >> 1] || k <= low[e >> 1]) sc[s][j][e] = -INFINITY;
+            for (int x = 0; x < 4; x++) {
+              const int k = tok + (x & 2);
+              if (!clive || k > high[n][x & 1] || k <= low[n][x & 1]) sc[s][n][x] = -INFINITY;
             }
           }
         }
-        mx[s][0] = fmaxf(fmaxf(sc[s][0][0], sc[s][0][1]), fmaxf(sc[s][1][0], sc[s][1][1]));
-        mx[s][1] = SPLIT ? mx[s][0] : fmaxf(fmaxf(sc[s][0][2], sc[s][0][3]), fmaxf(sc[s][1][2], sc[s][1][3]));
-      }
-      if (WIDE && NH == 2) {
-        mx[0][0] = mx[NH - 1][0] = fmaxf(mx[0][0], mx[NH - 1][0]);
-        mx[0][1] = mx[NH - 1][1] = fmaxf(mx[0][1], mx[NH - 1][1]);
-      }
 #pragma unroll
-      for (int s = 0; s < (WIDE ? 1 : NH); s++)
-#pragma unroll
-        for (int j = 0; j < (SPLIT ? 1 : 2); j++) {
-          mx[s][j] = fmaxf(mx[s][j], __shfl_xor_sync(0xffffffffu, mx[s][j], 1));
-          mx[s][j] = fmaxf(mx[s][j], __shfl_xor_sync(0xffffffffu, mx[s][j], 2));
+        for (int e = 0; e < 2; e++) {
+          const float mx = fmaxf(fmaxf(sc[0][n][e], sc[0][n][2 + e]), fmaxf(sc[1][n][e], sc[1][n][2 + e]));
+          grew |= mx > m[n][e] + 20.0f || mx + ve > M[n][e];
         }
-      // vs = vf · 2^ve.
-      float ve[NH], vf[NH];
-#pragma unroll
-      for (int s = 0; s < NH; s++) {
-        const int e = max(int(f2u(cvs[s]) >> 23) - 127, -126);
-        ve[s] = cvs[s] > 0.0f ? (float)e : -1e30f;  // a scale of zero: weights of zero
-        vf[s] = cvs[s] * u2f(uint32_t(127 - min(e, 126)) << 23) * (e > 126 ? 0.5f : 1.0f);
       }
-      float ms[2], Ms[2], top[2];
-      bool grew = false;
-#pragma unroll
-      for (int j = 0; j < (SPLIT ? 1 : 2); j++) {
-        float mn = m[j], Mn = M[j];
-#pragma unroll
-        for (int s = 0; s < (WIDE ? 1 : NH); s++) {
-          mn = fmaxf(mn, mx[s][j]);
-          if (cvs[s] > 0.0f) Mn = fmaxf(Mn, mx[s][j] + (ve[s] + 1.0f));
-        }
-        ms[j] = mn == -INFINITY ? 0.0f : mn;
-        Ms[j] = Mn == -INFINITY ? 0.0f : Mn;
-        top[j] = Mn;
-        l[j] *= ex2(m[j] - ms[j]);
-        grew |= Mn > M[j];
-        m[j] = mn;
-      }
-      if (SPLIT) ms[1] = ms[0], Ms[1] = Ms[0], top[1] = top[0];
       if (__any_sync(0xffffffffu, grew)) {
-        const float g0 = ex2(M[0] - Ms[0]), g1 = SPLIT ? g0 : ex2(M[1] - Ms[1]);
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-          o[d][0] *= g0;
-          o[d][1] *= g0;
-          o[d][2] *= g1;
-          o[d][3] *= g1;
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float mn = fmaxf(fmaxf(sc[0][n][e], sc[0][n][2 + e]), fmaxf(sc[1][n][e], sc[1][n][2 + e]));
+            float Mn = ve > -1e29f ? mn + (ve + 1.0f) : -INFINITY;
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+              mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
+              Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, x));
+            }
+            mn = fmaxf(mn, m[n][e]);
+            Mn = fmaxf(Mn, M[n][e]);
+            l[n][e] *= ex2(m[n][e] - (mn == -INFINITY ? 0.0f : mn));
+            const float g = ex2(M[n][e] - (Mn == -INFINITY ? 0.0f : Mn));
+#pragma unroll
+            for (int d = 0; d < ND / 2; d++) {
+              o[n][d][e] *= g;
+              o[n][d][2 + e] *= g;
+            }
+            m[n][e] = mn;
+            M[n][e] = Mn;
+          }
+      }
+      uint32_t pb[2][NT][TERMS][2];
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float ms[2], kap[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          ms[e] = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+          kap[e] = ex2(fminf(ms[e] - (M[n][e] == -INFINITY ? 0.0f : M[n][e]) + 14.0f + ve, 120.0f)) * vf;
         }
 #pragma unroll
-        for (int j = 0; j < 2; j++) M[j] = top[j];
-      }
-#pragma unroll
-      for (int s = 0; s < NH; s++) {
-        uint32_t pa[4];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
+        for (int s = 0; s < 2; s++) {
           float w[4];
 #pragma unroll
-          for (int e = 0; e < (SPLIT ? 2 : 4); e++) {
-            const float v = sc[s][j][e];
-            l[e >> 1] += ex2(v - ms[e >> 1]);
-            w[e] = ex2(v + (ve[s] + 14.0f - Ms[e >> 1])) * vf[s];
+          for (int x = 0; x < 4; x++) {
+            const float p = ex2(sc[s][n][x] - ms[x & 1]);
+            l[n][x & 1] += p;
+            w[x] = p * kap[x & 1];
           }
-          pa[2 * j] = pack_h2(w[0], w[1]);
-          pa[2 * j + 1] = SPLIT ? pack_rest(w[0], w[1], pa[2 * j]) : pack_h2(w[2], w[3]);
-        }
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-          uint32_t b0, b1;
-          i8_to_h2(vw[s][d], b0, b1);
-          mma16816(o[d], pa, b0, b1);
+          for (int j = 0; j < 2; j++) {
+            const uint32_t h = pack_h2(w[2 * j], w[2 * j + 1]);
+            pb[s][n][0][j] = transpose_h2(h);
+            if constexpr (TERMS == 2) pb[s][n][1][j] = transpose_h2(pack_rest(w[2 * j], w[2 * j + 1], h));
+          }
         }
       }
-      if (more) load_v(t + tw);
+#pragma unroll
+      for (int d = 0; d < ND / 2; d++) {
+        // Tokens 8c .. 8c + 7 of two dimensions.
+        const uint2 v0 = *reinterpret_cast<const uint2 *>(vt + (16 * d + r) * TT + 8 * c);
+        const uint2 v1 = *reinterpret_cast<const uint2 *>(vt + (16 * d + 8 + r) * TT + 8 * c);
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          uint32_t va[4];
+          i8_to_h2(s ? v0.y : v0.x, va[0], va[2]);
+          i8_to_h2(s ? v1.y : v1.x, va[1], va[3]);
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int x = TERMS - 1; x >= 0; x--) mma16816(o[n][d], va, pb[s][n][x][0], pb[s][n][x][1]);
+        }
+      }
     }
+    copy_wait<0>();
 
     // The warps' sums meet in shared memory.
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
-      l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
-    }
-    __syncthreads();  // the last unit's readers are done
-    float *so = s_o + warp * 16 * PITCH, *st = s_st + warp * 64;
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int d = 0; d < ND; d++) {
-      if constexpr (SPLIT) {
-        *reinterpret_cast<float2 *>(so + r * PITCH + 8 * d + 2 * c) = make_float2(o[d][0] + o[d][2], o[d][1] + o[d][3]);
-      } else {
-        *reinterpret_cast<float2 *>(so + r * PITCH + 8 * d + 2 * c) = make_float2(o[d][0], o[d][1]);
-        *reinterpret_cast<float2 *>(so + (r + 8) * PITCH + 8 * d + 2 * c) = make_float2(o[d][2], o[d][3]);
-      }
-    }
-    if (c == 0) {
+      for (int e = 0; e < 2; e++)
 #pragma unroll
-      for (int j = 0; j < (SPLIT ? 1 : 2); j++) {
-        st[4 * (r + 8 * j)] = m[j];
-        st[4 * (r + 8 * j) + 1] = M[j];
-        st[4 * (r + 8 * j) + 2] = l[j];
+        for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+    __syncthreads();  // the rings are free
+    float *so = s_o + warp * R * PITCH, *st = s_st + warp * R * 4;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float *row = so + (8 * n + 2 * c + e) * PITCH + r;
+#pragma unroll
+        for (int d = 0; d < ND / 2; d++) {
+          row[16 * d] = o[n][d][e];
+          row[16 * d + 8] = o[n][d][2 + e];
+        }
+        if (r == 0) {
+          float *x = st + 4 * (8 * n + 2 * c + e);
+          x[0] = m[n][e];
+          x[1] = M[n][e];
+          x[2] = l[n][e];
+        }
       }
-    }
     __syncthreads();
-    const bool starts = at == u0, ends = u1 <= end;
+    const bool starts = by_unit || at == u0, ends = by_unit || u1 <= end;
     float *part = parts + (2LL * blockIdx.x + (starts ? 1 : 0)) * a8_part_floats(HS);
-    const int unit_row0 = rg * rw * R, unit_rows = min(rw * R, all_rows - unit_row0);
     for (int row = warp; row < unit_rows; row += kA8Warps) {
       const int tile = row / R, rr = row % R;
       float mm = -INFINITY, MM = -INFINITY;
       for (int w = 0; w < tw; w++) {
-        mm = fmaxf(mm, s_st[(tile + w * rw) * 64 + 4 * rr]);
-        MM = fmaxf(MM, s_st[(tile + w * rw) * 64 + 4 * rr + 1]);
+        mm = fmaxf(mm, s_st[((tile + w * rw) * R + rr) * 4]);
+        MM = fmaxf(MM, s_st[((tile + w * rw) * R + rr) * 4 + 1]);
       }
       const float msafe = mm == -INFINITY ? 0.0f : mm, Msafe = MM == -INFINITY ? 0.0f : MM;
       float ll = 0.0f, g[kA8Warps];
 #pragma unroll
       for (int w = 0; w < kA8Warps; w++) {
         if (w >= tw) break;
-        const float *s = s_st + (tile + w * rw) * 64 + 4 * rr;
+        const float *s = s_st + ((tile + w * rw) * R + rr) * 4;
         ll += s[2] * exp2f(s[0] - msafe);
         g[w] = exp2f(s[1] - Msafe);
       }
@@ -574,7 +611,7 @@ __global__ void __launch_bounds__(kA8Threads, A8Shape<HS>::CTAS) k_attn8(Attn8Ar
 #pragma unroll
         for (int w = 0; w < kA8Warps; w++) {
           if (w >= tw) break;
-          v = fmaf(s_o[(tile + w * rw) * 16 * PITCH + rr * PITCH + d], g[w], v);
+          v = fmaf(s_o[((tile + w * rw) * R + rr) * PITCH + d], g[w], v);
         }
         if (starts && ends) o_store(a.out, type, oi + d, v * scale);
         else part[row * HS + d] = v;
@@ -586,7 +623,7 @@ __global__ void __launch_bounds__(kA8Threads, A8Shape<HS>::CTAS) k_attn8(Attn8Ar
         s[2] = ll;
       }
     }
-    if (at == begin && tid == 0) {
+    if (at == begin && tid == 0 && !by_unit) {
       A8Record rec;
       rec.first = starts ? -1 : (int)(u0 / per);
       rec.last = (int)((u1 - 1) / per);
@@ -599,12 +636,13 @@ __global__ void __launch_bounds__(kA8Threads, A8Shape<HS>::CTAS) k_attn8(Attn8Ar
       records[blockIdx.x] = rec;
     }
     at = min(end, u1);
+    __syncthreads();  // the merge buffers are free
   }
 }
 
-// The instances for one of the two query forms (each in a file of its own,
+// The instances for one number of float16 terms (each in a file of its own,
 // to be compiled side by side).
-template <bool SPLIT>
+template <int TERMS>
 struct A8 {
   template <class F>
   static cudaError_t at(int hs, F f) {
@@ -621,30 +659,30 @@ struct A8 {
     }
     return cudaErrorInvalidValue;
   }
+  // Two tiles of 8 rows a warp where the registers allow it: one term, heads
+  // up to 128.
   template <int HS>
-  static constexpr int smem() { return kA8Warps * 16 * (A8Shape<HS>::PITCH + 4) * 4; }
-
+  static constexpr bool two_tiles() { return TERMS == 1 && HS <= 128; }
   struct Init {
     template <int HS>
     cudaError_t operator()() const {
-      cudaError_t e = cudaFuncSetAttribute(k_attn8<HS, SPLIT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem<HS>());
-      if constexpr (A8Shape<HS>::TT == 32)
+      cudaError_t e = cudaFuncSetAttribute(k_attn8<HS, TERMS, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8Shape<HS>::RING);
+      if constexpr (two_tiles<HS>())
         if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(k_attn8<HS, SPLIT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem<HS>());
+          e = cudaFuncSetAttribute(k_attn8<HS, TERMS, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8Shape<HS>::RING);
       return e;
     }
   };
   struct Launch {
     const Attn8Args &a;
-    int type;
+    int type, nt;
     A8Grid g;
     cudaStream_t st;
     template <int HS>
     cudaError_t operator()() const {
-      if constexpr (A8Shape<HS>::TT == 32)
-        if (a.c.block >= 32)
-          return launch_k(k_attn8<HS, SPLIT, true>, g.ctas, kA8Threads, smem<HS>(), st, a, type, g);
-      return launch_k(k_attn8<HS, SPLIT, false>, g.ctas, kA8Threads, smem<HS>(), st, a, type, g);
+      if constexpr (two_tiles<HS>())
+        if (nt == 2) return launch_k(k_attn8<HS, TERMS, 2>, g.ctas, kA8Threads, A8Shape<HS>::RING, st, a, type, g);
+      return launch_k(k_attn8<HS, TERMS, 1>, g.ctas, kA8Threads, A8Shape<HS>::RING, st, a, type, g);
     }
   };
   static cudaError_t init() {
@@ -655,7 +693,7 @@ struct A8 {
   }
 };
 
-cudaError_t attn8_init_f32();
-cudaError_t attn8_main_f32(const Attn8Args &a, int type, A8Grid g, cudaStream_t st);
+cudaError_t attn8_init_two();
+cudaError_t attn8_main_two(const Attn8Args &a, int type, A8Grid g, cudaStream_t st);
 
 }  // namespace rk
