@@ -555,10 +555,11 @@ int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const voi
  * A query that sees no token gives zeros; one with a NaN or infinity gives
  * NaN. q and out are [tokens][heads][head_size] of `type`, rows q_stride and
  * out_stride elements apart; rows of no request are neither read nor
- * written. Scores, sums and weighted values are held in float32; the keys
- * and values enter exactly, the queries and softmax weights as float16
- * (a query scaled by a power of two first), in one term for 16-bit types
- * and in two (22 bits) for float32.
+ * written. Scores, sums and weighted values are held in float32, keys and
+ * values enter exactly. A row of queries enters as integers of 16 bits
+ * (float32: 24) of its largest magnitude, a softmax weight as float16
+ * (float32: as two, 22 bits); weights below 2^-126 of the largest count as
+ * zero.
  * workspace: rk_kv8_attention_workspace() bytes, 16-byte aligned, used during the
  * call's kernels only; calls that may run at once need one each. */
 int64_t rk_kv8_attention_workspace(rk_device *d, const rk_kv8 *c, int heads);

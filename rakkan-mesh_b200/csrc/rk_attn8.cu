@@ -4,25 +4,26 @@
 
 namespace rk {
 
-// Joins the parts of the unit that crosses into CTA blockIdx.x + 1: the CTAs
-// it crosses into share its rows.
-constexpr int kJoinThreads = 128, kJoinParts = 256;
+// Joins the parts of the unit that crosses into CTA blockIdx.x + 1. The CTAs
+// that a unit crosses into share its rows, a warp each; a warp's lanes weigh
+// 32 parts at once and then add them up, four dimensions a lane.
+constexpr int kJoinWarps = 4;
 
-__global__ void __launch_bounds__(kJoinThreads) k_attn8_join(Attn8Args a, int type, A8Grid grid) {
-  __shared__ float s_g[kJoinParts];
-  __shared__ float s_red[2][kJoinThreads / 32];
+__global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int type, A8Grid grid) {
   griddep_wait();
   const A8Record *records = static_cast<const A8Record *>(a.ws);
   const float *parts = reinterpret_cast<const float *>(records + grid.ctas);
-  const int b = blockIdx.x + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const A8Record rec = records[b];
   if (rec.first < 0) return;
   const int hs = a.c.head_size, G = a.heads / a.c.kv_heads, n = rec.last - rec.first + 1;
   const int64_t size = a8_part_floats(hs);
-  auto part_of = [&](int i) { return parts + (2LL * (rec.first + i) + (i == 0 ? 1 : 0)) * size; };
-  for (int row = b - rec.first - 1; row < rec.rows; row += n - 1) {
-    float mm = -INFINITY, MM = -INFINITY;
-    for (int i = tid; i < n; i += kJoinThreads) {
+  // Part i is CTA first + i's: its second slot where the unit begins, else its first.
+  const float *p0 = parts + 2LL * rec.first * size;
+  auto part_of = [&](int i) { return p0 + (2LL * i + (i == 0)) * size; };
+  for (int row = (b - rec.first - 1) * kJoinWarps + warp; row < rec.rows; row += (n - 1) * kJoinWarps) {
+    float mm = -INFINITY, MM = -INFINITY, ll = 0.0f;
+    for (int i = lane; i < n; i += 32) {
       const float *s = part_of(i) + 64 * hs + 4 * row;
       mm = fmaxf(mm, s[0]);
       MM = fmaxf(MM, s[1]);
@@ -32,47 +33,46 @@ __global__ void __launch_bounds__(kJoinThreads) k_attn8_join(Attn8Args a, int ty
       mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
       MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, o));
     }
-    __syncthreads();
-    if (lane == 0) {
-      s_red[0][warp] = mm;
-      s_red[1][warp] = MM;
-    }
-    __syncthreads();
-    for (int w = 0; w < kJoinThreads / 32; w++) {
-      mm = fmaxf(mm, s_red[0][w]);
-      MM = fmaxf(MM, s_red[1][w]);
-    }
     const float msafe = mm == -INFINITY ? 0.0f : mm, Msafe = MM == -INFINITY ? 0.0f : MM;
-    float ll = 0.0f, v0 = 0.0f, v1 = 0.0f;  // dimensions tid and tid + 128
-    for (int i0 = 0; i0 < n; i0 += kJoinParts) {
-      const int k = min(kJoinParts, n - i0);
-      __syncthreads();
-      for (int i = tid; i < k; i += kJoinThreads) {
-        const float *s = part_of(i0 + i) + 64 * hs + 4 * row;
-        s_g[i] = exp2f(s[1] - Msafe);
+    float4 v[2] = {};
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int k = min(32, n - i0);
+      float g = 0.0f;
+      if (lane < k) {
+        const float *s = part_of(i0 + lane) + 64 * hs + 4 * row;
+        g = exp2f(s[1] - Msafe);
         ll += s[2] * exp2f(s[0] - msafe);
       }
-      __syncthreads();
-      if (tid < hs) {
 #pragma unroll 8
-        for (int i = 0; i < k; i++) v0 = fmaf(part_of(i0 + i)[row * hs + tid], s_g[i], v0);
-        if (hs > kJoinThreads)
-#pragma unroll 8
-          for (int i = 0; i < k; i++) v1 = fmaf(part_of(i0 + i)[row * hs + tid + kJoinThreads], s_g[i], v1);
+      for (int i = 0; i < k; i++) {
+        const float w = __shfl_sync(0xffffffffu, g, i);
+        const float *p = part_of(i0 + i) + row * hs;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int d = 4 * lane + 128 * j;
+          if (d >= hs) break;
+          const float4 x = *reinterpret_cast<const float4 *>(p + d);
+          v[j].x = fmaf(x.x, w, v[j].x);
+          v[j].y = fmaf(x.y, w, v[j].y);
+          v[j].z = fmaf(x.z, w, v[j].z);
+          v[j].w = fmaf(x.w, w, v[j].w);
+        }
       }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
-    __syncthreads();
-    if (lane == 0) s_red[0][warp] = ll;
-    __syncthreads();
-    ll = 0.0f;
-    for (int w = 0; w < kJoinThreads / 32; w++) ll += s_red[0][w];
     const float scale = ll == 0.0f ? 0.0f : exp2f(Msafe - 14.0f - msafe) / ll;
     const int qrow = rec.row0 + row;
     const int64_t oi = (int64_t)(rec.q0 + qrow / G) * a.out_stride + (int64_t)(rec.head * G + qrow % G) * hs;
-    if (tid < hs) o_store(a.out, type, oi + tid, v0 * scale);
-    if (tid + kJoinThreads < hs) o_store(a.out, type, oi + tid + kJoinThreads, v1 * scale);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int d = 4 * lane + 128 * j;
+      if (d >= hs) break;
+      o_store(a.out, type, oi + d, v[j].x * scale);
+      o_store(a.out, type, oi + d + 1, v[j].y * scale);
+      o_store(a.out, type, oi + d + 2, v[j].z * scale);
+      o_store(a.out, type, oi + d + 3, v[j].w * scale);
+    }
   }
 }
 
@@ -102,7 +102,7 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   // for them before it reads.
   const bool pdl = g_pdl;
   g_pdl = true;
-  e = launch_k(k_attn8_join, g.ctas - 1, kJoinThreads, 0, st, a, type, g);
+  e = launch_k(k_attn8_join, g.ctas - 1, 32 * kJoinWarps, 0, st, a, type, g);
   g_pdl = pdl;
   return e;
 }

@@ -19,19 +19,22 @@
 // (r, c) = (lane / 4, lane % 4) holds terms {2c, 2c+1, 2c+8, 2c+9} of a step;
 // they are given to four neighbouring bytes, so that a lane's bytes of
 // several steps are one 16-, 8- or 4-byte load: of a key row, dimensions; of a
-// transposed value row, tokens. The scores come out as (token, query); a
+// transposed value row, tokens. (A step of bytes is 32 long: two such groups.) The scores come out as (token, query); a
 // transposing move of 8x8 registers makes them the second product's column
 // operand, which fixes the token of each key row.
 //
-// Precision. A float32 row of queries is scaled by a power of two to a
-// largest magnitude near 2^13 and split into two float16 terms (22 bits);
-// 16-bit queries are one exact term. The softmax weights likewise, with the
-// value scale in the weight: w_t = 2^(s_t - M + E + 14) f for vs = f 2^E, M
-// within a power of two of the running maximum of s_t + E + 1 and so
-// w_t < 2^16. The denominator has a reference of its own (m), so that pages
-// of any two scales are weighed rightly. 16-bit types round a weight once to
-// float16 (2^-12 of itself, an eighth of bfloat16's own rounding of the
-// result, and half of float16's on average over tokens).
+// Precision. The scores' product is mma.m16n8k32 on signed bytes: the keys
+// as they are, a row of queries as integers of two signed bytes (16-bit types,
+// the row's largest at 32639: off by at most 2^-16 of it) or three (float32,
+// 2^-24), each its own exact product, joined in float32. (float16 products
+// would want the keys converted, 160 of some 900 instructions a tile.) The
+// softmax weights are float16, one term for 16-bit types (2^-12 of itself:
+// an eighth of bfloat16's own rounding of the result, and half of float16's
+// on average over tokens) and two for float32 (22 bits), with the value scale
+// in the weight: w_t = 2^(s_t - M + E + 14) f for vs = f 2^E, M within a power of two
+// of the running maximum of s_t + E + 1 and so w_t < 2^16. The denominator has
+// a reference of its own (m), so that pages of any two scales are weighed
+// rightly.
 //
 // Work. A unit is a request's kv head and up to four tiles of query rows; its
 // keys are cut into tiles of 32 tokens. The tiles of all units in a row are dealt out in equal runs, one to a CTA, so that lengths
@@ -102,6 +105,12 @@ RK_DEV void mma16816(float *c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
   asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+RK_DEV void mma16832(int *c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
@@ -213,6 +222,7 @@ template <int HS, int TERMS, int NT>
 __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(Attn8Args a, int type, A8Grid grid) {
   using Shape = A8Shape<HS>;
   constexpr int TT = kA8Tile, KS = Shape::KS, PITCH = Shape::PITCH, R = 8 * NT, ND = HS / 8;
+  constexpr int DIGITS = TERMS + 1;  // signed bytes of a query
   static_assert(kA8Warps * R * (PITCH + 4) * 4 <= Shape::RING, "the merge buffers fit the rings");
   extern __shared__ __align__(128) char sm[];
   // The rings; between two units, the merge buffers [warps][R][PITCH] and [warps][R][4].
@@ -326,6 +336,8 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     // outside the cache is left out: page 0 is copied in its place, and masked.
     char *ring = sm + wt * 2 * Shape::TILE;
     const int *table = a.table + (int64_t)req * a.max_blocks;
+    const uint32_t page_bytes = (uint32_t)(H * HS) << lb;
+    const int8_t *k_head = a.c.k + (((int64_t)head * HS) << lb), *v_head = a.c.v + (((int64_t)head * HS) << lb);
     int page[2];
     float ks = 0.0f, vs = 0.0f;  // scales of the next tile, of the page of this lane's tokens
     bool live = false;
@@ -343,18 +355,20 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       if (t < t_end) {
         const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + stage * Shape::TILE);
         const int tok = (q.tile0 + t) * TT, in_page = tok & ((1 << lb) - 1);
-        const int64_t unit = (int64_t)HS << lb;
-        const int64_t p0 = usable(page[0]) ? ((int64_t)page[0] * H + head) * unit : 0;
-        const int64_t p1 = usable(page[1]) ? ((int64_t)page[1] * H + head) * unit : 0;
-        const int8_t *k0 = a.c.k + p0 + (int64_t)in_page * HS, *k1 = lb >= 5 ? k0 + 16 * HS : a.c.k + p1;
-        const int8_t *v0 = a.c.v + (lane & 1 ? (lb >= 5 ? p0 + in_page + 16 : p1) : p0 + in_page) + ((int64_t)(lane >> 1) << lb);
+        const int64_t p0 = usable(page[0]) ? (int64_t)((uint64_t)(uint32_t)page[0] * page_bytes) : 0;
+        const int8_t *k0 = k_head + p0 + in_page * HS, *k1 = k0, *v0 = v_head + p0 + in_page + 16 * (lane & 1);
+        if (lb == 4) {
+          const int64_t p1 = usable(page[1]) ? (int64_t)((uint64_t)(uint32_t)page[1] * page_bytes) : 0;
+          k1 = k_head + p1 - 16 * HS;
+          if (lane & 1) v0 = v_head + p1;
+        }
+        v0 += (lane >> 1) << lb;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
-          if (rw > 1 && i % rw != wr) continue;
+          if ((i & (rw - 1)) != wr) continue;
           const int at = 16 * (32 * i + lane);  // of the tile's keys
-          const int row = at / HS;
-          copy16(dst + (at ^ key_swizzle<HS>(row)), (at < 16 * HS ? k0 : k1 - 16 * HS) + at);
-          copy16(dst + Shape::KBYTES + at, v0 + ((int64_t)(16 * i) << lb));
+          copy16(dst + (at ^ key_swizzle<HS>(at / HS)), ((KS % 2 ? at < 16 * HS : 2 * i < KS) ? k0 : k1) + at);
+          copy16(dst + Shape::KBYTES + at, v0 + ((16 * i) << lb));
         }
       }
       copy_commit();
@@ -373,7 +387,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     look_up(t + tw);
 
     // Query fragments.
-    uint32_t qb[NT][TERMS][KS][2];
+    uint32_t qb[NT][DIGITS][KS + KS % 2];
     float f[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -393,23 +407,28 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       wrong = (__ballot_sync(0xffffffffu, wrong) >> (lane & 28) & 15) != 0;
-      // 2^-e brings the row's largest magnitude into [2^13, 2^14).
-      int e = top > 0.0f && !wrong ? int(f2u(top) >> 23) - 127 - 13 : 0;
-      e = max(e, -112);
-      const float down = u2f(uint32_t(127 - e) << 23);
-      const float fr = wrong ? u2f(kCanonNaN) : u2f(uint32_t(127 + e) << 23) * (a.scale * 1.44269504088896f);
+      // The row as integers of DIGITS signed bytes, its largest at the top.
+      constexpr float LIMIT = DIGITS == 2 ? 127 * 257 : 127 * 65793;
+      top = fmaxf(top, u2f(27u << 23));  // 2^-100: the quotients stay finite
+      const float up = LIMIT / top;
+      const float fr = wrong ? u2f(kCanonNaN) : (top / LIMIT) * (a.scale * 1.44269504088896f);
       f[n][0] = __shfl_sync(0xffffffffu, fr, 8 * c);
       f[n][1] = __shfl_sync(0xffffffffu, fr, 8 * c + 4);
 #pragma unroll
       for (int s = 0; s < KS; s++) {
+        int w[4];
 #pragma unroll
-        for (int b = 0; b < 4; b++) v[s][b] = wrong ? 0.0f : v[s][b] * down;
+        for (int b = 0; b < 4; b++) w[b] = wrong ? 0 : __float2int_rn(fminf(LIMIT, fmaxf(-LIMIT, v[s][b] * up)));
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          qb[n][0][s][h] = pack_h2(v[s][2 * h], v[s][2 * h + 1]);
-          if constexpr (TERMS == 2) qb[n][1][s][h] = pack_rest(v[s][2 * h], v[s][2 * h + 1], qb[n][0][s][h]);
+        for (int x = DIGITS - 1; x >= 0; x--) {  // the lowest byte first, as a signed one; the rest is a multiple of 256
+          qb[n][x][s] = prmt(prmt(w[0], w[1], 0x0040), prmt(w[2], w[3], 0x0040), 0x5410);
+#pragma unroll
+          for (int b = 0; b < 4; b++) w[b] = (w[b] + 128) >> 8;
         }
       }
+      if (KS % 2)
+#pragma unroll
+        for (int x = 0; x < DIGITS; x++) qb[n][x][KS] = 0;
     }
 
     float o[NT][ND / 2][4], m[NT][2], M[NT][2], l[NT][2];
@@ -436,23 +455,29 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       float sc[2][NT][4];
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-#pragma unroll
-        for (int n = 0; n < NT; n++) sc[s][n][0] = sc[s][n][1] = sc[s][n][2] = sc[s][n][3] = 0.0f;
         // Token of row r (and r + 8) of the 16: 8 (r/2) + 4s + r%2 (and + 2).
-        uint32_t kw[2][KS];
+        uint32_t kw[2][KS + KS % 2];
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int j = 0; j < 2; j++) {
           load_row<HS>(kt + (8 * (r >> 1) + 4 * s + 2 * j + (r & 1)) * HS, key_swizzle<HS>(r), c, kw[j]);
+          if (KS % 2) kw[j][KS] = 0;
+        }
+        int si[DIGITS][NT][4] = {};
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-          uint32_t ka[4];
-          i8_to_h2(kw[0][k], ka[0], ka[2]);
-          i8_to_h2(kw[1][k], ka[1], ka[3]);
+        for (int k = 0; k < KS; k += 2) {
+          const uint32_t ka[4] = {kw[0][k], kw[1][k], kw[0][k + 1], kw[1][k + 1]};
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int x = TERMS - 1; x >= 0; x--) mma16816(sc[s][n], ka, qb[n][x][k][0], qb[n][x][k][1]);
+            for (int x = 0; x < DIGITS; x++) mma16832(si[x][n], ka, qb[n][x][k], qb[n][x][k + 1]);
         }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            if constexpr (DIGITS == 2) sc[s][n][x] = (float)(256 * si[0][n][x] + si[1][n][x]);
+            else sc[s][n][x] = fmaf((float)si[0][n][x], 65536.0f, (float)(256 * si[1][n][x] + si[DIGITS - 1][n][x]));
+          }
       }
       // vs = vf · 2^ve; a scale of zero: weights of zero.
       const int ex = max(int(f2u(cvs) >> 23) - 127, -126);

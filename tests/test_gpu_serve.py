@@ -254,10 +254,12 @@ def test_append_leaves_out_slots_behind_the_cache(torch, dev):
 
 
 def attention_exact(torch, kv, q, table, lens, starts, scale, window):
-    """The definition in 64 bits, with each output's bound. Query terms are
-    held to 22 bits (2^-22 of the row's largest, a term each) and the products
-    summed in float32, so a score is off by at most
-      ds = scale * sum_d |q_d k_d| * (hs + 4) u + scale * max|q| * sum_d |k_d| * 2^-22,
+    """The definition in 64 bits, with each output's bound. A row of queries is
+    held as integers of its largest magnitude: 127 * 257 steps for 16-bit types
+    (half a step is 2^-16 of the largest), 127 * 65793 for float32 (2^-24, and
+    2^-24 for the product before the rounding), and the products are summed and
+    joined in float32, so a score is off by at most
+      ds = scale * sum_d |q_d k_d| * (hs + 4) u + scale * max|q| * sum_d |k_d| * (2^-16 or 2^-23 + 2^-22),
     and in powers of two |s| * 4u more; a weight by 2 ds + 2^-20 relative; the
     sums over n tokens by n u of the sum of magnitudes. Also returned: that sum,
     sum_t p_t |v_t|, and n 2^-38 of the largest value: weights enter as float16
@@ -288,7 +290,7 @@ def attention_exact(torch, kv, q, table, lens, starts, scale, window):
                 p = torch.softmax(s, -1)
                 out[t, h * G:(h + 1) * G] = p @ vv
                 ds = scale * (qq.abs() @ kk.abs().T) * (hs + 4) * U + s.abs() * 4 * U \
-                    + scale * qq.abs().amax(1, keepdim=True) * kk.abs().sum(1)[None] * 2.0 ** -22
+                    + scale * qq.abs().amax(1, keepdim=True) * kk.abs().sum(1)[None] * ((2.0 ** -23 if q.dtype == torch.float32 else 2.0 ** -16) + 2.0 ** -22)
                 rel = 2 * ds.amax(1, keepdim=True) + 2.0 ** -20 + 2 * len(keep) * U
                 bound[t, h * G:(h + 1) * G] = rel * (p @ vv.abs())
                 mass[t, h * G:(h + 1) * G] = p @ vv.abs()
