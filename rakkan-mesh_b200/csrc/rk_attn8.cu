@@ -5,11 +5,14 @@
 namespace rk {
 
 // Joins the parts of the unit that crosses into CTA blockIdx.x + 1. The CTAs
-// that a unit crosses into share its rows, a warp each; a warp's lanes weigh
-// 32 parts at once and then add them up, four dimensions a lane.
-constexpr int kJoinWarps = 4;
+// that a unit crosses into share its rows. A row of a few parts is one warp's:
+// its lanes weigh the parts side by side and then add them up, four
+// dimensions a lane. A row of many is a CTA's, a share of the parts to each warp.
+constexpr int kJoinWarps = 4, kJoinFew = 8;
 
 __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int type, A8Grid grid) {
+  __shared__ float4 s_v[kJoinWarps][2][32];
+  __shared__ float s_l[kJoinWarps];
   griddep_wait();
   const A8Record *records = static_cast<const A8Record *>(a.ws);
   const float *parts = reinterpret_cast<const float *>(records + grid.ctas);
@@ -21,7 +24,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int
   // Part i is CTA first + i's: its second slot where the unit begins, else its first.
   const float *p0 = parts + 2LL * rec.first * size;
   auto part_of = [&](int i) { return p0 + (2LL * i + (i == 0)) * size; };
-  for (int row = (b - rec.first - 1) * kJoinWarps + warp; row < rec.rows; row += (n - 1) * kJoinWarps) {
+  const bool few = n <= kJoinFew;
+  const int nth = b - rec.first - 1, step = n - 1;
+  const int row0 = few ? nth * kJoinWarps + warp : nth, row_step = few ? step * kJoinWarps : step;
+  const int my0 = few ? 0 : warp * 32, my_step = few ? 32 : 32 * kJoinWarps;  // parts of this warp
+  for (int row = row0; row < rec.rows; row += row_step) {
     float mm = -INFINITY, MM = -INFINITY, ll = 0.0f;
     for (int i = lane; i < n; i += 32) {
       const float *s = part_of(i) + 64 * hs + 4 * row;
@@ -35,7 +42,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int
     }
     const float msafe = mm == -INFINITY ? 0.0f : mm, Msafe = MM == -INFINITY ? 0.0f : MM;
     float4 v[2] = {};
-    for (int i0 = 0; i0 < n; i0 += 32) {
+    for (int i0 = my0; i0 < n; i0 += my_step) {
       const int k = min(32, n - i0);
       float g = 0.0f;
       if (lane < k) {
@@ -61,6 +68,22 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+    if (!few) {
+      __syncthreads();
+      s_v[warp][0][lane] = v[0];
+      s_v[warp][1][lane] = v[1];
+      if (lane == 0) s_l[warp] = ll;
+      __syncthreads();
+      if (warp > 0) continue;
+      for (int w = 1; w < kJoinWarps; w++) {
+        ll += s_l[w];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const float4 x = s_v[w][j][lane];
+          v[j].x += x.x, v[j].y += x.y, v[j].z += x.z, v[j].w += x.w;
+        }
+      }
+    }
     const float scale = ll == 0.0f ? 0.0f : exp2f(Msafe - 14.0f - msafe) / ll;
     const int qrow = rec.row0 + row;
     const int64_t oi = (int64_t)(rec.q0 + qrow / G) * a.out_stride + (int64_t)(rec.head * G + qrow % G) * hs;
@@ -91,7 +114,8 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   const bool rows = (int64_t)a.tokens * G > 8LL * a.n;
   const int terms = type == RK_ACT_F32 || (type == RK_ACT_F16 && !rows) ? 2 : 1;
   const int nt = terms == 1 && rows && hs <= 128 ? 2 : 1;
-  A8Grid g{sms * a8_ctas(hs, terms, nt), 4, a.c.block == 16 ? 4 : a.c.block == 32 ? 5 : a.c.block == 64 ? 6 : 7};
+  A8Grid g{sms * a8_ctas(hs, terms, nt), 4, a.c.block == 16 ? 4 : a.c.block == 32 ? 5 : a.c.block == 64 ? 6 : 7,
+           a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0};
   // Short tables: a unit's tiles are few for one CTA, and without units cut in
   // two there is nothing to join.
   const bool whole = (int64_t)a.max_blocks * a.c.block <= 512;

@@ -82,6 +82,7 @@ struct A8Grid {
   int ctas;       // CTAs of the main kernel
   int min_tiles;  // fewest tiles worth a CTA; 0: a CTA takes whole units
   int log_block;  // of the page's tokens
+  bool vec_q;     // rows of q lie on 16-byte boundaries
 };
 
 RK_DEV uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
@@ -164,20 +165,61 @@ RK_DEV void load_row(const char *row, int swizzle, int c, uint32_t *w) {
   }
   if constexpr (R % 32 != 0) w[HS / 16 - 1] = *reinterpret_cast<const uint32_t *>(row + HS - 16 + 4 * c);
 }
-// The dimension of byte b (0..3) of lane c's word s.
-template <int HS>
-RK_DEV int dim_of(int s, int c, int b) {
+// A lane's values of a query row, in load_row's order: 16, 8 and 4
+// neighbours, as 16-byte pieces where the rows allow it.
+template <int N>
+RK_DEV void load_values(const float *q, bool vec, float *v) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4 *>(q + i));
+      v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = __ldg(q + i);
+  }
+}
+template <bool BF16>
+RK_DEV float half_value(uint32_t bits16) {
+  return BF16 ? u2f(bits16 << 16) : __half2float(__ushort_as_half((unsigned short)bits16));
+}
+template <int N, bool BF16>
+RK_DEV void load_values16(const uint16_t *q, bool vec, float *v) {
+  if (vec) {  // 8-byte pieces: N = 4 has no more
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint2 x = __ldg(reinterpret_cast<const uint2 *>(q + i));
+      v[i] = half_value<BF16>(x.x & 0xffff), v[i + 1] = half_value<BF16>(x.x >> 16);
+      v[i + 2] = half_value<BF16>(x.y & 0xffff), v[i + 3] = half_value<BF16>(x.y >> 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = half_value<BF16>(__ldg(q + i));
+  }
+}
+template <int HS, class F>
+RK_DEV void by_stretch(int c, F f) {  // f<N>(first dimension, first word)
   constexpr int N64 = HS / 64, R = HS % 64;
-  if (s < 4 * N64) return 64 * (s / 4) + 16 * c + 4 * (s % 4) + b;
-  if (R >= 32 && s < 4 * N64 + 2) return 64 * N64 + 8 * c + 4 * (s - 4 * N64) + b;
-  return HS - 16 + 4 * c + b;
+#pragma unroll
+  for (int i = 0; i < N64; i++) f.template operator()<16>(64 * i + 16 * c, 4 * i);
+  if constexpr (R >= 32) f.template operator()<8>(64 * N64 + 8 * c, 4 * N64);
+  if constexpr (R % 32 != 0) f.template operator()<4>(HS - 16 + 4 * c, HS / 16 - 1);
 }
-
-RK_DEV float q_load(const void *q, int type, int64_t i) {
-  if (type == RK_ACT_F32) return static_cast<const float *>(q)[i];
-  if (type == RK_ACT_F16) return __half2float(static_cast<const __half *>(q)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16 *>(q)[i]);
-}
+template <int HS>
+struct LoadQuery {
+  const void *q;
+  int64_t at;
+  int type;
+  bool vec;
+  float *v;
+  template <int N>
+  RK_DEV void operator()(int d, int word) const {
+    if (type == RK_ACT_F32) load_values<N>(static_cast<const float *>(q) + at + d, vec, v + 4 * word);
+    else if (type == RK_ACT_F16) load_values16<N, false>(static_cast<const uint16_t *>(q) + at + d, vec, v + 4 * word);
+    else load_values16<N, true>(static_cast<const uint16_t *>(q) + at + d, vec, v + 4 * word);
+  }
+};
 RK_DEV void o_store(void *o, int type, int64_t i, float v) {
   if (type == RK_ACT_F32) static_cast<float *>(o)[i] = v;
   else if (type == RK_ACT_F16) static_cast<__half *>(o)[i] = __float2half_rn(v);
@@ -188,14 +230,14 @@ RK_DEV void o_store(void *o, int type, int64_t i, float v) {
 struct A8Req {
   int q0, nq;      // its rows of q
   int len;         // its tokens, at most the table's
-  long long last;  // position of its last query (lens - 1, the table's end apart)
+  int last;        // position of its last query (lens - 1, the table's end apart)
   int tile0, tiles;
   int units;       // of one kv head
   int rw;          // row tiles of a unit (1, 2 or 4)
 };
 
 template <int HS, int R>
-RK_DEV A8Req a8_req(const Attn8Args &a, int i) {
+RK_DEV A8Req a8_req(const Attn8Args &a, int lb, int i) {
   constexpr int TT = kA8Tile;
   A8Req q;
   if (a.q_start) {
@@ -205,12 +247,12 @@ RK_DEV A8Req a8_req(const Attn8Args &a, int i) {
     q.q0 = i;
     q.nq = 1;
   }
-  const int len = a.lens[i];
-  q.last = (long long)len - 1;
-  q.len = (int)max(0LL, min((long long)len, (long long)a.max_blocks * a.c.block));
-  const long long from = a.window > 0 ? max(0LL, q.last - (q.nq - 1) + 1 - a.window) : 0;
-  q.tile0 = (int)min((long long)q.len, from) / TT;
-  q.tiles = max(1, (q.len + TT - 1) / TT - q.tile0);
+  const int len = max(a.lens[i], 0);
+  q.last = len - 1;
+  q.len = a.max_blocks < (len >> lb) + 1 ? min(len, a.max_blocks << lb) : len;
+  const int first = q.last - (q.nq - 1);
+  q.tile0 = a.window > 0 && first >= a.window ? min(q.len, first - a.window + 1) / TT : 0;
+  q.tiles = max(1, q.len / TT + (q.len % TT != 0) - q.tile0);
   const long long rows = (long long)q.nq * (a.heads / a.c.kv_heads);
   const int rts = (int)((rows + R - 1) / R);
   q.rw = rts >= 4 ? 4 : rts >= 2 ? 2 : 1;
@@ -241,7 +283,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   const int i0 = min(a.n, tid * per_t), i1 = min(a.n, i0 + per_t);
   auto size_of = [&](const A8Req &q) { return (long long)H * q.units * (by_unit ? 1 : q.tiles); };
   long long mine = 0;
-  for (int i = i0; i < i1; i++) mine += size_of(a8_req<HS, R>(a, i));
+  for (int i = i0; i < i1; i++) mine += size_of(a8_req<HS, R>(a, lb, i));
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -266,7 +308,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   if (begin >= excl && begin < excl + mine) {
     long long p = excl;
     for (int i = i0; i < i1; i++) {
-      const long long size = size_of(a8_req<HS, R>(a, i));
+      const long long size = size_of(a8_req<HS, R>(a, lb, i));
       if (begin < p + size) {
         s_req = i;
         s_before = p;
@@ -278,13 +320,13 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   __syncthreads();
   int req = s_req;
   long long base = s_before;  // where the request's run begins
-  A8Req q = a8_req<HS, R>(a, req);
+  A8Req q = a8_req<HS, R>(a, lb, req);
 
   for (long long at = begin; at < end;) {
     // The unit at `at`, and this CTA's tiles of it.
     while (at >= base + size_of(q)) {
       base += size_of(q);
-      q = a8_req<HS, R>(a, ++req);
+      q = a8_req<HS, R>(a, lb, ++req);
     }
     const int step = by_unit ? 1 : q.tiles;
     const int u = (int)(at - base) / step;
@@ -300,7 +342,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     // Limits of this lane's query columns: visible tokens are (low, high].
     // Columns past the last row see all (their queries are zeros, their sums
     // are not stored).
-    const long long pos0 = q.last - (q.nq - 1);
+    const int pos0 = q.last - (q.nq - 1);
     int high[NT][2], low[NT][2], high_max = -1, high_min = 0x7fffffff, low_max = -1;
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -310,9 +352,9 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         high[n][e] = 0x7fffffff;
         low[n][e] = -1;
         if (row < all_rows) {
-          const long long pos = pos0 + row / G;
-          high[n][e] = (int)max(-1LL, min(pos, (long long)q.len - 1));
-          if (a.window > 0) low[n][e] = (int)max(-1LL, min(pos - a.window, (long long)q.len));
+          const int pos = pos0 + row / G;
+          high[n][e] = max(-1, min(pos, q.len - 1));
+          if (a.window > 0 && pos >= a.window) low[n][e] = pos - a.window;
           high_max = max(high_max, high[n][e]);
         }
         high_min = min(high_min, high[n][e]);
@@ -325,9 +367,10 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       low_max = max(low_max, __shfl_xor_sync(0xffffffffu, low_max, o));
     }
     // The same of the whole unit: the tiles that its warps go through together.
-    const int reach = (int)max(-1LL, min(pos0 + (unit_row0 + unit_rows - 1) / G, (long long)q.len - 1));
-    const long long under = a.window > 0 ? pos0 + unit_row0 / G - a.window + 1 : 0;  // its first visible token
-    const int t_first = max(t0, (int)(max(0LL, min(under, (long long)q.len)) / TT) - q.tile0);
+    const int reach = max(-1, min(pos0 + (unit_row0 + unit_rows - 1) / G, q.len - 1));
+    const int pos_first = pos0 + unit_row0 / G;
+    const int t_first = a.window > 0 && pos_first >= a.window
+                            ? max(t0, min(q.len, pos_first - a.window + 1) / TT - q.tile0) : t0;
     const int t_end = min(t1, reach / TT + (reach >= 0) - q.tile0);
 
     // A group of rw warps shares the tiles t_first + wt, + tw, ..., and copies
@@ -397,10 +440,12 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       float top = 0.0f, v[KS][4];
       bool wrong = false;
 #pragma unroll
+      for (int s = 0; s < KS; s++) v[s][0] = v[s][1] = v[s][2] = v[s][3] = 0.0f;
+      if (have) by_stretch<HS>(c, LoadQuery<HS>{a.q, qi, type, grid.vec_q, v[0]});
+#pragma unroll
       for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-          v[s][b] = have ? q_load(a.q, type, qi + dim_of<HS>(s, c, b)) : 0.0f;
           top = fmaxf(top, fabsf(v[s][b]));
           wrong |= !(fabsf(v[s][b]) < INFINITY);
         }
