@@ -214,16 +214,24 @@ extern "C" int rk_w4_upload(rk_device *d, int rows, int cols, int group, int sca
     for (size_t i = 0; i < groups; i++)
       if (zeros[i] > 15) return bad("w4: zero point %d is not four bits", zeros[i]);
   OnDevice on(d, nullptr);
-  const size_t wb = (size_t)rows * cols / 2, sb = groups * act_size(scale_type);
-  const size_t o_s = (wb + 255) & ~size_t(255), o_z = o_s + ((sb + 255) & ~size_t(255));
-  const size_t total = o_z + (zeros ? groups : 0) + 256;
-  uint8_t *buf = nullptr;
+  // The caller's order goes through a buffer of its own, freed at the end.
+  const int sz = (int)act_size(scale_type);
+  const size_t wb = (size_t)rows * cols / 2, sb = groups * sz;
+  const auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
+  const size_t o_s = up(w4_weight_bytes(rows, cols)), o_z = o_s + up(w4_group_bytes(rows, cols / group, sz));
+  const size_t total = o_z + (zeros ? up(w4_group_bytes(rows, cols / group, 1)) : 0);
+  uint8_t *buf = nullptr, *raw = nullptr;
   cudaError_t e = on.e;
   if (e == cudaSuccess) e = cudaMalloc(&buf, total);
-  if (e == cudaSuccess) e = cudaMemcpyAsync(buf, w, wb, cudaMemcpyHostToDevice, on.st);
-  if (e == cudaSuccess) e = cudaMemcpyAsync(buf + o_s, scales, sb, cudaMemcpyHostToDevice, on.st);
-  if (e == cudaSuccess && zeros) e = cudaMemcpyAsync(buf + o_z, zeros, groups, cudaMemcpyHostToDevice, on.st);
+  if (e == cudaSuccess) e = cudaMalloc(&raw, up(wb) + up(sb) + groups);
+  uint8_t *raw_s = raw + up(wb), *raw_z = raw_s + up(sb);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(raw, w, wb, cudaMemcpyHostToDevice, on.st);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(raw_s, scales, sb, cudaMemcpyHostToDevice, on.st);
+  if (e == cudaSuccess && zeros) e = cudaMemcpyAsync(raw_z, zeros, groups, cudaMemcpyHostToDevice, on.st);
+  if (e == cudaSuccess)
+    e = launch_w4_layout(raw, raw_s, zeros ? raw_z : nullptr, rows, cols, group, sz, buf, buf + o_s, buf + o_z, on.st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(on.st);
+  cudaFree(raw);
   rk_w4 *m = e == cudaSuccess ? new (std::nothrow) rk_w4() : nullptr;
   if (!m) {
     cudaFree(buf);

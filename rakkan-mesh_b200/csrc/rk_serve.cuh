@@ -53,7 +53,7 @@ cudaError_t launch_add_rmsnorm_q8(const Norm8Args &a, int type, int sms, cudaStr
 struct W4Args {
   int rows, cols, group, x_group, n;
   int scale_type;
-  const uint8_t *w;
+  const uint8_t *w;      // in the order of launch_w4_layout, as are scales and zeros
   const void *scales;
   const uint8_t *zeros;  // null: 8
   const int8_t *x;
@@ -61,6 +61,11 @@ struct W4Args {
   void *out;
   int64_t out_stride;
 };
+// Bytes of the laid out weights, and of `each` bytes a group.
+inline int64_t w4_weight_bytes(int rows, int cols) { return (int64_t)((rows + 15) / 16) * ((cols + 63) / 64) * 512; }
+inline int64_t w4_group_bytes(int rows, int groups, int each) { return (int64_t)((rows + 15) / 16) * 16 * groups * each; }
+cudaError_t launch_w4_layout(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group,
+                             int scale_bytes, uint8_t *w_out, void *s_out, uint8_t *z_out, cudaStream_t st);
 cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st);
 
 // Dynamic shared memory opt-ins (once per device, at open).

@@ -1,49 +1,280 @@
 // rk_w4.cu — products of a 4-bit matrix with group scales and 8-bit vectors.
+//
+//   out[v][row] = Σ over segments  sw · sx · Σ_k (u_k − z) x_k
+// A segment is a run of columns with one weight scale and one vector scale.
+// Up to 16 vectors the bytes of the weights bound the product (half a byte a
+// weight), so what a warp does for them has to stay below an SM's share of
+// the memory bandwidth: about 44 instructions for 256 bytes. The sums run on
+// mma.m16n8k32 on signed bytes (16 rows, 8 vectors; one vector fills one
+// column, the others ride along), exact in int32. The weights are laid out
+// once, at upload, in the order in which a warp's lanes hold the operand, and
+// as two's complement nibbles of u − 8: the upper half of a byte, its lower
+// half masked away, is then 16 (u − 8) as a signed byte, so unpacking eight
+// weights takes three instructions and the 16 goes into the scale. A zero point other than
+// 8 takes 16 (z − 8) Σ x off, with Σ x from one more product by a constant operand.
+//
+// Work. A CTA takes MT tiles of 16 rows and a share of the columns, its eight
+// warps a share each; the warps' float32 sums meet in shared memory, those of
+// a cluster's CTAs (more than one where the rows are few) in the first one's.
+#include <cooperative_groups.h>
+
 #include "rk_act.cuh"
 #include "rk_serve.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace rk {
 
-// A warp per (row, vector): lane j takes every 32nd block of 32 columns.
-constexpr int kW4Warps = 4;
+constexpr int kW4Warps = 8;
 
-RK_DEV float scale_at(const void *s, int type, int64_t i) {
-  if (type == RK_ACT_F32) return static_cast<const float *>(s)[i];
-  if (type == RK_ACT_F16) return __half2float(static_cast<const __half *>(s)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16 *>(s)[i]);
+// Columns of a lane's nibbles, for column pair kp (64 columns), word 2s + h
+// (32-column step s, row r + 8h of the tile): low halves 8c .. 8c + 3 of the
+// step, high halves 8c + 4 .. 8c + 7. Its vector bytes are eight neighbours.
+RK_DEV int w4_col(int kp, int s, int c) { return 64 * kp + 32 * s + 8 * c; }
+
+__global__ void k_w4_layout(const uint8_t *w, int rows, int cols, int kpairs, uint32_t *out, int64_t words) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= words) return;
+  const int word = i & 3, lane = (i >> 2) & 31, r = lane >> 2, c = lane & 3;
+  const int64_t tile = (i >> 7) / kpairs;
+  const int kp = (int)((i >> 7) % kpairs), s = word >> 1;
+  const int64_t row = tile * 16 + r + 8 * (word & 1);
+  uint32_t v = 0;
+  if (row < rows)
+    for (int b = 0; b < 8; b++) {
+      const int col = w4_col(kp, s, c) + b;
+      if (col >= cols) break;
+      const uint8_t x = w[row * (cols / 2) + (col / 32) * 16 + col % 16];  // columns j and j + 16 of a block share byte j
+      const uint32_t u = (col % 32 < 16 ? x & 15 : x >> 4) ^ 8;
+      v |= u << (b < 4 ? 8 * b : 8 * (b - 4) + 4);
+    }
+  out[i] = v;
 }
 
+// [rows][groups] into [tile][group][16], `fill` behind the last row.
 template <class T>
-__global__ void __launch_bounds__(32 * kW4Warps) k_w4_rows(W4Args a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kW4Warps + (threadIdx.x >> 5), v = blockIdx.y;
-  if (row >= a.rows) return;
-  const int blocks = a.cols / 32, groups = a.cols / a.group, xgroups = a.cols / a.x_group;
-  float acc = 0.0f;
-  for (int b = lane; b < blocks; b += 32) {
-    const int64_t g = row * groups + 32 * b / a.group;
-    const int z = a.zeros ? a.zeros[g] : 8;
-    const uint8_t *w = a.w + row * (a.cols / 2) + 16 * b;
-    const int8_t *x = a.x + v * a.cols + 32 * b;
-    int dot = 0;
-    for (int j = 0; j < 16; j++) dot += ((w[j] & 15) - z) * x[j] + ((w[j] >> 4) - z) * x[j + 16];
-    acc = fmaf((float)dot, scale_at(a.scales, a.scale_type, g) * a.x_scales[v * xgroups + 32 * b / a.x_group], acc);
-  }
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (lane == 0) act_store(static_cast<T *>(a.out) + v * a.out_stride + row, acc);
+__global__ void k_w4_tile(const T *in, int rows, int groups, T fill, T *out, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int64_t row = (i >> 4) / groups * 16 + (i & 15);
+  out[i] = row < rows ? in[row * groups + (i >> 4) % groups] : fill;
 }
 
-cudaError_t launch_w4_mulvec(const W4Args &a, int type, int, cudaStream_t st) {
-  for (int v = 0; v < a.n; v += 32768) {  // grid.y's limit
+cudaError_t launch_w4_layout(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group,
+                             int scale_bytes, uint8_t *w_out, void *s_out, uint8_t *z_out, cudaStream_t st) {
+  const int kpairs = (cols + 63) / 64, groups = cols / group, tiles = (rows + 15) / 16;
+  const int64_t words = (int64_t)tiles * kpairs * 128, n = (int64_t)tiles * groups * 16;
+  const auto grid = [](int64_t k) { return dim3((unsigned)((k + 255) / 256)); };
+  cudaError_t e = launch_k(k_w4_layout, grid(words), 256, 0, st, w, rows, cols, kpairs, reinterpret_cast<uint32_t *>(w_out), words);
+  if (e == cudaSuccess) {
+    if (scale_bytes == 4)
+      e = launch_k(k_w4_tile<uint32_t>, grid(n), 256, 0, st, static_cast<const uint32_t *>(scales), rows, groups, 0u,
+                   static_cast<uint32_t *>(s_out), n);
+    else
+      e = launch_k(k_w4_tile<uint16_t>, grid(n), 256, 0, st, static_cast<const uint16_t *>(scales), rows, groups, (uint16_t)0,
+                   static_cast<uint16_t *>(s_out), n);
+  }
+  if (e == cudaSuccess && zeros) e = launch_k(k_w4_tile<uint8_t>, grid(n), 256, 0, st, zeros, rows, groups, (uint8_t)8, z_out, n);
+  return e;
+}
+
+RK_DEV float w4_scale(const void *s, int type, int64_t i) {
+  if (type == RK_ACT_F32) return __ldg(static_cast<const float *>(s) + i);
+  const unsigned short h = __ldg(static_cast<const unsigned short *>(s) + i);
+  return type == RK_ACT_F16 ? __half2float(__ushort_as_half(h)) : u2f((uint32_t)h << 16);
+}
+
+RK_DEV void imma(int *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// MT tiles of 16 rows, NT of 8 vectors; SEG columns share their scales.
+template <int MT, int NT, int SEG, bool ZEROS, class T>
+__global__ void __launch_bounds__(32 * kW4Warps) k_w4(W4Args a, int kpairs, int split) {
+  constexpr int AHEAD = 4;  // column pairs of weights in flight
+  __shared__ float s_part[kW4Warps][16 * MT][8 * NT];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+  const int tiles = (a.rows + 15) / 16, tile0 = (blockIdx.x / split) * MT, rank = blockIdx.x % split;
+  const int v0 = blockIdx.y * 8 * NT;
+  const int groups = a.cols / a.group, xgroups = a.cols / a.x_group;
+  // This warp's column pairs: a share in whole pairs of pairs (128 columns).
+  const int quads = (kpairs + 1) / 2, shares = split * kW4Warps, share = rank * kW4Warps + warp;
+  const int k0 = 2 * (int)((int64_t)quads * share / shares), k1 = min(kpairs, 2 * (int)((int64_t)quads * (share + 1) / shares));
+
+  const uint4 *w[MT];
+  int tile[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    tile[m] = min(tile0 + m, tiles - 1);  // a tile behind the last: computed again, not stored
+    w[m] = reinterpret_cast<const uint4 *>(a.w) + (int64_t)tile[m] * kpairs * 32 + lane;
+  }
+  const int8_t *x[NT];
+  bool have[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    have[n] = v0 + 8 * n + r < a.n;
+    x[n] = a.x + (have[n] ? (int64_t)(v0 + 8 * n + r) * a.cols : 0) + 8 * c;
+  }
+  int64_t xs_at[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) xs_at[n][e] = (int64_t)min(v0 + 8 * n + 2 * c + e, a.n - 1) * xgroups;
+
+  float acc[MT][NT][4] = {};
+  int sum[MT][NT][4] = {}, ones[NT][4] = {};
+  uint4 buf[AHEAD][MT];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+      buf[i][m] = k0 + i < k1 ? __ldcs(w[m] + (int64_t)(k0 + i) * 32) : make_uint4(0, 0, 0, 0);
+
+  auto flush = [&](int col) {  // the segment that holds column col
+    const int g = col / a.group, xg = col / a.x_group;
+    float sx[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      sx[n][0] = __ldg(a.x_scales + xs_at[n][0] + xg) * 0.0625f;
+      sx[n][1] = __ldg(a.x_scales + xs_at[n][1] + xg) * 0.0625f;
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+      const int64_t at = ((int64_t)tile[m] * groups + g) * 16 + r;
+      const float sw[2] = {w4_scale(a.scales, a.scale_type, at), w4_scale(a.scales, a.scale_type, at + 8)};
+      int z[2] = {0, 0};
+      if (ZEROS) {
+        z[0] = 8 - (int)__ldg(a.zeros + at);
+        z[1] = 8 - (int)__ldg(a.zeros + at + 8);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          int s = sum[m][n][e];
+          if (ZEROS) s += z[e >> 1] * ones[n][e];
+          acc[m][n][e] = fmaf((float)s, sw[e >> 1] * sx[n][e & 1], acc[m][n][e]);
+          sum[m][n][e] = 0;
+        }
+    }
+    if (ZEROS)
+#pragma unroll
+      for (int n = 0; n < NT; n++) ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0;
+  };
+
+  for (int kb = k0; kb < k1; kb += AHEAD) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) {
+      const int kp = kb + i;
+      if (kp >= k1) break;
+      uint2 xv[2][NT];
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const bool in = have[n] && (SEG > 32 || 64 * kp + 32 * s < a.cols);
+          xv[s][n] = in ? __ldg(reinterpret_cast<const uint2 *>(x[n] + 64 * kp + 32 * s)) : make_uint2(0, 0);
+        }
+      uint4 cur[MT];
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        cur[m] = buf[i][m];
+        if (kp + AHEAD < k1) buf[i][m] = __ldcs(w[m] + (int64_t)(kp + AHEAD) * 32);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        if (SEG == 32 && s == 1 && 64 * kp + 32 >= a.cols) break;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+          const uint32_t p = s ? cur[m].z : cur[m].x, q = s ? cur[m].w : cur[m].y;
+          const uint32_t a0 = (p << 4) & 0xf0f0f0f0u, a2 = p & 0xf0f0f0f0u;
+          const uint32_t a1 = (q << 4) & 0xf0f0f0f0u, a3 = q & 0xf0f0f0f0u;
+#pragma unroll
+          for (int n = 0; n < NT; n++) imma(sum[m][n], a0, a1, a2, a3, xv[s][n].x, xv[s][n].y);
+        }
+        if (ZEROS)
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+            imma(ones[n], 0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u, xv[s][n].x, xv[s][n].y);
+        if (SEG == 32) flush(64 * kp + 32 * s);
+      }
+      if (SEG == 64 || (SEG == 128 && (kp & 1))) flush(64 * kp);
+    }
+  }
+
+#pragma unroll
+  for (int m = 0; m < MT; m++)
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s_part[warp][16 * m + r + 8 * (e >> 1)][8 * n + 2 * c + (e & 1)] = acc[m][n][e];
+  __syncthreads();
+  // The warps in order, then the cluster's CTAs in order.
+  for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += 32 * kW4Warps) {
+    float v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kW4Warps; k++) v += (&s_part[k][0][0])[i];
+    (&s_part[0][0][0])[i] = v;
+  }
+  if (split > 1) cg::this_cluster().sync();
+  else __syncthreads();
+  if (rank == 0) {
+    for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += 32 * kW4Warps) {
+      // Neighbouring threads store neighbouring rows of a vector.
+      const int row = i % (16 * MT), vec = i / (16 * MT);
+      float v = s_part[0][row][vec];
+      for (int k = 1; k < split; k++) v += cg::this_cluster().map_shared_rank(&s_part[0][0][0], k)[row * 8 * NT + vec];
+      const int64_t to = (int64_t)tile0 * 16 + row;
+      if (to < a.rows && v0 + vec < a.n) act_store(static_cast<T *>(a.out) + (int64_t)(v0 + vec) * a.out_stride + to, v);
+    }
+  }
+  if (split > 1) cg::this_cluster().sync();  // a member's shared memory stays until it has been read
+}
+
+template <int MT, int NT, int SEG, bool ZEROS>
+static cudaError_t w4_run(const W4Args &a, int type, int split, cudaStream_t st) {
+  const int kpairs = (a.cols + 63) / 64, tiles = (a.rows + 15) / 16;
+  const dim3 grid((unsigned)((tiles + MT - 1) / MT * split), (unsigned)((a.n + 8 * NT - 1) / (8 * NT)));
+  const dim3 cl(split, 1, 1);
+  switch (type) {
+    case RK_ACT_F32: return launch_kc(k_w4<MT, NT, SEG, ZEROS, float>, grid, 32 * kW4Warps, cl, 0, st, a, kpairs, split);
+    case RK_ACT_F16: return launch_kc(k_w4<MT, NT, SEG, ZEROS, __half>, grid, 32 * kW4Warps, cl, 0, st, a, kpairs, split);
+    default: return launch_kc(k_w4<MT, NT, SEG, ZEROS, __nv_bfloat16>, grid, 32 * kW4Warps, cl, 0, st, a, kpairs, split);
+  }
+}
+
+template <int MT, int NT>
+static cudaError_t w4_seg(const W4Args &a, int type, int split, cudaStream_t st) {
+  const int seg = a.group % 128 == 0 && a.x_group % 128 == 0 ? 128 : a.group % 64 == 0 && a.x_group % 64 == 0 ? 64 : 32;
+  if (a.zeros) {
+    if (seg == 128) return w4_run<MT, NT, 128, true>(a, type, split, st);
+    if (seg == 64) return w4_run<MT, NT, 64, true>(a, type, split, st);
+    return w4_run<MT, NT, 32, true>(a, type, split, st);
+  }
+  if (seg == 128) return w4_run<MT, NT, 128, false>(a, type, split, st);
+  if (seg == 64) return w4_run<MT, NT, 64, false>(a, type, split, st);
+  return w4_run<MT, NT, 32, false>(a, type, split, st);
+}
+
+cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st) {
+  const int tiles = (a.rows + 15) / 16;
+  // More than 8 vectors: two tiles of 16 rows share a warp's vectors and
+  // their scales.
+  const int mt = a.n > 8 ? 2 : 1;
+  // CTAs of a cluster share the columns until every SM has two, as long as a
+  // warp keeps 256 columns.
+  int split = 1;
+  while (split < 8 && (int64_t)((tiles + mt - 1) / mt) * split < 2 * sms && a.cols / (split * 2 * kW4Warps) >= 256) split *= 2;
+  const int64_t width = 65535LL * 8;  // of grid.y
+  for (int64_t v = 0; v < a.n; v += width) {
     W4Args b = a;
-    b.n = a.n - v < 32768 ? a.n - v : 32768;
-    b.x += (int64_t)v * a.cols;
-    b.x_scales += (int64_t)v * (a.cols / a.x_group);
-    b.out = static_cast<char *>(a.out) + (int64_t)v * a.out_stride * (type == RK_ACT_F32 ? 4 : 2);
-    const dim3 grid((a.rows + kW4Warps - 1) / kW4Warps, b.n);
-    cudaError_t e = type == RK_ACT_F32   ? launch_k(k_w4_rows<float>, grid, 32 * kW4Warps, 0, st, b)
-                    : type == RK_ACT_F16 ? launch_k(k_w4_rows<__half>, grid, 32 * kW4Warps, 0, st, b)
-                                         : launch_k(k_w4_rows<__nv_bfloat16>, grid, 32 * kW4Warps, 0, st, b);
+    b.n = (int)(a.n - v < width ? a.n - v : width);
+    b.x += v * a.cols;
+    b.x_scales += v * (a.cols / a.x_group);
+    b.out = static_cast<char *>(a.out) + v * a.out_stride * (type == RK_ACT_F32 ? 4 : 2);
+    const cudaError_t e = mt == 2 ? w4_seg<2, 2>(b, type, split, st) : w4_seg<1, 1>(b, type, split, st);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
