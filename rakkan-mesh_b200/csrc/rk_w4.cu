@@ -78,23 +78,52 @@ cudaError_t launch_w4_layout(const uint8_t *w, const void *scales, const uint8_t
   return e;
 }
 
-RK_DEV float w4_scale(const void *s, int type, int64_t i) {
-  if (type == RK_ACT_F32) return __ldg(static_cast<const float *>(s) + i);
-  const unsigned short h = __ldg(static_cast<const unsigned short *>(s) + i);
-  return type == RK_ACT_F16 ? __half2float(__ushort_as_half(h)) : u2f((uint32_t)h << 16);
-}
-
 RK_DEV void imma(int *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Scales and zero points go through shared memory, a warp's own, for
+// kW4Chunk columns at a time: read from global memory where a segment ends
+// they cost a round trip for each (25.7 and 62.9 us for 28672x4096 by one vector
+// and 4096x14336 by 16).
+constexpr int kW4Chunk = 1024;
+// Groups that a chunk meets (its first column is a multiple of 128).
+__host__ __device__ inline int w4_chunk_groups(int group) {
+  return kW4Chunk % group == 0 && group <= 128 ? kW4Chunk / group : kW4Chunk / group + 2;
+}
+// Bytes of a warp's buffer: scales [groups][16 MT], zero points, vector scales [groups][8 NT].
+struct W4Smem {
+  int zeros, x, size;
+};
+__host__ __device__ inline W4Smem w4_smem(const W4Args &a, int mt, int nt) {
+  const int g = w4_chunk_groups(a.group) * 16 * mt;
+  W4Smem s;
+  s.zeros = g * (a.scale_type == RK_ACT_F32 ? 4 : 2);
+  s.x = s.zeros + (a.zeros ? g : 0);
+  s.size = s.x + w4_chunk_groups(a.x_group) * 8 * nt * 4;
+  return s;
+}
+
+RK_DEV void w4_copy16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+RK_DEV void w4_copy4(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
+RK_DEV float w4_scale(const char *s, int type, int i) {
+  if (type == RK_ACT_F32) return reinterpret_cast<const float *>(s)[i];
+  const unsigned short h = reinterpret_cast<const unsigned short *>(s)[i];
+  return type == RK_ACT_F16 ? __half2float(__ushort_as_half(h)) : u2f((uint32_t)h << 16);
+}
+
 // MT tiles of 16 rows, NT of 8 vectors; SEG columns share their scales.
 template <int MT, int NT, int SEG, bool ZEROS, class T>
-__global__ void __launch_bounds__(32 * kW4Warps) k_w4(W4Args a, int kpairs, int split) {
-  constexpr int AHEAD = 4;  // column pairs of weights in flight
-  __shared__ float s_part[kW4Warps][16 * MT][8 * NT];
+__global__ void __launch_bounds__(32 * kW4Warps, MT > 1 ? 2 : 3) k_w4(W4Args a, int kpairs, int split, int bufs) {
+  constexpr int AHEAD = MT > 1 ? 2 : 4;  // column pairs in flight
+  extern __shared__ __align__(16) char sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
   const int tiles = (a.rows + 15) / 16, tile0 = (blockIdx.x / split) * MT, rank = blockIdx.x % split;
   const int v0 = blockIdx.y * 8 * NT;
@@ -104,11 +133,11 @@ __global__ void __launch_bounds__(32 * kW4Warps) k_w4(W4Args a, int kpairs, int 
   const int k0 = 2 * (int)((int64_t)quads * share / shares), k1 = min(kpairs, 2 * (int)((int64_t)quads * (share + 1) / shares));
 
   const uint4 *w[MT];
-  int tile[MT];
+  int64_t tile[MT];
 #pragma unroll
   for (int m = 0; m < MT; m++) {
     tile[m] = min(tile0 + m, tiles - 1);  // a tile behind the last: computed again, not stored
-    w[m] = reinterpret_cast<const uint4 *>(a.w) + (int64_t)tile[m] * kpairs * 32 + lane;
+    w[m] = reinterpret_cast<const uint4 *>(a.w) + tile[m] * kpairs * 32 + lane;
   }
   const int8_t *x[NT];
   bool have[NT];
@@ -117,115 +146,160 @@ __global__ void __launch_bounds__(32 * kW4Warps) k_w4(W4Args a, int kpairs, int 
     have[n] = v0 + 8 * n + r < a.n;
     x[n] = a.x + (have[n] ? (int64_t)(v0 + 8 * n + r) * a.cols : 0) + 8 * c;
   }
-  int64_t xs_at[NT][2];
+  uint4 wbuf[AHEAD][MT];
+  uint2 xbuf[AHEAD][2][NT];
+  auto fetch = [&](int i, int kp) {
 #pragma unroll
-  for (int n = 0; n < NT; n++)
+    for (int m = 0; m < MT; m++)
+      if (kp < k1) wbuf[i][m] = __ldcs(w[m] + (int64_t)kp * 32);
 #pragma unroll
-    for (int e = 0; e < 2; e++) xs_at[n][e] = (int64_t)min(v0 + 8 * n + 2 * c + e, a.n - 1) * xgroups;
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const bool in = kp < k1 && have[n] && (SEG > 32 || 64 * kp + 32 * s < a.cols);
+        xbuf[i][s][n] = in ? __ldg(reinterpret_cast<const uint2 *>(x[n] + 64 * kp + 32 * s)) : make_uint2(0, 0);
+      }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) fetch(i, k0 + i);
+
+  const W4Smem lay = w4_smem(a, MT, NT);
+  const int es = a.scale_type == RK_ACT_F32 ? 4 : 2;
+  char *mine = sm + warp * bufs * lay.size;
+  auto stage = [&](int kp, char *to) {  // the scales of the chunk from column pair kp on
+    if (kp < k1) {
+      const int col = 64 * kp, last = min(64 * min(kp + kW4Chunk / 64, k1), a.cols) - 1;
+      const int g0 = col / a.group, ng = last / a.group - g0 + 1;
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        const char *src = static_cast<const char *>(a.scales) + (tile[m] * groups + g0) * 16 * es;
+        for (int i = lane; i < ng * es; i += 32) w4_copy16(to + (m * ng * es + i) * 16, src + 16 * i);
+        if (ZEROS)
+          for (int i = lane; i < ng; i += 32)
+            w4_copy16(to + lay.zeros + (m * ng + i) * 16, a.zeros + (tile[m] * groups + g0 + i) * 16);
+      }
+      const int x0 = col / a.x_group, nx = last / a.x_group - x0 + 1;
+      for (int i = lane; i < nx * 8 * NT; i += 32) {
+        const int v = i / nx, j = i % nx;
+        w4_copy4(to + lay.x + (j * 8 * NT + v) * 4, a.x_scales + (int64_t)min(v0 + v, a.n - 1) * xgroups + x0 + j);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  stage(k0, mine);
 
   float acc[MT][NT][4] = {};
   int sum[MT][NT][4] = {}, ones[NT][4] = {};
-  uint4 buf[AHEAD][MT];
-#pragma unroll
-  for (int i = 0; i < AHEAD; i++)
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-      buf[i][m] = k0 + i < k1 ? __ldcs(w[m] + (int64_t)(k0 + i) * 32) : make_uint4(0, 0, 0, 0);
-
-  auto flush = [&](int col) {  // the segment that holds column col
-    const int g = col / a.group, xg = col / a.x_group;
-    float sx[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      sx[n][0] = __ldg(a.x_scales + xs_at[n][0] + xg) * 0.0625f;
-      sx[n][1] = __ldg(a.x_scales + xs_at[n][1] + xg) * 0.0625f;
+  int buf = 0;
+  for (int kc = k0; kc < k1; kc += kW4Chunk / 64) {
+    const int kn = min(k1, kc + kW4Chunk / 64);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    const char *now = mine + buf * lay.size;
+    if (bufs > 1) {
+      buf ^= 1;
+      stage(kn, mine + buf * lay.size);
     }
+    // Where the chunk's columns lie in their groups.
+    const int col0 = 64 * kc, ng = (min(64 * kn, a.cols) - 1) / a.group - col0 / a.group + 1;
+    int g = 0, g_left = a.group - col0 % a.group, xg = 0, x_left = a.x_group - col0 % a.x_group;
+
+    auto flush = [&]() {  // the segment that ends here
+      float2 sx[NT];
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
-      const int64_t at = ((int64_t)tile[m] * groups + g) * 16 + r;
-      const float sw[2] = {w4_scale(a.scales, a.scale_type, at), w4_scale(a.scales, a.scale_type, at + 8)};
-      int z[2] = {0, 0};
-      if (ZEROS) {
-        z[0] = 8 - (int)__ldg(a.zeros + at);
-        z[1] = 8 - (int)__ldg(a.zeros + at + 8);
+      for (int n = 0; n < NT; n++) {
+        sx[n] = *reinterpret_cast<const float2 *>(now + lay.x + (xg * 8 * NT + 8 * n + 2 * c) * 4);
+        sx[n].x *= 0.0625f;
+        sx[n].y *= 0.0625f;
       }
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          int s = sum[m][n][e];
-          if (ZEROS) s += z[e >> 1] * ones[n][e];
-          acc[m][n][e] = fmaf((float)s, sw[e >> 1] * sx[n][e & 1], acc[m][n][e]);
-          sum[m][n][e] = 0;
-        }
-    }
-    if (ZEROS)
-#pragma unroll
-      for (int n = 0; n < NT; n++) ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0;
-  };
-
-  for (int kb = k0; kb < k1; kb += AHEAD) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; i++) {
-      const int kp = kb + i;
-      if (kp >= k1) break;
-      uint2 xv[2][NT];
-#pragma unroll
-      for (int s = 0; s < 2; s++)
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const bool in = have[n] && (SEG > 32 || 64 * kp + 32 * s < a.cols);
-          xv[s][n] = in ? __ldg(reinterpret_cast<const uint2 *>(x[n] + 64 * kp + 32 * s)) : make_uint2(0, 0);
-        }
-      uint4 cur[MT];
 #pragma unroll
       for (int m = 0; m < MT; m++) {
-        cur[m] = buf[i][m];
-        if (kp + AHEAD < k1) buf[i][m] = __ldcs(w[m] + (int64_t)(kp + AHEAD) * 32);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; s++) {
-        if (SEG == 32 && s == 1 && 64 * kp + 32 >= a.cols) break;
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-          const uint32_t p = s ? cur[m].z : cur[m].x, q = s ? cur[m].w : cur[m].y;
-          const uint32_t a0 = (p << 4) & 0xf0f0f0f0u, a2 = p & 0xf0f0f0f0u;
-          const uint32_t a1 = (q << 4) & 0xf0f0f0f0u, a3 = q & 0xf0f0f0f0u;
-#pragma unroll
-          for (int n = 0; n < NT; n++) imma(sum[m][n], a0, a1, a2, a3, xv[s][n].x, xv[s][n].y);
+        const int at = (m * ng + g) * 16 + r;
+        const float sw[2] = {w4_scale(now, a.scale_type, at), w4_scale(now, a.scale_type, at + 8)};
+        int z[2] = {0, 0};
+        if (ZEROS) {
+          z[0] = 8 - (int)*reinterpret_cast<const uint8_t *>(now + lay.zeros + at);
+          z[1] = 8 - (int)*reinterpret_cast<const uint8_t *>(now + lay.zeros + at + 8);
         }
-        if (ZEROS)
 #pragma unroll
-          for (int n = 0; n < NT; n++)
-            imma(ones[n], 0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u, xv[s][n].x, xv[s][n].y);
-        if (SEG == 32) flush(64 * kp + 32 * s);
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            int s = sum[m][n][e];
+            if (ZEROS) s += z[e >> 1] * ones[n][e];
+            acc[m][n][e] = fmaf((float)s, sw[e >> 1] * (e & 1 ? sx[n].y : sx[n].x), acc[m][n][e]);
+            sum[m][n][e] = 0;
+          }
       }
-      if (SEG == 64 || (SEG == 128 && (kp & 1))) flush(64 * kp);
+      if (ZEROS)
+#pragma unroll
+        for (int n = 0; n < NT; n++) ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0;
+      if ((g_left -= SEG) == 0) g++, g_left = a.group;
+      if ((x_left -= SEG) == 0) xg++, x_left = a.x_group;
+    };
+
+    for (int kb = kc; kb < kn; kb += AHEAD) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) {
+        const int kp = kb + i;
+        if (kp >= kn) break;
+        uint4 cw[MT];
+        uint2 cx[2][NT];
+#pragma unroll
+        for (int m = 0; m < MT; m++) cw[m] = wbuf[i][m];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+          for (int n = 0; n < NT; n++) cx[s][n] = xbuf[i][s][n];
+        fetch(i, kp + AHEAD);
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          if (SEG == 32 && s == 1 && 64 * kp + 32 >= a.cols) break;
+#pragma unroll
+          for (int m = 0; m < MT; m++) {
+            const uint32_t p = s ? cw[m].z : cw[m].x, q = s ? cw[m].w : cw[m].y;
+            const uint32_t a0 = (p << 4) & 0xf0f0f0f0u, a2 = p & 0xf0f0f0f0u;
+            const uint32_t a1 = (q << 4) & 0xf0f0f0f0u, a3 = q & 0xf0f0f0f0u;
+#pragma unroll
+            for (int n = 0; n < NT; n++) imma(sum[m][n], a0, a1, a2, a3, cx[s][n].x, cx[s][n].y);
+          }
+          if (ZEROS)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+              imma(ones[n], 0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u, cx[s][n].x, cx[s][n].y);
+          if (SEG == 32) flush();
+        }
+        if (SEG == 64 || (SEG == 128 && (kp & 1))) flush();
+      }
     }
   }
 
+  // The warps' sums, in order, then the cluster's CTAs', in order.
+  __syncthreads();
+  float *part = reinterpret_cast<float *>(sm);  // [warps][rows][vectors]
+  constexpr int TILE = 16 * MT * 8 * NT;
 #pragma unroll
   for (int m = 0; m < MT; m++)
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) s_part[warp][16 * m + r + 8 * (e >> 1)][8 * n + 2 * c + (e & 1)] = acc[m][n][e];
+      for (int e = 0; e < 4; e++)
+        part[warp * TILE + (16 * m + r + 8 * (e >> 1)) * 8 * NT + 8 * n + 2 * c + (e & 1)] = acc[m][n][e];
   __syncthreads();
-  // The warps in order, then the cluster's CTAs in order.
-  for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += 32 * kW4Warps) {
+  for (int i = threadIdx.x; i < TILE; i += 32 * kW4Warps) {
     float v = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kW4Warps; k++) v += (&s_part[k][0][0])[i];
-    (&s_part[0][0][0])[i] = v;
+    for (int k = 0; k < kW4Warps; k++) v += part[k * TILE + i];
+    part[i] = v;
   }
   if (split > 1) cg::this_cluster().sync();
   else __syncthreads();
   if (rank == 0) {
-    for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += 32 * kW4Warps) {
+    for (int i = threadIdx.x; i < TILE; i += 32 * kW4Warps) {
       // Neighbouring threads store neighbouring rows of a vector.
       const int row = i % (16 * MT), vec = i / (16 * MT);
-      float v = s_part[0][row][vec];
-      for (int k = 1; k < split; k++) v += cg::this_cluster().map_shared_rank(&s_part[0][0][0], k)[row * 8 * NT + vec];
+      float v = part[row * 8 * NT + vec];
+      for (int k = 1; k < split; k++) v += cg::this_cluster().map_shared_rank(part, k)[row * 8 * NT + vec];
       const int64_t to = (int64_t)tile0 * 16 + row;
       if (to < a.rows && v0 + vec < a.n) act_store(static_cast<T *>(a.out) + (int64_t)(v0 + vec) * a.out_stride + to, v);
     }
@@ -238,10 +312,16 @@ static cudaError_t w4_run(const W4Args &a, int type, int split, cudaStream_t st)
   const int kpairs = (a.cols + 63) / 64, tiles = (a.rows + 15) / 16;
   const dim3 grid((unsigned)((tiles + MT - 1) / MT * split), (unsigned)((a.n + 8 * NT - 1) / (8 * NT)));
   const dim3 cl(split, 1, 1);
+  // One buffer of scales where a chunk takes the longest share.
+  const int64_t quads = (kpairs + 1) / 2, shares = split * kW4Warps;
+  const int bufs = (quads + shares - 1) / shares * 128 <= kW4Chunk ? 1 : 2;
+  const size_t stage = (size_t)kW4Warps * bufs * w4_smem(a, MT, NT).size, part = (size_t)kW4Warps * 16 * MT * 8 * NT * 4;
+  const size_t smem = stage > part ? stage : part;
   switch (type) {
-    case RK_ACT_F32: return launch_kc(k_w4<MT, NT, SEG, ZEROS, float>, grid, 32 * kW4Warps, cl, 0, st, a, kpairs, split);
-    case RK_ACT_F16: return launch_kc(k_w4<MT, NT, SEG, ZEROS, __half>, grid, 32 * kW4Warps, cl, 0, st, a, kpairs, split);
-    default: return launch_kc(k_w4<MT, NT, SEG, ZEROS, __nv_bfloat16>, grid, 32 * kW4Warps, cl, 0, st, a, kpairs, split);
+    case RK_ACT_F32: return launch_kc(k_w4<MT, NT, SEG, ZEROS, float>, grid, 32 * kW4Warps, cl, smem, st, a, kpairs, split, bufs);
+    case RK_ACT_F16: return launch_kc(k_w4<MT, NT, SEG, ZEROS, __half>, grid, 32 * kW4Warps, cl, smem, st, a, kpairs, split, bufs);
+    default:
+      return launch_kc(k_w4<MT, NT, SEG, ZEROS, __nv_bfloat16>, grid, 32 * kW4Warps, cl, smem, st, a, kpairs, split, bufs);
   }
 }
 
@@ -280,6 +360,30 @@ cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st
   return cudaSuccess;
 }
 
-cudaError_t init_w4_attributes() { return cudaSuccess; }
+// The most shared memory of any matrix: float32 scales of groups of 32, two buffers.
+template <int MT, int NT, int SEG, bool ZEROS>
+static cudaError_t w4_attr() {
+  const int most = kW4Warps * 2 * (kW4Chunk / 32 * (16 * MT * (4 + ZEROS) + 8 * NT * 4));
+  const cudaFuncAttribute at = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e = cudaFuncSetAttribute(k_w4<MT, NT, SEG, ZEROS, float>, at, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_w4<MT, NT, SEG, ZEROS, __half>, at, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_w4<MT, NT, SEG, ZEROS, __nv_bfloat16>, at, most);
+  return e;
+}
+template <int MT, int NT>
+static cudaError_t w4_attrs() {
+  cudaError_t e = w4_attr<MT, NT, 32, false>();
+  if (e == cudaSuccess) e = w4_attr<MT, NT, 64, false>();
+  if (e == cudaSuccess) e = w4_attr<MT, NT, 128, false>();
+  if (e == cudaSuccess) e = w4_attr<MT, NT, 32, true>();
+  if (e == cudaSuccess) e = w4_attr<MT, NT, 64, true>();
+  if (e == cudaSuccess) e = w4_attr<MT, NT, 128, true>();
+  return e;
+}
+
+cudaError_t init_w4_attributes() {
+  const cudaError_t e = w4_attrs<1, 1>();
+  return e != cudaSuccess ? e : w4_attrs<2, 2>();
+}
 
 }  // namespace rk
