@@ -62,7 +62,7 @@ struct W4Args {
   int64_t out_stride;
 };
 // Bytes of the laid out weights, and of `each` bytes a group.
-inline int64_t w4_weight_bytes(int rows, int cols) { return (int64_t)((rows + 15) / 16) * ((cols + 63) / 64) * 512; }
+inline int64_t w4_weight_bytes(int rows, int cols) { return (int64_t)((rows + 15) / 16) * ((cols + 127) / 128) * 1024; }
 inline int64_t w4_group_bytes(int rows, int groups, int each) { return (int64_t)((rows + 15) / 16) * 16 * groups * each; }
 cudaError_t launch_w4_layout(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group,
                              int scale_bytes, uint8_t *w_out, void *s_out, uint8_t *z_out, cudaStream_t st);

@@ -13,9 +13,11 @@
 // weights takes three instructions and the 16 goes into the scale. A zero point other than
 // 8 takes 16 (z − 8) Σ x off, with Σ x from one more product by a constant operand.
 //
-// Work. A CTA takes MT tiles of 16 rows and a share of the columns, its eight
-// warps a share each; the warps' float32 sums meet in shared memory, those of
-// a cluster's CTAs (more than one where the rows are few) in the first one's.
+// Work. A warp takes MT tiles of 16 rows and a share of their columns, as few
+// shares as give every SM sixteen warps (a warp's beginning and end cost as
+// much as ten column pairs): first among a CTA's eight warps, which else take
+// tiles of their own, then among the CTAs of a cluster. The float32 sums of a
+// tile's shares meet in shared memory, in order.
 #include <cooperative_groups.h>
 
 #include "rk_act.cuh"
@@ -27,7 +29,8 @@ namespace rk {
 
 constexpr int kW4Warps = 8;
 
-// Columns of a lane's nibbles, for column pair kp (64 columns), word 2s + h
+// Rows are padded to 16 and columns to 128, with zeros. Columns of a lane's
+// nibbles, for column pair kp (64 columns), word 2s + h
 // (32-column step s, row r + 8h of the tile): low halves 8c .. 8c + 3 of the
 // step, high halves 8c + 4 .. 8c + 7. Its vector bytes are eight neighbours.
 RK_DEV int w4_col(int kp, int s, int c) { return 64 * kp + 32 * s + 8 * c; }
@@ -62,7 +65,7 @@ __global__ void k_w4_tile(const T *in, int rows, int groups, T fill, T *out, int
 
 cudaError_t launch_w4_layout(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group,
                              int scale_bytes, uint8_t *w_out, void *s_out, uint8_t *z_out, cudaStream_t st) {
-  const int kpairs = (cols + 63) / 64, groups = cols / group, tiles = (rows + 15) / 16;
+  const int kpairs = (cols + 127) / 128 * 2, groups = cols / group, tiles = (rows + 15) / 16;
   const int64_t words = (int64_t)tiles * kpairs * 128, n = (int64_t)tiles * groups * 16;
   const auto grid = [](int64_t k) { return dim3((unsigned)((k + 255) / 256)); };
   cudaError_t e = launch_k(k_w4_layout, grid(words), 256, 0, st, w, rows, cols, kpairs, reinterpret_cast<uint32_t *>(w_out), words);
@@ -121,155 +124,161 @@ RK_DEV float w4_scale(const char *s, int type, int i) {
 
 // MT tiles of 16 rows, NT of 8 vectors; SEG columns share their scales.
 template <int MT, int NT, int SEG, bool ZEROS, class T>
-__global__ void __launch_bounds__(32 * kW4Warps, MT > 1 ? 2 : 3) k_w4(W4Args a, int kpairs, int split, int bufs) {
-  constexpr int AHEAD = MT > 1 ? 2 : 4;  // column pairs in flight
+__global__ void __launch_bounds__(32 * kW4Warps, MT > 1 ? 2 : 3) k_w4(W4Args a, int quads, int split, int log_kw, int bufs) {
+  constexpr int AHEAD = 2;  // stretches of 128 columns in flight
   extern __shared__ __align__(16) char sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int tiles = (a.rows + 15) / 16, tile0 = (blockIdx.x / split) * MT, rank = blockIdx.x % split;
+  // Of the CTA's eight warps, 2^log_kw share the columns of a tile; so do the
+  // CTAs of a cluster, `split` of them (a power of two as well).
+  const int tiles = (a.rows + 15) / 16, rank = blockIdx.x & (split - 1), kw = 1 << log_kw;
+  const int cta_tile0 = blockIdx.x / split * (kW4Warps >> log_kw) * MT, tile0 = cta_tile0 + (warp >> log_kw) * MT;
   const int v0 = blockIdx.y * 8 * NT;
-  const int groups = a.cols / a.group, xgroups = a.cols / a.x_group;
-  // This warp's column pairs: a share in whole pairs of pairs (128 columns).
-  const int quads = (kpairs + 1) / 2, shares = split * kW4Warps, share = rank * kW4Warps + warp;
-  const int k0 = 2 * (int)((int64_t)quads * share / shares), k1 = min(kpairs, 2 * (int)((int64_t)quads * (share + 1) / shares));
+  // This warp's columns, in whole stretches of 128.
+  const int log_shares = __ffs(split) - 1 + log_kw, share = (rank << log_kw) + (warp & (kw - 1));
+  const int q0 = (quads * share) >> log_shares, q1 = (quads * (share + 1)) >> log_shares;  // quads <= 2^11, shares <= 2^6
 
+  // A tile behind the last and a vector behind the last are computed from
+  // the last one's, and not stored.
   const uint4 *w[MT];
-  int64_t tile[MT];
+  int tile[MT];
 #pragma unroll
   for (int m = 0; m < MT; m++) {
-    tile[m] = min(tile0 + m, tiles - 1);  // a tile behind the last: computed again, not stored
-    w[m] = reinterpret_cast<const uint4 *>(a.w) + tile[m] * kpairs * 32 + lane;
+    tile[m] = min(tile0 + m, tiles - 1);
+    w[m] = reinterpret_cast<const uint4 *>(a.w) + ((int64_t)tile[m] * quads + q0) * 64 + lane;
   }
   const int8_t *x[NT];
-  bool have[NT];
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
-    have[n] = v0 + 8 * n + r < a.n;
-    x[n] = a.x + (have[n] ? (int64_t)(v0 + 8 * n + r) * a.cols : 0) + 8 * c;
-  }
-  uint4 wbuf[AHEAD][MT];
-  uint2 xbuf[AHEAD][2][NT];
-  auto fetch = [&](int i, int kp) {
+  for (int n = 0; n < NT; n++) x[n] = a.x + (int64_t)min(v0 + 8 * n + r, a.n - 1) * a.cols + 128 * q0 + 8 * c;
+  uint4 wbuf[AHEAD][MT][2];
+  uint2 xbuf[AHEAD][NT][4];
+  auto fetch = [&](int i, int q) {  // the next stretch, q, into buffer i
+    if (q < q1) {
 #pragma unroll
-    for (int m = 0; m < MT; m++)
-      if (kp < k1) wbuf[i][m] = __ldcs(w[m] + (int64_t)kp * 32);
-#pragma unroll
-    for (int s = 0; s < 2; s++)
+      for (int m = 0; m < MT; m++) {
+        wbuf[i][m][0] = __ldcs(w[m]);
+        wbuf[i][m][1] = __ldcs(w[m] + 32);
+        w[m] += 64;
+      }
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        const bool in = kp < k1 && have[n] && (SEG > 32 || 64 * kp + 32 * s < a.cols);
-        xbuf[i][s][n] = in ? __ldg(reinterpret_cast<const uint2 *>(x[n] + 64 * kp + 32 * s)) : make_uint2(0, 0);
-      }
-  };
 #pragma unroll
-  for (int i = 0; i < AHEAD; i++) fetch(i, k0 + i);
+        for (int s = 0; s < 4; s++) {
+          // Only rows of less than whole stretches end inside one (their weights are zeros there).
+          if (SEG == 128 || 128 * q + 32 * s < a.cols) xbuf[i][n][s] = __ldg(reinterpret_cast<const uint2 *>(x[n] + 32 * s));
+        }
+        x[n] += 128;
+      }
+    }
+  };
+  if (SEG < 128)
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+      for (int n = 0; n < NT; n++) xbuf[i][n][0] = xbuf[i][n][1] = xbuf[i][n][2] = xbuf[i][n][3] = make_uint2(0, 0);
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) fetch(i, q0 + i);
 
+  const int groups = a.cols / a.group, xgroups = a.cols / a.x_group;
   const W4Smem lay = w4_smem(a, MT, NT);
   const int es = a.scale_type == RK_ACT_F32 ? 4 : 2;
   char *mine = sm + warp * bufs * lay.size;
-  auto stage = [&](int kp, char *to) {  // the scales of the chunk from column pair kp on
-    if (kp < k1) {
-      const int col = 64 * kp, last = min(64 * min(kp + kW4Chunk / 64, k1), a.cols) - 1;
+  auto stage = [&](int q, char *to) {  // the scales of the chunk from stretch q on
+    if (q < q1) {
+      const int col = 128 * q, last = min(128 * min(q + kW4Chunk / 128, q1), a.cols) - 1;
       const int g0 = col / a.group, ng = last / a.group - g0 + 1;
 #pragma unroll
       for (int m = 0; m < MT; m++) {
-        const char *src = static_cast<const char *>(a.scales) + (tile[m] * groups + g0) * 16 * es;
+        const char *src = static_cast<const char *>(a.scales) + ((int64_t)tile[m] * groups + g0) * 16 * es;
         for (int i = lane; i < ng * es; i += 32) w4_copy16(to + (m * ng * es + i) * 16, src + 16 * i);
         if (ZEROS)
           for (int i = lane; i < ng; i += 32)
-            w4_copy16(to + lay.zeros + (m * ng + i) * 16, a.zeros + (tile[m] * groups + g0 + i) * 16);
+            w4_copy16(to + lay.zeros + (m * ng + i) * 16, a.zeros + ((int64_t)tile[m] * groups + g0 + i) * 16);
       }
       const int x0 = col / a.x_group, nx = last / a.x_group - x0 + 1;
-      for (int i = lane; i < nx * 8 * NT; i += 32) {
-        const int v = i / nx, j = i % nx;
-        w4_copy4(to + lay.x + (j * 8 * NT + v) * 4, a.x_scales + (int64_t)min(v0 + v, a.n - 1) * xgroups + x0 + j);
-      }
+      for (int j = c; j < nx; j += 4)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+          w4_copy4(to + lay.x + (j * 8 * NT + 8 * n + r) * 4, a.x_scales + (int64_t)min(v0 + 8 * n + r, a.n - 1) * xgroups + x0 + j);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  stage(k0, mine);
+  stage(q0, mine);
 
   float acc[MT][NT][4] = {};
-  int sum[MT][NT][4] = {}, ones[NT][4] = {};
   int buf = 0;
-  for (int kc = k0; kc < k1; kc += kW4Chunk / 64) {
-    const int kn = min(k1, kc + kW4Chunk / 64);
+  for (int qc = q0; qc < q1; qc += kW4Chunk / 128) {
+    const int qn = min(q1, qc + kW4Chunk / 128);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
     const char *now = mine + buf * lay.size;
     if (bufs > 1) {
       buf ^= 1;
-      stage(kn, mine + buf * lay.size);
+      stage(qn, mine + buf * lay.size);
     }
     // Where the chunk's columns lie in their groups.
-    const int col0 = 64 * kc, ng = (min(64 * kn, a.cols) - 1) / a.group - col0 / a.group + 1;
-    int g = 0, g_left = a.group - col0 % a.group, xg = 0, x_left = a.x_group - col0 % a.x_group;
+    const int col0 = 128 * qc, ng = (min(128 * qn, a.cols) - 1) / a.group - col0 / a.group + 1;
+    int g_left = a.group - col0 % a.group, x_left = a.x_group - col0 % a.x_group;
+    const char *sw_at = now + r * es, *z_at = now + lay.zeros + r, *sx_at = now + lay.x + 8 * c;
 
-    auto flush = [&]() {  // the segment that ends here
-      float2 sx[NT];
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        sx[n] = *reinterpret_cast<const float2 *>(now + lay.x + (xg * 8 * NT + 8 * n + 2 * c) * 4);
-        sx[n].x *= 0.0625f;
-        sx[n].y *= 0.0625f;
-      }
-#pragma unroll
-      for (int m = 0; m < MT; m++) {
-        const int at = (m * ng + g) * 16 + r;
-        const float sw[2] = {w4_scale(now, a.scale_type, at), w4_scale(now, a.scale_type, at + 8)};
-        int z[2] = {0, 0};
-        if (ZEROS) {
-          z[0] = 8 - (int)*reinterpret_cast<const uint8_t *>(now + lay.zeros + at);
-          z[1] = 8 - (int)*reinterpret_cast<const uint8_t *>(now + lay.zeros + at + 8);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            int s = sum[m][n][e];
-            if (ZEROS) s += z[e >> 1] * ones[n][e];
-            acc[m][n][e] = fmaf((float)s, sw[e >> 1] * (e & 1 ? sx[n].y : sx[n].x), acc[m][n][e]);
-            sum[m][n][e] = 0;
-          }
-      }
-      if (ZEROS)
-#pragma unroll
-        for (int n = 0; n < NT; n++) ones[n][0] = ones[n][1] = ones[n][2] = ones[n][3] = 0;
-      if ((g_left -= SEG) == 0) g++, g_left = a.group;
-      if ((x_left -= SEG) == 0) xg++, x_left = a.x_group;
-    };
-
-    for (int kb = kc; kb < kn; kb += AHEAD) {
+    for (int qb = qc; qb < qn; qb += AHEAD) {
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
-        const int kp = kb + i;
-        if (kp >= kn) break;
-        uint4 cw[MT];
-        uint2 cx[2][NT];
+        const int q = qb + i;
+        if (q >= qn) break;
+        int sum[MT][NT][4], ones[NT][4];
 #pragma unroll
-        for (int m = 0; m < MT; m++) cw[m] = wbuf[i][m];
+        for (int s = 0; s < 4; s++) {
+          if (SEG < 128 && 128 * q + 32 * s >= a.cols) break;
+          const bool first = s * 32 % SEG == 0, last = (s + 1) * 32 % SEG == 0;
+          if (first) {
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int n = 0; n < NT; n++) cx[s][n] = xbuf[i][s][n];
-        fetch(i, kp + AHEAD);
+              for (int e = 0; e < 4; e++) {
+                ones[n][e] = 0;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-          if (SEG == 32 && s == 1 && 64 * kp + 32 >= a.cols) break;
+                for (int m = 0; m < MT; m++) sum[m][n][e] = 0;
+              }
+          }
 #pragma unroll
           for (int m = 0; m < MT; m++) {
-            const uint32_t p = s ? cw[m].z : cw[m].x, q = s ? cw[m].w : cw[m].y;
+            const uint4 cw = wbuf[i][m][s >> 1];
+            const uint32_t p = s & 1 ? cw.z : cw.x, u = s & 1 ? cw.w : cw.y;
             const uint32_t a0 = (p << 4) & 0xf0f0f0f0u, a2 = p & 0xf0f0f0f0u;
-            const uint32_t a1 = (q << 4) & 0xf0f0f0f0u, a3 = q & 0xf0f0f0f0u;
+            const uint32_t a1 = (u << 4) & 0xf0f0f0f0u, a3 = u & 0xf0f0f0f0u;
 #pragma unroll
-            for (int n = 0; n < NT; n++) imma(sum[m][n], a0, a1, a2, a3, cx[s][n].x, cx[s][n].y);
+            for (int n = 0; n < NT; n++) imma(sum[m][n], a0, a1, a2, a3, xbuf[i][n][s].x, xbuf[i][n][s].y);
           }
           if (ZEROS)
 #pragma unroll
             for (int n = 0; n < NT; n++)
-              imma(ones[n], 0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u, cx[s][n].x, cx[s][n].y);
-          if (SEG == 32) flush();
+              imma(ones[n], 0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u, xbuf[i][n][s].x, xbuf[i][n][s].y);
+          if (last) {  // a segment ends
+            float2 sx[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) sx[n] = *reinterpret_cast<const float2 *>(sx_at + 32 * n);
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+              const char *sp = sw_at + m * ng * 16 * es;
+              const float sw[2] = {w4_scale(sp, a.scale_type, 0) * 0.0625f, w4_scale(sp, a.scale_type, 8) * 0.0625f};
+              int z[2] = {0, 0};
+              if (ZEROS) {
+                z[0] = 8 - (int)*reinterpret_cast<const uint8_t *>(z_at + m * ng * 16);
+                z[1] = 8 - (int)*reinterpret_cast<const uint8_t *>(z_at + m * ng * 16 + 8);
+              }
+#pragma unroll
+              for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  const int v = ZEROS ? sum[m][n][e] + z[e >> 1] * ones[n][e] : sum[m][n][e];
+                  acc[m][n][e] = fmaf((float)v, sw[e >> 1] * (e & 1 ? sx[n].y : sx[n].x), acc[m][n][e]);
+                }
+            }
+            if ((g_left -= SEG) == 0) sw_at += 16 * es, z_at += 16, g_left = a.group;
+            if ((x_left -= SEG) == 0) sx_at += 32 * NT, x_left = a.x_group;
+          }
         }
-        if (SEG == 64 || (SEG == 128 && (kp & 1))) flush();
+        fetch(i, q + AHEAD);
       }
     }
   }
@@ -286,21 +295,23 @@ __global__ void __launch_bounds__(32 * kW4Warps, MT > 1 ? 2 : 3) k_w4(W4Args a, 
       for (int e = 0; e < 4; e++)
         part[warp * TILE + (16 * m + r + 8 * (e >> 1)) * 8 * NT + 8 * n + 2 * c + (e & 1)] = acc[m][n][e];
   __syncthreads();
-  for (int i = threadIdx.x; i < TILE; i += 32 * kW4Warps) {
-    float v = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kW4Warps; k++) v += part[k * TILE + i];
-    part[i] = v;
+  const int all = TILE * (kW4Warps >> log_kw);
+  for (int i = threadIdx.x; i < all; i += 32 * kW4Warps) {
+    const int at = (i / TILE << log_kw) * TILE + i % TILE;
+    float v = part[at];
+    for (int k = 1; k < kw; k++) v += part[at + k * TILE];
+    part[at] = v;
   }
   if (split > 1) cg::this_cluster().sync();
   else __syncthreads();
   if (rank == 0) {
-    for (int i = threadIdx.x; i < TILE; i += 32 * kW4Warps) {
+    for (int i = threadIdx.x; i < all; i += 32 * kW4Warps) {
       // Neighbouring threads store neighbouring rows of a vector.
-      const int row = i % (16 * MT), vec = i / (16 * MT);
-      float v = part[row * 8 * NT + vec];
-      for (int k = 1; k < split; k++) v += cg::this_cluster().map_shared_rank(part, k)[row * 8 * NT + vec];
-      const int64_t to = (int64_t)tile0 * 16 + row;
+      const int row = i % (16 * MT), vec = i / (16 * MT) % (8 * NT), t = i / TILE;
+      const int at = (t << log_kw) * TILE + row * 8 * NT + vec;
+      float v = part[at];
+      for (int k = 1; k < split; k++) v += cg::this_cluster().map_shared_rank(part, k)[at];
+      const int64_t to = (int64_t)(cta_tile0 + t * MT) * 16 + row;
       if (to < a.rows && v0 + vec < a.n) act_store(static_cast<T *>(a.out) + (int64_t)(v0 + vec) * a.out_stride + to, v);
     }
   }
@@ -308,34 +319,35 @@ __global__ void __launch_bounds__(32 * kW4Warps, MT > 1 ? 2 : 3) k_w4(W4Args a, 
 }
 
 template <int MT, int NT, int SEG, bool ZEROS>
-static cudaError_t w4_run(const W4Args &a, int type, int split, cudaStream_t st) {
-  const int kpairs = (a.cols + 63) / 64, tiles = (a.rows + 15) / 16;
-  const dim3 grid((unsigned)((tiles + MT - 1) / MT * split), (unsigned)((a.n + 8 * NT - 1) / (8 * NT)));
+static cudaError_t w4_run(const W4Args &a, int type, int split, int log_kw, cudaStream_t st) {
+  const int quads = (a.cols + 127) / 128, tiles = (a.rows + 15) / 16;
+  const int per_cta = (kW4Warps >> log_kw) * MT;
+  const dim3 grid((unsigned)((tiles + per_cta - 1) / per_cta * split), (unsigned)((a.n + 8 * NT - 1) / (8 * NT)));
   const dim3 cl(split, 1, 1);
   // One buffer of scales where a chunk takes the longest share.
-  const int64_t quads = (kpairs + 1) / 2, shares = split * kW4Warps;
+  const int64_t shares = split << log_kw;
   const int bufs = (quads + shares - 1) / shares * 128 <= kW4Chunk ? 1 : 2;
   const size_t stage = (size_t)kW4Warps * bufs * w4_smem(a, MT, NT).size, part = (size_t)kW4Warps * 16 * MT * 8 * NT * 4;
   const size_t smem = stage > part ? stage : part;
   switch (type) {
-    case RK_ACT_F32: return launch_kc(k_w4<MT, NT, SEG, ZEROS, float>, grid, 32 * kW4Warps, cl, smem, st, a, kpairs, split, bufs);
-    case RK_ACT_F16: return launch_kc(k_w4<MT, NT, SEG, ZEROS, __half>, grid, 32 * kW4Warps, cl, smem, st, a, kpairs, split, bufs);
+    case RK_ACT_F32: return launch_kc(k_w4<MT, NT, SEG, ZEROS, float>, grid, 32 * kW4Warps, cl, smem, st, a, quads, split, log_kw, bufs);
+    case RK_ACT_F16: return launch_kc(k_w4<MT, NT, SEG, ZEROS, __half>, grid, 32 * kW4Warps, cl, smem, st, a, quads, split, log_kw, bufs);
     default:
-      return launch_kc(k_w4<MT, NT, SEG, ZEROS, __nv_bfloat16>, grid, 32 * kW4Warps, cl, smem, st, a, kpairs, split, bufs);
+      return launch_kc(k_w4<MT, NT, SEG, ZEROS, __nv_bfloat16>, grid, 32 * kW4Warps, cl, smem, st, a, quads, split, log_kw, bufs);
   }
 }
 
 template <int MT, int NT>
-static cudaError_t w4_seg(const W4Args &a, int type, int split, cudaStream_t st) {
+static cudaError_t w4_seg(const W4Args &a, int type, int split, int log_kw, cudaStream_t st) {
   const int seg = a.group % 128 == 0 && a.x_group % 128 == 0 ? 128 : a.group % 64 == 0 && a.x_group % 64 == 0 ? 64 : 32;
   if (a.zeros) {
-    if (seg == 128) return w4_run<MT, NT, 128, true>(a, type, split, st);
-    if (seg == 64) return w4_run<MT, NT, 64, true>(a, type, split, st);
-    return w4_run<MT, NT, 32, true>(a, type, split, st);
+    if (seg == 128) return w4_run<MT, NT, 128, true>(a, type, split, log_kw, st);
+    if (seg == 64) return w4_run<MT, NT, 64, true>(a, type, split, log_kw, st);
+    return w4_run<MT, NT, 32, true>(a, type, split, log_kw, st);
   }
-  if (seg == 128) return w4_run<MT, NT, 128, false>(a, type, split, st);
-  if (seg == 64) return w4_run<MT, NT, 64, false>(a, type, split, st);
-  return w4_run<MT, NT, 32, false>(a, type, split, st);
+  if (seg == 128) return w4_run<MT, NT, 128, false>(a, type, split, log_kw, st);
+  if (seg == 64) return w4_run<MT, NT, 64, false>(a, type, split, log_kw, st);
+  return w4_run<MT, NT, 32, false>(a, type, split, log_kw, st);
 }
 
 cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st) {
@@ -343,10 +355,13 @@ cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st
   // More than 8 vectors: two tiles of 16 rows share a warp's vectors and
   // their scales.
   const int mt = a.n > 8 ? 2 : 1;
-  // CTAs of a cluster share the columns until every SM has two, as long as a
-  // warp keeps 256 columns.
-  int split = 1;
-  while (split < 8 && (int64_t)((tiles + mt - 1) / mt) * split < 2 * sms && a.cols / (split * 2 * kW4Warps) >= 256) split *= 2;
+  // Shares of the columns until every SM has sixteen warps, as long as a warp
+  // keeps 256 columns.
+  const int64_t units = (tiles + mt - 1) / mt;
+  int log_kw = 0, split = 1;
+  const auto more = [&] { return (units * split << log_kw) < 16 * sms && a.cols / (split * 2 << log_kw) >= 256; };
+  while (log_kw < 3 && more()) log_kw++;
+  while (log_kw == 3 && split < 8 && more()) split *= 2;
   const int64_t width = 65535LL * 8;  // of grid.y
   for (int64_t v = 0; v < a.n; v += width) {
     W4Args b = a;
@@ -354,7 +369,7 @@ cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st
     b.x += v * a.cols;
     b.x_scales += v * (a.cols / a.x_group);
     b.out = static_cast<char *>(a.out) + v * a.out_stride * (type == RK_ACT_F32 ? 4 : 2);
-    const cudaError_t e = mt == 2 ? w4_seg<2, 2>(b, type, split, st) : w4_seg<1, 1>(b, type, split, st);
+    const cudaError_t e = mt == 2 ? w4_seg<2, 2>(b, type, split, log_kw, st) : w4_seg<1, 1>(b, type, split, log_kw, st);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
