@@ -196,9 +196,8 @@ extern "C" int rk_add_rmsnorm_q8(rk_device *d, int type, int rows, int cols, int
 struct rk_w4 {
   rk_device *d = nullptr;
   int rows = 0, cols = 0, group = 0, scale_type = 0;
-  bool has_zeros = false;
-  uint8_t *buf = nullptr, *w = nullptr, *zeros = nullptr;
-  void *scales = nullptr;
+  bool zeros = false;
+  uint8_t *w = nullptr;
   int64_t bytes = 0;
 };
 
@@ -215,21 +214,18 @@ extern "C" int rk_w4_upload(rk_device *d, int rows, int cols, int group, int sca
       if (zeros[i] > 15) return bad("w4: zero point %d is not four bits", zeros[i]);
   OnDevice on(d, nullptr);
   // The caller's order goes through a buffer of its own, freed at the end.
-  const int sz = (int)act_size(scale_type);
-  const size_t wb = (size_t)rows * cols / 2, sb = groups * sz;
+  const size_t wb = (size_t)rows * cols / 2, sb = groups * act_size(scale_type);
   const auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
-  const size_t o_s = up(w4_weight_bytes(rows, cols)), o_z = o_s + up(w4_group_bytes(rows, cols / group, sz));
-  const size_t total = o_z + (zeros ? up(w4_group_bytes(rows, cols / group, 1)) : 0);
+  const size_t total = up(w4_bytes(rows, cols, group, scale_type, zeros != nullptr));
   uint8_t *buf = nullptr, *raw = nullptr;
   cudaError_t e = on.e;
   if (e == cudaSuccess) e = cudaMalloc(&buf, total);
   if (e == cudaSuccess) e = cudaMalloc(&raw, up(wb) + up(sb) + groups);
-  uint8_t *raw_s = raw + up(wb), *raw_z = raw_s + up(sb);
+  uint8_t *raw_s = raw + up(wb), *raw_z = zeros ? raw_s + up(sb) : nullptr;
   if (e == cudaSuccess) e = cudaMemcpyAsync(raw, w, wb, cudaMemcpyHostToDevice, on.st);
   if (e == cudaSuccess) e = cudaMemcpyAsync(raw_s, scales, sb, cudaMemcpyHostToDevice, on.st);
   if (e == cudaSuccess && zeros) e = cudaMemcpyAsync(raw_z, zeros, groups, cudaMemcpyHostToDevice, on.st);
-  if (e == cudaSuccess)
-    e = launch_w4_layout(raw, raw_s, zeros ? raw_z : nullptr, rows, cols, group, sz, buf, buf + o_s, buf + o_z, on.st);
+  if (e == cudaSuccess) e = launch_w4_stream(raw, raw_s, raw_z, rows, cols, group, scale_type, buf, on.st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(on.st);
   cudaFree(raw);
   rk_w4 *m = e == cudaSuccess ? new (std::nothrow) rk_w4() : nullptr;
@@ -243,10 +239,8 @@ extern "C" int rk_w4_upload(rk_device *d, int rows, int cols, int group, int sca
   m->cols = cols;
   m->group = group;
   m->scale_type = scale_type;
-  m->buf = buf;
+  m->zeros = zeros != nullptr;
   m->w = buf;
-  m->scales = buf + o_s;
-  m->zeros = zeros ? buf + o_z : nullptr;
   m->bytes = (int64_t)total;
   internal_device_count(d, m->bytes);
   *out = m;
@@ -256,7 +250,7 @@ extern "C" int rk_w4_upload(rk_device *d, int rows, int cols, int group, int sca
 extern "C" void rk_w4_free(rk_w4 *m) {
   if (!m) return;
   OnDevice on(m->d, nullptr);
-  cudaFree(m->buf);  // waits for the device's work, so products in flight have ended
+  cudaFree(m->w);  // waits for the device's work, so products in flight have ended
   internal_device_count(m->d, -m->bytes);
   delete m;
 }
@@ -276,7 +270,7 @@ extern "C" int rk_w4_mulvec(rk_w4 *m, int n, const int8_t *x, const float *x_sca
   if (out_stride < m->rows) return bad("w4: output rows overlap");
   if (!aligned(x, 16) || !aligned(x_scales, 4) || !aligned(out, act_size(type))) return bad("w4: a misaligned buffer");
   OnDevice on(m->d, stream);
-  W4Args a{m->rows, m->cols, m->group, x_group, n, m->scale_type, m->w, m->scales, m->zeros, x, x_scales, out,
+  W4Args a{m->rows, m->cols, m->group, x_group, n, m->scale_type, m->zeros, m->w, x, x_scales, out,
            out_stride};
   return on.done(on.e == cudaSuccess ? launch_w4_mulvec(a, type, on.sms, on.st) : on.e, "w4 product");
 }

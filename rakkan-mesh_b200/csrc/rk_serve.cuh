@@ -53,19 +53,18 @@ cudaError_t launch_add_rmsnorm_q8(const Norm8Args &a, int type, int sms, cudaStr
 struct W4Args {
   int rows, cols, group, x_group, n;
   int scale_type;
-  const uint8_t *w;      // in the order of launch_w4_layout, as are scales and zeros
-  const void *scales;
-  const uint8_t *zeros;  // null: 8
+  bool zeros;        // zero points in the stream (else 8)
+  const uint8_t *w;  // the stream of launch_w4_stream
   const int8_t *x;
   const float *x_scales;
   void *out;
   int64_t out_stride;
 };
-// Bytes of the laid out weights, and of `each` bytes a group.
-inline int64_t w4_weight_bytes(int rows, int cols) { return (int64_t)((rows + 15) / 16) * ((cols + 127) / 128) * 1024; }
-inline int64_t w4_group_bytes(int rows, int groups, int each) { return (int64_t)((rows + 15) / 16) * 16 * groups * each; }
-cudaError_t launch_w4_layout(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group,
-                             int scale_bytes, uint8_t *w_out, void *s_out, uint8_t *z_out, cudaStream_t st);
+// Bytes of a matrix's stream, and the stream from the caller's order (device
+// buffers; zeros may be null).
+int64_t w4_bytes(int rows, int cols, int group, int scale_type, bool zeros);
+cudaError_t launch_w4_stream(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group,
+                             int scale_type, uint8_t *out, cudaStream_t st);
 cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st);
 
 // Dynamic shared memory opt-ins (once per device, at open).

@@ -4,81 +4,109 @@
 // A segment is a run of columns with one weight scale and one vector scale.
 // Up to 16 vectors the bytes of the weights bound the product (half a byte a
 // weight), so what a warp does for them has to stay below an SM's share of
-// the memory bandwidth: about 44 instructions for 256 bytes. The sums run on
+// the memory bandwidth: about 180 instructions for a KB. The sums run on
 // mma.m16n8k32 on signed bytes (16 rows, 8 vectors; one vector fills one
-// column, the others ride along), exact in int32. The weights are laid out
-// once, at upload, in the order in which a warp's lanes hold the operand, and
-// as two's complement nibbles of u − 8: the upper half of a byte, its lower
-// half masked away, is then 16 (u − 8) as a signed byte, so unpacking eight
-// weights takes three instructions and the 16 goes into the scale. A zero point other than
-// 8 takes 16 (z − 8) Σ x off, with Σ x from one more product by a constant operand.
+// column, the others ride along), exact in int32.
 //
-// Work. A warp takes MT tiles of 16 rows and a share of their columns, as few
-// shares as give every SM sixteen warps (a warp's beginning and end cost as
-// much as ten column pairs): first among a CTA's eight warps, which else take
-// tiles of their own, then among the CTAs of a cluster. The float32 sums of a
-// tile's shares meet in shared memory, in order.
-#include <cooperative_groups.h>
-
+// Layout. At upload the matrix becomes a stream of records, one for each tile
+// of 16 rows and stretch of 128 columns: 1 KB of weights in the order in which
+// a warp's lanes hold the operand, then the scales (and zero points) of the
+// stretch's segments, repeated where a group is wider, so that a record is
+// one contiguous copy and needs no arithmetic on groups. Weights are two's
+// complement nibbles of u − 8: the upper half of a byte, its lower half masked
+// away, is then 16 (u − 8) as a signed byte, so unpacking eight weights takes
+// three instructions, and the 16 goes into the vectors' scales. A zero point
+// other than 8 adds (8 − z) · 16 Σ x, with Σ x made once for each segment.
+//
+// Work. One CTA of sixteen warps an SM goes through tiles of 16 rows. KW warps
+// of it (a team) share a tile's columns, or a cluster's CTAs do where there
+// are few rows; each warp keeps its share of the columns from tile to tile, so
+// the vectors and their scales are brought into shared memory once. The
+// records come through a ring of each warp in shared memory, which runs on
+// over the tiles: no load waits for a tile's end. (A CTA for each tile took
+// 22.3 us for 28672x4096 by one vector: its beginning and end cost as much as
+// ten column pairs a warp, and the last wave of CTAs left SMs idle.) The
+// float32 sums of a tile's shares meet in shared memory, in order, while the
+// warps are at the next tile.
 #include "rk_act.cuh"
 #include "rk_serve.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace rk {
 
-constexpr int kW4Warps = 8;
+constexpr int kW4Warps = 16;
+constexpr int kW4Smem = 227 * 1024;
 
-// Rows are padded to 16 and columns to 128, with zeros. Columns of a lane's
-// nibbles, for column pair kp (64 columns), word 2s + h
-// (32-column step s, row r + 8h of the tile): low halves 8c .. 8c + 3 of the
-// step, high halves 8c + 4 .. 8c + 7. Its vector bytes are eight neighbours.
-RK_DEV int w4_col(int kp, int s, int c) { return 64 * kp + 32 * s + 8 * c; }
+// Columns of the weights' segments, of both's.
+static int w4_width(int group) { return group % 128 == 0 ? 128 : group % 64 == 0 ? 64 : 32; }
+static int w4_segment(const W4Args &a) {
+  const int w = w4_width(a.group), x = w4_width(a.x_group);
+  return w < x ? w : x;
+}
+// Bytes of a segment's scales in a record: for r < 8, rows r and r + 8, each
+// the scale (and 8 − z: in the upper half of a 16-bit scale's word, or in a
+// word of its own).
+__host__ __device__ constexpr int w4_entry(bool s32, bool zeros) { return 32 * (s32 ? 2 : 1) * (zeros ? 2 : 1); }
+static int w4_record(int group, bool s32, bool zeros) { return 1024 + 128 / w4_width(group) * w4_entry(s32, zeros); }
+int64_t w4_bytes(int rows, int cols, int group, int scale_type, bool zeros) {
+  return (int64_t)((rows + 15) / 16) * ((cols + 127) / 128) * w4_record(group, scale_type == RK_ACT_F32, zeros);
+}
 
-__global__ void k_w4_layout(const uint8_t *w, int rows, int cols, int kpairs, uint32_t *out, int64_t words) {
+// The stream from the caller's order, a word a thread. Rows are padded to 16
+// and columns to 128 with zeros. Word `word` of lane (r, c) in 64 columns has
+// the nibbles of row r + 8 (word % 2) and step s = word / 2 of 32 columns: low
+// halves columns 8c .. 8c + 3 of the step, high halves 8c + 4 .. 8c + 7, so
+// that a lane's vector bytes are eight neighbours.
+__global__ void k_w4_stream(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group, bool s32,
+                            int width, int record, uint32_t *out, int64_t words) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= words) return;
-  const int word = i & 3, lane = (i >> 2) & 31, r = lane >> 2, c = lane & 3;
-  const int64_t tile = (i >> 7) / kpairs;
-  const int kp = (int)((i >> 7) % kpairs), s = word >> 1;
-  const int64_t row = tile * 16 + r + 8 * (word & 1);
+  const int quads = (cols + 127) / 128;
+  const int64_t rec = i / (record / 4), tile = rec / quads;
+  const int q = (int)(rec % quads), at = (int)(i % (record / 4));
   uint32_t v = 0;
-  if (row < rows)
-    for (int b = 0; b < 8; b++) {
-      const int col = w4_col(kp, s, c) + b;
-      if (col >= cols) break;
-      const uint8_t x = w[row * (cols / 2) + (col / 32) * 16 + col % 16];  // columns j and j + 16 of a block share byte j
-      const uint32_t u = (col % 32 < 16 ? x & 15 : x >> 4) ^ 8;
-      v |= u << (b < 4 ? 8 * b : 8 * (b - 4) + 4);
+  if (at < 256) {
+    const int word = at & 3, lane = (at >> 2) & 31, r = lane >> 2, c = lane & 3;
+    const int64_t row = tile * 16 + r + 8 * (word & 1);
+    if (row < rows)
+      for (int b = 0; b < 8; b++) {
+        const int col = 128 * q + 64 * (at >> 7) + 32 * (word >> 1) + 8 * c + b;
+        if (col >= cols) break;
+        const uint8_t x = w[row * (cols / 2) + (col / 32) * 16 + col % 16];  // columns j and j + 16 of a block share byte j
+        const uint32_t u = (col % 32 < 16 ? x & 15 : x >> 4) ^ 8;
+        v |= u << (b < 4 ? 8 * b : 8 * (b - 4) + 4);
+      }
+  } else {
+    const int per_row = (s32 ? 4 : 2) + (zeros ? (s32 ? 4 : 2) : 0);  // bytes
+    const int byte = 4 * (at - 256), entry = byte / (16 * per_row), in = byte % (16 * per_row);
+    const int col = 128 * q + width * entry;
+    const auto row_of = [&](int b) { return tile * 16 + b / (2 * per_row) + 8 * (b / per_row % 2); };
+    const auto group_at = [&](int64_t row) { return row * (cols / group) + col / group; };
+    if (col < cols) {
+      if (s32) {
+        const int64_t row = row_of(in);
+        if (row < rows)
+          v = in % per_row == 0 ? static_cast<const uint32_t *>(scales)[group_at(row)] : (uint32_t)(8 - (int)zeros[group_at(row)]);
+      } else if (zeros) {
+        const int64_t row = row_of(in);
+        if (row < rows)
+          v = static_cast<const uint16_t *>(scales)[group_at(row)] | (uint32_t)(8 - (int)zeros[group_at(row)]) << 16;
+      } else {
+        for (int h = 0; h < 2; h++) {
+          const int64_t row = row_of(in + 2 * h);
+          if (row < rows) v |= (uint32_t)static_cast<const uint16_t *>(scales)[group_at(row)] << (16 * h);
+        }
+      }
     }
+  }
   out[i] = v;
 }
 
-// [rows][groups] into [tile][group][16], `fill` behind the last row.
-template <class T>
-__global__ void k_w4_tile(const T *in, int rows, int groups, T fill, T *out, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int64_t row = (i >> 4) / groups * 16 + (i & 15);
-  out[i] = row < rows ? in[row * groups + (i >> 4) % groups] : fill;
-}
-
-cudaError_t launch_w4_layout(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group,
-                             int scale_bytes, uint8_t *w_out, void *s_out, uint8_t *z_out, cudaStream_t st) {
-  const int kpairs = (cols + 127) / 128 * 2, groups = cols / group, tiles = (rows + 15) / 16;
-  const int64_t words = (int64_t)tiles * kpairs * 128, n = (int64_t)tiles * groups * 16;
-  const auto grid = [](int64_t k) { return dim3((unsigned)((k + 255) / 256)); };
-  cudaError_t e = launch_k(k_w4_layout, grid(words), 256, 0, st, w, rows, cols, kpairs, reinterpret_cast<uint32_t *>(w_out), words);
-  if (e == cudaSuccess) {
-    if (scale_bytes == 4)
-      e = launch_k(k_w4_tile<uint32_t>, grid(n), 256, 0, st, static_cast<const uint32_t *>(scales), rows, groups, 0u,
-                   static_cast<uint32_t *>(s_out), n);
-    else
-      e = launch_k(k_w4_tile<uint16_t>, grid(n), 256, 0, st, static_cast<const uint16_t *>(scales), rows, groups, (uint16_t)0,
-                   static_cast<uint16_t *>(s_out), n);
-  }
-  if (e == cudaSuccess && zeros) e = launch_k(k_w4_tile<uint8_t>, grid(n), 256, 0, st, zeros, rows, groups, (uint8_t)8, z_out, n);
-  return e;
+cudaError_t launch_w4_stream(const uint8_t *w, const void *scales, const uint8_t *zeros, int rows, int cols, int group,
+                             int scale_type, uint8_t *out, cudaStream_t st) {
+  const bool s32 = scale_type == RK_ACT_F32;
+  const int64_t words = w4_bytes(rows, cols, group, scale_type, zeros != nullptr) / 4;
+  return launch_k(k_w4_stream, dim3((unsigned)((words + 255) / 256)), 256, 0, st, w, scales, zeros, rows, cols, group, s32,
+                  w4_width(group), w4_record(group, s32, zeros != nullptr), reinterpret_cast<uint32_t *>(out), words);
 }
 
 RK_DEV void imma(int *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -86,282 +114,377 @@ RK_DEV void imma(int *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uin
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
-// Scales and zero points go through shared memory, a warp's own, for
-// kW4Chunk columns at a time: read from global memory where a segment ends
-// they cost a round trip for each (25.7 and 62.9 us for 28672x4096 by one vector
-// and 4096x14336 by 16).
-constexpr int kW4Chunk = 1024;
-// Groups that a chunk meets (its first column is a multiple of 128).
-__host__ __device__ inline int w4_chunk_groups(int group) {
-  return kW4Chunk % group == 0 && group <= 128 ? kW4Chunk / group : kW4Chunk / group + 2;
+// The same from sums of zero.
+RK_DEV void imma_first(int *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
-// Bytes of a warp's buffer: scales [groups][16 MT], zero points, vector scales [groups][8 NT].
-struct W4Smem {
-  int zeros, x, size;
+
+// Shared memory by 32-bit addresses.
+RK_DEV uint32_t s_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+RK_DEV uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+RK_DEV uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+RK_DEV uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+RK_DEV void copy16_s(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+RK_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+RK_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Stores v at `to` (an address in this CTA's shared memory) of the cluster's first CTA.
+RK_DEV void store_first(uint32_t to, float v) {
+  asm volatile(
+      "{\n\t.reg .b32 p;\n\t"
+      "mapa.shared::cluster.u32 p, %0, 0;\n\t"
+      "st.shared::cluster.f32 [p], %1;\n\t}" ::"r"(to),
+      "f"(v)
+      : "memory");
+}
+
+// How a product is dealt out, and its shared memory.
+struct W4Plan {
+  int quads;      // stretches of 128 columns
+  int log_kw;     // log2 of the warps of a team
+  int split;      // CTAs of a cluster, which share a tile's columns (then teams are whole CTAs)
+  int teams;      // of all CTAs or clusters
+  int cta_quads;  // stretches of a CTA, at most
+  int x_stride;   // bytes between vectors in shared memory; 0: they stay in global memory
+  int record, log_width;  // of the stream: bytes of a record, log2 of a segment's columns
+  int at_xs, at_ring, at_part, at_far, size;
 };
-__host__ __device__ inline W4Smem w4_smem(const W4Args &a, int mt, int nt) {
-  const int g = w4_chunk_groups(a.group) * 16 * mt;
-  W4Smem s;
-  s.zeros = g * (a.scale_type == RK_ACT_F32 ? 4 : 2);
-  s.x = s.zeros + (a.zeros ? g : 0);
-  s.size = s.x + w4_chunk_groups(a.x_group) * 8 * nt * 4;
-  return s;
-}
+// Stages of a warp's ring.
+__host__ __device__ constexpr int w4_depth(int nt) { return nt > 1 ? 3 : 4; }
 
-RK_DEV void w4_copy16(void *dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
-RK_DEV void w4_copy4(void *dst, const void *src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
-
-RK_DEV float w4_scale(const char *s, int type, int i) {
-  if (type == RK_ACT_F32) return reinterpret_cast<const float *>(s)[i];
-  const unsigned short h = reinterpret_cast<const unsigned short *>(s)[i];
-  return type == RK_ACT_F16 ? __half2float(__ushort_as_half(h)) : u2f((uint32_t)h << 16);
-}
-
-// MT tiles of 16 rows, NT of 8 vectors; SEG columns share their scales.
-template <int MT, int NT, int SEG, bool ZEROS, class T>
-__global__ void __launch_bounds__(32 * kW4Warps, MT > 1 ? 2 : 3) k_w4(W4Args a, int quads, int split, int log_kw, int bufs) {
-  constexpr int AHEAD = 2;  // stretches of 128 columns in flight
-  extern __shared__ __align__(16) char sm[];
+// NT tiles of 8 vectors; SEG columns share their scales; XS: the vectors lie
+// in shared memory; S32: float32 scales.
+template <int NT, int SEG, bool ZEROS, bool XS, bool S32>
+__global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int out_type) {
+  constexpr int DEPTH = w4_depth(NT), TILE = 16 * 8 * NT, SEGS = 128 / SEG, ENTRY = w4_entry(S32, ZEROS);
+  constexpr int XSB = ZEROS ? 8 : 4;  // bytes of a vector's entry for a segment: its scale / 16 (and 16 Σ x)
+  extern __shared__ __align__(128) char sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  // Of the CTA's eight warps, 2^log_kw share the columns of a tile; so do the
-  // CTAs of a cluster, `split` of them (a power of two as well).
-  const int tiles = (a.rows + 15) / 16, rank = blockIdx.x & (split - 1), kw = 1 << log_kw;
-  const int cta_tile0 = blockIdx.x / split * (kW4Warps >> log_kw) * MT, tile0 = cta_tile0 + (warp >> log_kw) * MT;
-  const int v0 = blockIdx.y * 8 * NT;
-  // This warp's columns, in whole stretches of 128.
-  const int log_shares = __ffs(split) - 1 + log_kw, share = (rank << log_kw) + (warp & (kw - 1));
-  const int q0 = (quads * share) >> log_shares, q1 = (quads * (share + 1)) >> log_shares;  // quads <= 2^11, shares <= 2^6
+  const int kw = 1 << p.log_kw, tiles = (a.rows + 15) / 16;
+  const int rank = blockIdx.x & (p.split - 1);
+  const int team = p.split > 1 ? blockIdx.x / p.split : blockIdx.x * (kW4Warps >> p.log_kw) + (warp >> p.log_kw);
+  const int v0 = blockIdx.y * 8 * NT, nv = min(8 * NT, a.n - v0);
+  // The CTA's columns, and this warp's.
+  const int cq0 = p.quads * rank / p.split, cq1 = p.quads * (rank + 1) / p.split;
+  const int share = warp & (kw - 1);
+  const int q0 = cq0 + (((cq1 - cq0) * share) >> p.log_kw), q1 = cq0 + (((cq1 - cq0) * (share + 1)) >> p.log_kw);
 
-  // A tile behind the last and a vector behind the last are computed from
-  // the last one's, and not stored.
-  const uint4 *w[MT];
-  int tile[MT];
-#pragma unroll
-  for (int m = 0; m < MT; m++) {
-    tile[m] = min(tile0 + m, tiles - 1);
-    w[m] = reinterpret_cast<const uint4 *>(a.w) + ((int64_t)tile[m] * quads + q0) * 64 + lane;
-  }
-  const int8_t *x[NT];
-#pragma unroll
-  for (int n = 0; n < NT; n++) x[n] = a.x + (int64_t)min(v0 + 8 * n + r, a.n - 1) * a.cols + 128 * q0 + 8 * c;
-  uint4 wbuf[AHEAD][MT][2];
-  uint2 xbuf[AHEAD][NT][4];
-  auto fetch = [&](int i, int q) {  // the next stretch, q, into buffer i
-    if (q < q1) {
-#pragma unroll
-      for (int m = 0; m < MT; m++) {
-        wbuf[i][m][0] = __ldcs(w[m]);
-        wbuf[i][m][1] = __ldcs(w[m] + 32);
-        w[m] += 64;
+  // The ring. Records left to copy, and left of the tile's share.
+  const int len = q1 - q0, my_tiles = team < tiles ? (tiles - 1 - team) / p.teams + 1 : 0;
+  const uint32_t ring = s_addr(sm) + p.at_ring + warp * DEPTH * p.record, ring_end = ring + DEPTH * p.record;
+  int c_left = len * my_tiles, c_tile = len;
+  uint32_t c_to = ring + 16 * lane;
+  const uint8_t *c_from = a.w + ((int64_t)team * p.quads + q0) * p.record + 16 * lane;
+  const int64_t c_jump = ((int64_t)p.teams * p.quads - len) * p.record;
+  const bool c_tail = 1024 + 16 * lane < p.record;
+  auto copy = [&] {
+    if (c_left > 0) {
+      copy16_s(c_to, c_from);
+      copy16_s(c_to + 512, c_from + 512);
+      if (c_tail) copy16_s(c_to + 1024, c_from + 1024);
+      c_from += p.record;
+      c_to += p.record;
+      if (c_to >= ring_end) c_to = ring + 16 * lane;
+      c_left--;
+      if (--c_tile == 0) {
+        c_tile = len;
+        c_from += c_jump;
       }
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-          // Only rows of less than whole stretches end inside one (their weights are zeros there).
-          if (SEG == 128 || 128 * q + 32 * s < a.cols) xbuf[i][n][s] = __ldg(reinterpret_cast<const uint2 *>(x[n] + 32 * s));
-        }
-        x[n] += 128;
-      }
-    }
-  };
-  if (SEG < 128)
-#pragma unroll
-    for (int i = 0; i < AHEAD; i++)
-#pragma unroll
-      for (int n = 0; n < NT; n++) xbuf[i][n][0] = xbuf[i][n][1] = xbuf[i][n][2] = xbuf[i][n][3] = make_uint2(0, 0);
-#pragma unroll
-  for (int i = 0; i < AHEAD; i++) fetch(i, q0 + i);
-
-  const int groups = a.cols / a.group, xgroups = a.cols / a.x_group;
-  const W4Smem lay = w4_smem(a, MT, NT);
-  const int es = a.scale_type == RK_ACT_F32 ? 4 : 2;
-  char *mine = sm + warp * bufs * lay.size;
-  auto stage = [&](int q, char *to) {  // the scales of the chunk from stretch q on
-    if (q < q1) {
-      const int col = 128 * q, last = min(128 * min(q + kW4Chunk / 128, q1), a.cols) - 1;
-      const int g0 = col / a.group, ng = last / a.group - g0 + 1;
-#pragma unroll
-      for (int m = 0; m < MT; m++) {
-        const char *src = static_cast<const char *>(a.scales) + ((int64_t)tile[m] * groups + g0) * 16 * es;
-        for (int i = lane; i < ng * es; i += 32) w4_copy16(to + (m * ng * es + i) * 16, src + 16 * i);
-        if (ZEROS)
-          for (int i = lane; i < ng; i += 32)
-            w4_copy16(to + lay.zeros + (m * ng + i) * 16, a.zeros + ((int64_t)tile[m] * groups + g0 + i) * 16);
-      }
-      const int x0 = col / a.x_group, nx = last / a.x_group - x0 + 1;
-      for (int j = c; j < nx; j += 4)
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-          w4_copy4(to + lay.x + (j * 8 * NT + 8 * n + r) * 4, a.x_scales + (int64_t)min(v0 + 8 * n + r, a.n - 1) * xgroups + x0 + j);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  stage(q0, mine);
+#pragma unroll
+  for (int i = 0; i < DEPTH - 1; i++) copy();
 
-  float acc[MT][NT][4] = {};
-  int buf = 0;
-  for (int qc = q0; qc < q1; qc += kW4Chunk / 128) {
-    const int qn = min(q1, qc + kW4Chunk / 128);
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncwarp();
-    const char *now = mine + buf * lay.size;
-    if (bufs > 1) {
-      buf ^= 1;
-      stage(qn, mine + buf * lay.size);
+  // The CTA's columns of the vectors, and their entries: [segment][8 NT].
+  const int x0 = 128 * cq0, x_cols = min(a.cols, 128 * cq1) - x0;
+  if (XS)
+    for (int i = threadIdx.x; i < nv * (x_cols / 16); i += 32 * kW4Warps) {
+      const int v = i / (x_cols / 16), j = i % (x_cols / 16);
+      *reinterpret_cast<uint4 *>(sm + v * p.x_stride + 16 * j) =
+          __ldg(reinterpret_cast<const uint4 *>(a.x + (int64_t)(v0 + v) * a.cols + x0) + j);
     }
-    // Where the chunk's columns lie in their groups.
-    const int col0 = 128 * qc, ng = (min(128 * qn, a.cols) - 1) / a.group - col0 / a.group + 1;
-    int g_left = a.group - col0 % a.group, x_left = a.x_group - col0 % a.x_group;
-    const char *sw_at = now + r * es, *z_at = now + lay.zeros + r, *sx_at = now + lay.x + 8 * c;
-
-    for (int qb = qc; qb < qn; qb += AHEAD) {
+  for (int i = threadIdx.x; i < x_cols / SEG * 8 * NT; i += 32 * kW4Warps) {
+    const int v = v0 + min(i % (8 * NT), nv - 1), col = x0 + SEG * (i / (8 * NT));
+    const float s = __ldg(a.x_scales + (int64_t)v * (a.cols / a.x_group) + col / a.x_group) * 0.0625f;
+    if (ZEROS) {
+      const uint4 *at = reinterpret_cast<const uint4 *>(a.x + (int64_t)v * a.cols + col);
+      int sum = 0;
 #pragma unroll
-      for (int i = 0; i < AHEAD; i++) {
-        const int q = qb + i;
-        if (q >= qn) break;
-        int sum[MT][NT][4], ones[NT][4];
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-          if (SEG < 128 && 128 * q + 32 * s >= a.cols) break;
-          const bool first = s * 32 % SEG == 0, last = (s + 1) * 32 % SEG == 0;
-          if (first) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                ones[n][e] = 0;
-#pragma unroll
-                for (int m = 0; m < MT; m++) sum[m][n][e] = 0;
-              }
-          }
-#pragma unroll
-          for (int m = 0; m < MT; m++) {
-            const uint4 cw = wbuf[i][m][s >> 1];
-            const uint32_t p = s & 1 ? cw.z : cw.x, u = s & 1 ? cw.w : cw.y;
-            const uint32_t a0 = (p << 4) & 0xf0f0f0f0u, a2 = p & 0xf0f0f0f0u;
-            const uint32_t a1 = (u << 4) & 0xf0f0f0f0u, a3 = u & 0xf0f0f0f0u;
-#pragma unroll
-            for (int n = 0; n < NT; n++) imma(sum[m][n], a0, a1, a2, a3, xbuf[i][n][s].x, xbuf[i][n][s].y);
-          }
-          if (ZEROS)
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-              imma(ones[n], 0x10101010u, 0x10101010u, 0x10101010u, 0x10101010u, xbuf[i][n][s].x, xbuf[i][n][s].y);
-          if (last) {  // a segment ends
-            float2 sx[NT];
-#pragma unroll
-            for (int n = 0; n < NT; n++) sx[n] = *reinterpret_cast<const float2 *>(sx_at + 32 * n);
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-              const char *sp = sw_at + m * ng * 16 * es;
-              const float sw[2] = {w4_scale(sp, a.scale_type, 0) * 0.0625f, w4_scale(sp, a.scale_type, 8) * 0.0625f};
-              int z[2] = {0, 0};
-              if (ZEROS) {
-                z[0] = 8 - (int)*reinterpret_cast<const uint8_t *>(z_at + m * ng * 16);
-                z[1] = 8 - (int)*reinterpret_cast<const uint8_t *>(z_at + m * ng * 16 + 8);
-              }
-#pragma unroll
-              for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                  const int v = ZEROS ? sum[m][n][e] + z[e >> 1] * ones[n][e] : sum[m][n][e];
-                  acc[m][n][e] = fmaf((float)v, sw[e >> 1] * (e & 1 ? sx[n].y : sx[n].x), acc[m][n][e]);
-                }
-            }
-            if ((g_left -= SEG) == 0) sw_at += 16 * es, z_at += 16, g_left = a.group;
-            if ((x_left -= SEG) == 0) sx_at += 32 * NT, x_left = a.x_group;
-          }
-        }
-        fetch(i, q + AHEAD);
+      for (int k = 0; k < SEG / 16; k++) {
+        const uint4 u = __ldg(at + k);
+        sum = __dp4a((int)u.x, 0x10101010, sum);
+        sum = __dp4a((int)u.y, 0x10101010, sum);
+        sum = __dp4a((int)u.z, 0x10101010, sum);
+        sum = __dp4a((int)u.w, 0x10101010, sum);
       }
+      *reinterpret_cast<float2 *>(sm + p.at_xs + XSB * i) = make_float2(s, __int_as_float(sum));
+    } else {
+      *reinterpret_cast<float *>(sm + p.at_xs + XSB * i) = s;
     }
   }
-
-  // The warps' sums, in order, then the cluster's CTAs', in order.
   __syncthreads();
-  float *part = reinterpret_cast<float *>(sm);  // [warps][rows][vectors]
-  constexpr int TILE = 16 * MT * 8 * NT;
+
+  // A vector behind the last is computed from the last one's, and not stored.
+  uint32_t xr[NT];
+  const int8_t *xg[NT];
 #pragma unroll
-  for (int m = 0; m < MT; m++)
+  for (int n = 0; n < NT; n++) {
+    const int v = min(8 * n + r, nv - 1);
+    xr[n] = s_addr(sm) + v * p.x_stride + 128 * (q0 - cq0) + 8 * c;
+    xg[n] = a.x + (int64_t)(v0 + v) * a.cols + 128 * q0 + 8 * c;
+  }
+  const uint32_t x_first = s_addr(sm) + p.at_xs + (q0 - cq0) * SEGS * 8 * NT * XSB + 2 * c * XSB;
+  // Where a step's scales lie in a record (SEG may be narrower than the weights' segments).
+  uint32_t s_at[4];
+#pragma unroll
+  for (int s = 0; s < 4; s++) s_at[s] = 1024 + ((32 * s) >> p.log_width) * ENTRY + r * (ENTRY / 8);
+  const bool bf16 = a.scale_type == RK_ACT_BF16;
+  const auto half_scale = [&](uint32_t h) { return bf16 ? u2f(h << 16) : __half2float(__ushort_as_half((unsigned short)h)); };
+
+  float *part = reinterpret_cast<float *>(sm + p.at_part), *far = reinterpret_cast<float *>(sm + p.at_far);
+  uint32_t now = ring;
+  int flip = 0, far_tile = -1;
+  constexpr int MINE = (TILE + 32 * kW4Warps - 1) / (32 * kW4Warps);  // of a tile's sums, where the team is the CTA
+  float kept[MINE];
+  // Element i of a tile's sums: neighbours are neighbouring rows of a vector.
+  auto put = [&](int t, int i, float v) {
+    const int64_t row = (int64_t)t * 16 + i % 16;
+    const int vec = i / 16;
+    if (row >= a.rows || vec >= nv) return;
+    const int64_t to = (int64_t)(v0 + vec) * a.out_stride + row;
+    if (out_type == RK_ACT_F32) act_store(static_cast<float *>(a.out) + to, v);
+    else if (out_type == RK_ACT_F16) act_store(static_cast<__half *>(a.out) + to, v);
+    else act_store(static_cast<__nv_bfloat16 *>(a.out) + to, v);
+  };
+  auto join_far = [&] {  // the first CTA of a cluster: the other CTAs' sums of tile far_tile have come
+#pragma unroll
+    for (int k = 0; k < MINE; k++) {
+      const int i = threadIdx.x + k * 32 * kW4Warps;
+      if (i >= TILE) break;
+      float v = kept[k];
+      for (int o = 1; o < p.split; o++) v += far[((flip ^ 1) * (p.split - 1) + o - 1) * TILE + i];
+      put(far_tile, i, v);
+    }
+  };
+
+  for (int t = team; t < tiles; t += p.teams) {
+    float acc[NT][4] = {};
+    uint32_t x_at = x_first, xq[NT];
+    const int8_t *xp[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) xq[n] = xr[n], xp[n] = xg[n];
+    for (int q = q0; q < q1; q++) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
+      __syncwarp();
+      copy();
+      const uint4 w01 = lds128(now + 16 * lane), w23 = lds128(now + 512 + 16 * lane);
+      int sum[NT][4];
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        if (SEG < 128 && 128 * q + 32 * s >= a.cols) break;  // rows may end inside a stretch
+        const uint4 w = s < 2 ? w01 : w23;
+        const uint32_t lo = s & 1 ? w.z : w.x, hi = s & 1 ? w.w : w.y;  // rows r and r + 8
+        const uint32_t a0 = (lo << 4) & 0xf0f0f0f0u, a1 = (hi << 4) & 0xf0f0f0f0u, a2 = lo & 0xf0f0f0f0u, a3 = hi & 0xf0f0f0f0u;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const uint2 xv = XS ? lds64(xq[n] + 32 * s) : __ldg(reinterpret_cast<const uint2 *>(xp[n] + 32 * s));
+          if (s * 32 % SEG == 0) imma_first(sum[n], a0, a1, a2, a3, xv.x, xv.y);
+          else imma(sum[n], a0, a1, a2, a3, xv.x, xv.y);
+        }
+        if ((s + 1) * 32 % SEG == 0) {  // a segment ends
+          float sw[2];
+          int z[2] = {0, 0};
+          if constexpr (S32 && ZEROS) {
+            const uint4 e = lds128(now + s_at[s]);
+            sw[0] = u2f(e.x), z[0] = (int)e.y, sw[1] = u2f(e.z), z[1] = (int)e.w;
+          } else if constexpr (S32) {
+            const uint2 e = lds64(now + s_at[s]);
+            sw[0] = u2f(e.x), sw[1] = u2f(e.y);
+          } else if constexpr (ZEROS) {
+            const uint2 e = lds64(now + s_at[s]);
+            sw[0] = half_scale(e.x & 0xffff), z[0] = (int)e.x >> 16, sw[1] = half_scale(e.y & 0xffff), z[1] = (int)e.y >> 16;
+          } else {
+            const uint32_t e = lds32(now + s_at[s]);
+            sw[0] = half_scale(e & 0xffff), sw[1] = half_scale(e >> 16);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            float f[2];  // of vectors 2c and 2c + 1
+            if constexpr (ZEROS) {
+              const uint4 e = lds128(x_at + 8 * n * XSB);
+              f[0] = u2f(e.x), f[1] = u2f(e.z);
+              sum[n][0] += z[0] * (int)e.y;
+              sum[n][1] += z[0] * (int)e.w;
+              sum[n][2] += z[1] * (int)e.y;
+              sum[n][3] += z[1] * (int)e.w;
+            } else {
+              const uint2 e = lds64(x_at + 8 * n * XSB);
+              f[0] = u2f(e.x), f[1] = u2f(e.y);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[n][e] = fmaf((float)sum[n][e], sw[e >> 1] * f[e & 1], acc[n][e]);
+          }
+          x_at += 8 * NT * XSB;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++) xq[n] += 128, xp[n] += 128;
+      now += p.record;
+      if (now == ring_end) now = ring;
+    }
+    // The team's sums: one barrier a tile, since the next tile's go to the
+    // other half, and are read behind the next barrier.
+    float *mine = part + (flip * kW4Warps + warp) * TILE;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        part[warp * TILE + (16 * m + r + 8 * (e >> 1)) * 8 * NT + 8 * n + 2 * c + (e & 1)] = acc[m][n][e];
-  __syncthreads();
-  const int all = TILE * (kW4Warps >> log_kw);
-  for (int i = threadIdx.x; i < all; i += 32 * kW4Warps) {
-    const int at = (i / TILE << log_kw) * TILE + i % TILE;
-    float v = part[at];
-    for (int k = 1; k < kw; k++) v += part[at + k * TILE];
-    part[at] = v;
-  }
-  if (split > 1) cg::this_cluster().sync();
-  else __syncthreads();
-  if (rank == 0) {
-    for (int i = threadIdx.x; i < all; i += 32 * kW4Warps) {
-      // Neighbouring threads store neighbouring rows of a vector.
-      const int row = i % (16 * MT), vec = i / (16 * MT) % (8 * NT), t = i / TILE;
-      const int at = (t << log_kw) * TILE + row * 8 * NT + vec;
-      float v = part[at];
-      for (int k = 1; k < split; k++) v += cg::this_cluster().map_shared_rank(part, k)[at];
-      const int64_t to = (int64_t)(cta_tile0 + t * MT) * 16 + row;
-      if (to < a.rows && v0 + vec < a.n) act_store(static_cast<T *>(a.out) + (int64_t)(v0 + vec) * a.out_stride + to, v);
+      for (int e = 0; e < 4; e++) mine[(8 * n + 2 * c + (e & 1)) * 16 + r + 8 * (e >> 1)] = acc[n][e];
+    if (p.log_kw == 0) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(warp >> p.log_kw), "r"(32 << p.log_kw) : "memory");
+    const float *first = part + (flip * kW4Warps + (warp & ~(kw - 1))) * TILE;
+    if (p.split == 1) {
+      for (int i = share * 32 + lane; i < TILE; i += 32 << p.log_kw) {
+        float v = first[i];
+        for (int k = 1; k < kw; k++) v += first[k * TILE + i];
+        put(t, i, v);
+      }
+      flip ^= 1;
+    } else {
+      float here[MINE];
+#pragma unroll
+      for (int k = 0; k < MINE; k++) {
+        const int i = threadIdx.x + k * 32 * kW4Warps;
+        here[k] = 0.0f;
+        if (i < TILE) {
+          here[k] = first[i];
+          for (int o = 1; o < kw; o++) here[k] += first[o * TILE + i];
+        }
+      }
+      // The other CTAs' sums of the tile before have come: they are waited for a tile late.
+      if (far_tile >= 0) {
+        cluster_wait();
+        if (rank == 0) join_far();
+      } else {  // every CTA of the cluster has begun, before its memory is written
+        cluster_arrive();
+        cluster_wait();
+      }
+#pragma unroll
+      for (int k = 0; k < MINE; k++) {
+        const int i = threadIdx.x + k * 32 * kW4Warps;
+        if (rank == 0) kept[k] = here[k];
+        else if (i < TILE) store_first(s_addr(far + (flip * (p.split - 1) + rank - 1) * TILE + i), here[k]);
+      }
+      cluster_arrive();
+      far_tile = t;
+      flip ^= 1;
     }
   }
-  if (split > 1) cg::this_cluster().sync();  // a member's shared memory stays until it has been read
+  if (p.split > 1 && far_tile >= 0) {
+    cluster_wait();
+    if (rank == 0) join_far();
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <int MT, int NT, int SEG, bool ZEROS>
-static cudaError_t w4_run(const W4Args &a, int type, int split, int log_kw, cudaStream_t st) {
-  const int quads = (a.cols + 127) / 128, tiles = (a.rows + 15) / 16;
-  const int per_cta = (kW4Warps >> log_kw) * MT;
-  const dim3 grid((unsigned)((tiles + per_cta - 1) / per_cta * split), (unsigned)((a.n + 8 * NT - 1) / (8 * NT)));
-  const dim3 cl(split, 1, 1);
-  // One buffer of scales where a chunk takes the longest share.
-  const int64_t shares = split << log_kw;
-  const int bufs = (quads + shares - 1) / shares * 128 <= kW4Chunk ? 1 : 2;
-  const size_t stage = (size_t)kW4Warps * bufs * w4_smem(a, MT, NT).size, part = (size_t)kW4Warps * 16 * MT * 8 * NT * 4;
-  const size_t smem = stage > part ? stage : part;
-  switch (type) {
-    case RK_ACT_F32: return launch_kc(k_w4<MT, NT, SEG, ZEROS, float>, grid, 32 * kW4Warps, cl, smem, st, a, quads, split, log_kw, bufs);
-    case RK_ACT_F16: return launch_kc(k_w4<MT, NT, SEG, ZEROS, __half>, grid, 32 * kW4Warps, cl, smem, st, a, quads, split, log_kw, bufs);
-    default:
-      return launch_kc(k_w4<MT, NT, SEG, ZEROS, __nv_bfloat16>, grid, 32 * kW4Warps, cl, smem, st, a, quads, split, log_kw, bufs);
-  }
+// Shared memory of a plan (teams, log_kw, split set); the vectors go to
+// shared memory if that fits.
+static void w4_layout_smem(const W4Args &a, W4Plan &p) {
+  const int nt = a.n > 8 ? 2 : 1, nv = a.n < 8 * nt ? a.n : 8 * nt;
+  p.cta_quads = (p.quads + p.split - 1) / p.split;
+  const int xs = (128 * p.cta_quads / w4_segment(a) * 8 * nt * (a.zeros ? 8 : 4) + 127) / 128 * 128;
+  const int ring = (kW4Warps * w4_depth(nt) * p.record + 127) / 128 * 128;
+  const int part = 2 * kW4Warps * 16 * 8 * nt * 4, far = 2 * (p.split - 1) * 16 * 8 * nt * 4;
+  p.x_stride = 128 * p.cta_quads + 32;  // rows of eight lanes' reads fall on different banks
+  if ((int64_t)nv * p.x_stride + 128 + xs + ring + part + far > kW4Smem) p.x_stride = 0;
+  p.at_xs = (nv * p.x_stride + 127) / 128 * 128;
+  p.at_ring = p.at_xs + xs;
+  p.at_part = p.at_ring + ring;
+  p.at_far = p.at_part + part;
+  p.size = p.at_far + far;
 }
 
-template <int MT, int NT>
-static cudaError_t w4_seg(const W4Args &a, int type, int split, int log_kw, cudaStream_t st) {
-  const int seg = a.group % 128 == 0 && a.x_group % 128 == 0 ? 128 : a.group % 64 == 0 && a.x_group % 64 == 0 ? 64 : 32;
-  if (a.zeros) {
-    if (seg == 128) return w4_run<MT, NT, 128, true>(a, type, split, log_kw, st);
-    if (seg == 64) return w4_run<MT, NT, 64, true>(a, type, split, log_kw, st);
-    return w4_run<MT, NT, 32, true>(a, type, split, log_kw, st);
+// f<NT, SEG, ZEROS, XS, S32>() of the instance for a product.
+template <int NT, bool XS, bool S32, class F>
+static cudaError_t w4_seg(int seg, bool zeros, F f) {
+  if (zeros) {
+    if (seg == 128) return f.template operator()<NT, 128, true, XS, S32>();
+    if (seg == 64) return f.template operator()<NT, 64, true, XS, S32>();
+    return f.template operator()<NT, 32, true, XS, S32>();
   }
-  if (seg == 128) return w4_run<MT, NT, 128, false>(a, type, split, log_kw, st);
-  if (seg == 64) return w4_run<MT, NT, 64, false>(a, type, split, log_kw, st);
-  return w4_run<MT, NT, 32, false>(a, type, split, log_kw, st);
+  if (seg == 128) return f.template operator()<NT, 128, false, XS, S32>();
+  if (seg == 64) return f.template operator()<NT, 64, false, XS, S32>();
+  return f.template operator()<NT, 32, false, XS, S32>();
 }
+template <class F>
+static cudaError_t w4_at(int nt, bool xs, bool s32, int seg, bool zeros, F f) {
+  if (nt > 1) {
+    if (xs) return s32 ? w4_seg<2, true, true>(seg, zeros, f) : w4_seg<2, true, false>(seg, zeros, f);
+    return s32 ? w4_seg<2, false, true>(seg, zeros, f) : w4_seg<2, false, false>(seg, zeros, f);
+  }
+  if (xs) return s32 ? w4_seg<1, true, true>(seg, zeros, f) : w4_seg<1, true, false>(seg, zeros, f);
+  return s32 ? w4_seg<1, false, true>(seg, zeros, f) : w4_seg<1, false, false>(seg, zeros, f);
+}
+
+struct W4Launch {
+  const W4Args &a;
+  int type;
+  const W4Plan &p;
+  cudaStream_t st;
+  template <int NT, int SEG, bool ZEROS, bool XS, bool S32>
+  cudaError_t operator()() const {
+    const int ctas = p.split > 1 ? p.teams * p.split : p.teams / (kW4Warps >> p.log_kw);
+    const dim3 grid(ctas, (unsigned)((a.n + 8 * NT - 1) / (8 * NT))), cl(p.split, 1, 1);
+    return launch_kc(k_w4<NT, SEG, ZEROS, XS, S32>, grid, 32 * kW4Warps, cl, p.size, st, a, p, type);
+  }
+};
 
 cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st) {
   const int tiles = (a.rows + 15) / 16;
-  // More than 8 vectors: two tiles of 16 rows share a warp's vectors and
-  // their scales.
-  const int mt = a.n > 8 ? 2 : 1;
-  // Shares of the columns until every SM has sixteen warps, as long as a warp
-  // keeps 256 columns.
-  const int64_t units = (tiles + mt - 1) / mt;
-  int log_kw = 0, split = 1;
-  const auto more = [&] { return (units * split << log_kw) < 16 * sms && a.cols / (split * 2 << log_kw) >= 256; };
-  while (log_kw < 3 && more()) log_kw++;
-  while (log_kw == 3 && split < 8 && more()) split *= 2;
+  const bool s32 = a.scale_type == RK_ACT_F32;
+  W4Plan best{};
+  double least = 0;
+  // The time of a plan in stretches: a team's tiles, each its longest share and
+  // an end (about two stretches' instructions; another four for the exchange in
+  // a cluster); vectors that stay in global memory take four times as long.
+  const auto take = [&](int log_kw, int split) {
+    W4Plan p{};
+    p.quads = (a.cols + 127) / 128;
+    p.log_kw = log_kw;
+    p.split = split;
+    p.record = w4_record(a.group, s32, a.zeros);
+    p.log_width = w4_width(a.group) == 128 ? 7 : w4_width(a.group) == 64 ? 6 : 5;
+    w4_layout_smem(a, p);
+    if (p.size > kW4Smem) return;
+    const int units = split > 1 ? sms / split : sms * (kW4Warps >> log_kw);
+    const int rounds = (tiles + units - 1) / units;
+    const int share = (p.cta_quads + (1 << log_kw) - 1) >> log_kw;
+    const double cost = rounds * (share * (p.x_stride ? 1.0 : 4.0) + 2 + (split > 1 ? 4 : 0));
+    const int per_cta = kW4Warps >> log_kw;
+    p.teams = split > 1 ? (tiles < units ? tiles : units) : (tiles < units ? (tiles + per_cta - 1) / per_cta * per_cta : units);
+    if (least == 0 || cost < least) {
+      least = cost;
+      best = p;
+    }
+  };
+  for (int k = 4; k >= 0; k--) take(k, 1);
+  for (int s = 2; s <= 8; s *= 2) take(4, s);
+  if (least == 0) return cudaErrorInvalidValue;
   const int64_t width = 65535LL * 8;  // of grid.y
   for (int64_t v = 0; v < a.n; v += width) {
     W4Args b = a;
@@ -369,36 +492,26 @@ cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st
     b.x += v * a.cols;
     b.x_scales += v * (a.cols / a.x_group);
     b.out = static_cast<char *>(a.out) + v * a.out_stride * (type == RK_ACT_F32 ? 4 : 2);
-    const cudaError_t e = mt == 2 ? w4_seg<2, 2>(b, type, split, log_kw, st) : w4_seg<1, 1>(b, type, split, log_kw, st);
+    const cudaError_t e = w4_at(a.n > 8 ? 2 : 1, best.x_stride > 0, s32, w4_segment(a), a.zeros, W4Launch{b, type, best, st});
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
-// The most shared memory of any matrix: float32 scales of groups of 32, two buffers.
-template <int MT, int NT, int SEG, bool ZEROS>
-static cudaError_t w4_attr() {
-  const int most = kW4Warps * 2 * (kW4Chunk / 32 * (16 * MT * (4 + ZEROS) + 8 * NT * 4));
-  const cudaFuncAttribute at = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  cudaError_t e = cudaFuncSetAttribute(k_w4<MT, NT, SEG, ZEROS, float>, at, most);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_w4<MT, NT, SEG, ZEROS, __half>, at, most);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_w4<MT, NT, SEG, ZEROS, __nv_bfloat16>, at, most);
-  return e;
-}
-template <int MT, int NT>
-static cudaError_t w4_attrs() {
-  cudaError_t e = w4_attr<MT, NT, 32, false>();
-  if (e == cudaSuccess) e = w4_attr<MT, NT, 64, false>();
-  if (e == cudaSuccess) e = w4_attr<MT, NT, 128, false>();
-  if (e == cudaSuccess) e = w4_attr<MT, NT, 32, true>();
-  if (e == cudaSuccess) e = w4_attr<MT, NT, 64, true>();
-  if (e == cudaSuccess) e = w4_attr<MT, NT, 128, true>();
-  return e;
-}
+struct W4Init {
+  template <int NT, int SEG, bool ZEROS, bool XS, bool S32>
+  cudaError_t operator()() const {
+    return cudaFuncSetAttribute(k_w4<NT, SEG, ZEROS, XS, S32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4Smem);
+  }
+};
 
 cudaError_t init_w4_attributes() {
-  const cudaError_t e = w4_attrs<1, 1>();
-  return e != cudaSuccess ? e : w4_attrs<2, 2>();
+  for (int i = 0; i < 16; i++)
+    for (int seg = 32; seg <= 128; seg *= 2) {
+      const cudaError_t e = w4_at(1 + (i & 1), (i & 2) != 0, (i & 4) != 0, seg, (i & 8) != 0, W4Init{});
+      if (e != cudaSuccess) return e;
+    }
+  return cudaSuccess;
 }
 
 }  // namespace rk
