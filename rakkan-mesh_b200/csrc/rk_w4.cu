@@ -19,11 +19,14 @@
 // other than 8 adds (8 − z) · 16 Σ x, with Σ x made once for each segment.
 //
 // Work. One CTA of sixteen warps an SM goes through tiles of 16 rows. KW warps
-// of it (a team) share a tile's columns, or a cluster's CTAs do where there
-// are few rows; each warp keeps its share of the columns from tile to tile, so
-// the vectors and their scales are brought into shared memory once. The
-// records come through a ring of each warp in shared memory, which runs on
-// over the tiles: no load waits for a tile's end. (A CTA for each tile took
+// of it (a team) share a tile's columns; each warp keeps its share of the
+// columns from tile to tile, so the vectors and their scales are brought into
+// shared memory once (vectors that do not fit come with each record, from L2,
+// and so do scales that do not).
+// The records come through a ring of each warp in shared memory, which runs on
+// over the tiles: no load waits for a tile's end. Sharing a tile's columns over
+// the CTAs of a cluster was tried for vectors that do not fit and for few rows:
+// the exchange cost 1 to 3 us a tile. (A CTA for each tile took
 // 22.3 us for 28672x4096 by one vector: its beginning and end cost as much as
 // ten column pairs a warp, and the last wave of CTAs left SMs idle.) The
 // float32 sums of a tile's shares meet in shared memory, in order, while the
@@ -138,67 +141,80 @@ RK_DEV uint4 lds128(uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
+RK_DEV void copy4_s(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 RK_DEV void copy16_s(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-RK_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-RK_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// Stores v at `to` (an address in this CTA's shared memory) of the cluster's first CTA.
-RK_DEV void store_first(uint32_t to, float v) {
-  asm volatile(
-      "{\n\t.reg .b32 p;\n\t"
-      "mapa.shared::cluster.u32 p, %0, 0;\n\t"
-      "st.shared::cluster.f32 [p], %1;\n\t}" ::"r"(to),
-      "f"(v)
-      : "memory");
-}
-
 // How a product is dealt out, and its shared memory.
 struct W4Plan {
   int quads;      // stretches of 128 columns
   int log_kw;     // log2 of the warps of a team
-  int split;      // CTAs of a cluster, which share a tile's columns (then teams are whole CTAs)
-  int teams;      // of all CTAs or clusters
-  int cta_quads;  // stretches of a CTA, at most
-  int x_stride;   // bytes between vectors in shared memory; 0: they stay in global memory
+  int teams;      // of all CTAs
+  int vectors;    // W4_KEPT, ...
+  int x_stride;   // bytes between kept vectors
   int record, log_width;  // of the stream: bytes of a record, log2 of a segment's columns
-  int at_xs, at_ring, at_part, at_far, size;
+  int stage;      // bytes of a ring stage: a record, and the vectors' columns that come with it
+  int at_xs, at_ring, at_part, size;
 };
 // Stages of a warp's ring.
 __host__ __device__ constexpr int w4_depth(int nt) { return nt > 1 ? 3 : 4; }
 
-// NT tiles of 8 vectors; SEG columns share their scales; XS: the vectors lie
-// in shared memory; S32: float32 scales.
-template <int NT, int SEG, bool ZEROS, bool XS, bool S32>
+// Where the vectors lie: in shared memory, or they come with the records, or
+// their scales do too.
+enum { W4_KEPT = 2, W4_PASSING = 1, W4_ALL_PASSING = 0 };
+
+// NT tiles of 8 vectors; SEG columns share their scales; S32: float32 scales.
+template <int NT, int SEG, bool ZEROS, int VECTORS, bool S32>
 __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int out_type) {
   constexpr int DEPTH = w4_depth(NT), TILE = 16 * 8 * NT, SEGS = 128 / SEG, ENTRY = w4_entry(S32, ZEROS);
-  constexpr int XSB = ZEROS ? 8 : 4;  // bytes of a vector's entry for a segment: its scale / 16 (and 16 Σ x)
+  constexpr bool XS = VECTORS == W4_KEPT, ENTRIES = VECTORS != W4_ALL_PASSING, SUMS = ZEROS && ENTRIES;
+  constexpr int XSB = SUMS ? 8 : 4;  // bytes of a vector's entry for a segment: its scale / 16 (and 16 Σ x)
   extern __shared__ __align__(128) char sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
   const int kw = 1 << p.log_kw, tiles = (a.rows + 15) / 16;
-  const int rank = blockIdx.x & (p.split - 1);
-  const int team = p.split > 1 ? blockIdx.x / p.split : blockIdx.x * (kW4Warps >> p.log_kw) + (warp >> p.log_kw);
+  const int team = blockIdx.x * (kW4Warps >> p.log_kw) + (warp >> p.log_kw);
   const int v0 = blockIdx.y * 8 * NT, nv = min(8 * NT, a.n - v0);
-  // The CTA's columns, and this warp's.
-  const int cq0 = p.quads * rank / p.split, cq1 = p.quads * (rank + 1) / p.split;
-  const int share = warp & (kw - 1);
-  const int q0 = cq0 + (((cq1 - cq0) * share) >> p.log_kw), q1 = cq0 + (((cq1 - cq0) * (share + 1)) >> p.log_kw);
+  const int share = warp & (kw - 1);  // this warp's columns
+  const int q0 = (p.quads * share) >> p.log_kw, q1 = (p.quads * (share + 1)) >> p.log_kw;
 
   // The ring. Records left to copy, and left of the tile's share.
   const int len = q1 - q0, my_tiles = team < tiles ? (tiles - 1 - team) / p.teams + 1 : 0;
-  const uint32_t ring = s_addr(sm) + p.at_ring + warp * DEPTH * p.record, ring_end = ring + DEPTH * p.record;
+  const uint32_t ring = s_addr(sm) + p.at_ring + warp * DEPTH * p.stage, ring_end = ring + DEPTH * p.stage;
   int c_left = len * my_tiles, c_tile = len;
   uint32_t c_to = ring + 16 * lane;
   const uint8_t *c_from = a.w + ((int64_t)team * p.quads + q0) * p.record + 16 * lane;
   const int64_t c_jump = ((int64_t)p.teams * p.quads - len) * p.record;
   const bool c_tail = 1024 + 16 * lane < p.record;
+  // Vectors that come with the records: 16-byte piece lane % 8 of vector lane / 8 + 4i.
+  const int8_t *c_x = a.x + (int64_t)(v0 + (lane >> 3)) * a.cols + 128 * q0 + 16 * (lane & 7);
+  const uint32_t c_xto = p.record + (lane >> 3) * 128 + 16 * ((lane & 7) ^ (((lane >> 3) & 3) << 1)) - 16 * lane;
+  const bool c_tail_x = SEG < 128 && 128 * (q1 - 1) + 16 * (lane & 7) >= a.cols;  // behind the row's end in its last stretch
   auto copy = [&] {
     if (c_left > 0) {
       copy16_s(c_to, c_from);
       copy16_s(c_to + 512, c_from + 512);
       if (c_tail) copy16_s(c_to + 1024, c_from + 1024);
+      if (!XS) {
+#pragma unroll
+        for (int i = 0; i < 2 * NT; i++)
+          if ((lane >> 3) + 4 * i < nv && !(c_tile == 1 && c_tail_x)) copy16_s(c_to + c_xto + 512 * i, c_x + (int64_t)4 * i * a.cols);
+        c_x += 128;
+        if (c_tile == 1) c_x -= 128 * len;
+      }
+      if (!ENTRIES) {
+        const int col = 128 * (q1 - c_tile);
+#pragma unroll
+        for (int i = lane; i < SEGS * 8 * NT; i += 32) {
+          const int v = i % (8 * NT), at = col + SEG * (i / (8 * NT));
+          if (v < nv && at < a.cols)
+            copy4_s(c_to - 16 * lane + p.stage - SEGS * 8 * NT * 4 + 4 * i,
+                    a.x_scales + (int64_t)(v0 + v) * (a.cols / a.x_group) + at / a.x_group);
+        }
+      }
       c_from += p.record;
-      c_to += p.record;
+      c_to += p.stage;
       if (c_to >= ring_end) c_to = ring + 16 * lane;
       c_left--;
       if (--c_tile == 0) {
@@ -211,18 +227,17 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
 #pragma unroll
   for (int i = 0; i < DEPTH - 1; i++) copy();
 
-  // The CTA's columns of the vectors, and their entries: [segment][8 NT].
-  const int x0 = 128 * cq0, x_cols = min(a.cols, 128 * cq1) - x0;
+  // The vectors, and their entries: [segment][8 NT].
   if (XS)
-    for (int i = threadIdx.x; i < nv * (x_cols / 16); i += 32 * kW4Warps) {
-      const int v = i / (x_cols / 16), j = i % (x_cols / 16);
+    for (int i = threadIdx.x; i < nv * (a.cols / 16); i += 32 * kW4Warps) {
+      const int v = i / (a.cols / 16), j = i % (a.cols / 16);
       *reinterpret_cast<uint4 *>(sm + v * p.x_stride + 16 * j) =
-          __ldg(reinterpret_cast<const uint4 *>(a.x + (int64_t)(v0 + v) * a.cols + x0) + j);
+          __ldg(reinterpret_cast<const uint4 *>(a.x + (int64_t)(v0 + v) * a.cols) + j);
     }
-  for (int i = threadIdx.x; i < x_cols / SEG * 8 * NT; i += 32 * kW4Warps) {
-    const int v = v0 + min(i % (8 * NT), nv - 1), col = x0 + SEG * (i / (8 * NT));
+  for (int i = threadIdx.x; ENTRIES && i < a.cols / SEG * 8 * NT; i += 32 * kW4Warps) {
+    const int v = v0 + min(i % (8 * NT), nv - 1), col = SEG * (i / (8 * NT));
     const float s = __ldg(a.x_scales + (int64_t)v * (a.cols / a.x_group) + col / a.x_group) * 0.0625f;
-    if (ZEROS) {
+    if (SUMS) {
       const uint4 *at = reinterpret_cast<const uint4 *>(a.x + (int64_t)v * a.cols + col);
       int sum = 0;
 #pragma unroll
@@ -240,16 +255,15 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
   }
   __syncthreads();
 
-  // A vector behind the last is computed from the last one's, and not stored.
-  uint32_t xr[NT];
-  const int8_t *xg[NT];
+  // A vector behind the last is computed from the last one's (or from what
+  // lies in the ring), and not stored.
+  uint32_t xr[NT], x_step[4];
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
-    const int v = min(8 * n + r, nv - 1);
-    xr[n] = s_addr(sm) + v * p.x_stride + 128 * (q0 - cq0) + 8 * c;
-    xg[n] = a.x + (int64_t)(v0 + v) * a.cols + 128 * q0 + 8 * c;
-  }
-  const uint32_t x_first = s_addr(sm) + p.at_xs + (q0 - cq0) * SEGS * 8 * NT * XSB + 2 * c * XSB;
+  for (int n = 0; n < NT; n++)
+    xr[n] = XS ? s_addr(sm) + min(8 * n + r, nv - 1) * p.x_stride + 128 * q0 + 8 * c : p.record + (8 * n + r) * 128 + 8 * (c & 1);
+#pragma unroll
+  for (int s = 0; s < 4; s++) x_step[s] = XS ? 32 * s : 16 * ((2 * s + (c >> 1)) ^ ((r & 3) << 1));
+  const uint32_t x_first = s_addr(sm) + p.at_xs + q0 * SEGS * 8 * NT * XSB + 2 * c * XSB;
   // Where a step's scales lie in a record (SEG may be narrower than the weights' segments).
   uint32_t s_at[4];
 #pragma unroll
@@ -257,11 +271,9 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
   const bool bf16 = a.scale_type == RK_ACT_BF16;
   const auto half_scale = [&](uint32_t h) { return bf16 ? u2f(h << 16) : __half2float(__ushort_as_half((unsigned short)h)); };
 
-  float *part = reinterpret_cast<float *>(sm + p.at_part), *far = reinterpret_cast<float *>(sm + p.at_far);
+  float *part = reinterpret_cast<float *>(sm + p.at_part);
   uint32_t now = ring;
-  int flip = 0, far_tile = -1;
-  constexpr int MINE = (TILE + 32 * kW4Warps - 1) / (32 * kW4Warps);  // of a tile's sums, where the team is the CTA
-  float kept[MINE];
+  int flip = 0;
   // Element i of a tile's sums: neighbours are neighbouring rows of a vector.
   auto put = [&](int t, int i, float v) {
     const int64_t row = (int64_t)t * 16 + i % 16;
@@ -272,29 +284,17 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
     else if (out_type == RK_ACT_F16) act_store(static_cast<__half *>(a.out) + to, v);
     else act_store(static_cast<__nv_bfloat16 *>(a.out) + to, v);
   };
-  auto join_far = [&] {  // the first CTA of a cluster: the other CTAs' sums of tile far_tile have come
-#pragma unroll
-    for (int k = 0; k < MINE; k++) {
-      const int i = threadIdx.x + k * 32 * kW4Warps;
-      if (i >= TILE) break;
-      float v = kept[k];
-      for (int o = 1; o < p.split; o++) v += far[((flip ^ 1) * (p.split - 1) + o - 1) * TILE + i];
-      put(far_tile, i, v);
-    }
-  };
 
   for (int t = team; t < tiles; t += p.teams) {
     float acc[NT][4] = {};
-    uint32_t x_at = x_first, xq[NT];
-    const int8_t *xp[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) xq[n] = xr[n], xp[n] = xg[n];
+    uint32_t x_now = 0, x_at = x_first;
     for (int q = q0; q < q1; q++) {
       asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
       __syncwarp();
       copy();
       const uint4 w01 = lds128(now + 16 * lane), w23 = lds128(now + 512 + 16 * lane);
-      int sum[NT][4];
+      if (!ENTRIES) x_at = now + p.stage - SEGS * 8 * NT * 4 + 8 * c;
+      int sum[NT][4], ones[NT][4];
 #pragma unroll
       for (int s = 0; s < 4; s++) {
         if (SEG < 128 && 128 * q + 32 * s >= a.cols) break;  // rows may end inside a stretch
@@ -303,9 +303,14 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
         const uint32_t a0 = (lo << 4) & 0xf0f0f0f0u, a1 = (hi << 4) & 0xf0f0f0f0u, a2 = lo & 0xf0f0f0f0u, a3 = hi & 0xf0f0f0f0u;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-          const uint2 xv = XS ? lds64(xq[n] + 32 * s) : __ldg(reinterpret_cast<const uint2 *>(xp[n] + 32 * s));
+          const uint2 xv = lds64((XS ? x_now : now) + xr[n] + x_step[s]);
           if (s * 32 % SEG == 0) imma_first(sum[n], a0, a1, a2, a3, xv.x, xv.y);
           else imma(sum[n], a0, a1, a2, a3, xv.x, xv.y);
+          if constexpr (ZEROS && !ENTRIES) {
+            constexpr uint32_t all = 0x10101010u;
+            if (s * 32 % SEG == 0) imma_first(ones[n], all, all, all, all, xv.x, xv.y);
+            else imma(ones[n], all, all, all, all, xv.x, xv.y);
+          }
         }
         if ((s + 1) * 32 % SEG == 0) {  // a segment ends
           float sw[2];
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
 #pragma unroll
           for (int n = 0; n < NT; n++) {
             float f[2];  // of vectors 2c and 2c + 1
-            if constexpr (ZEROS) {
+            if constexpr (SUMS) {
               const uint4 e = lds128(x_at + 8 * n * XSB);
               f[0] = u2f(e.x), f[1] = u2f(e.z);
               sum[n][0] += z[0] * (int)e.y;
@@ -336,6 +341,10 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
             } else {
               const uint2 e = lds64(x_at + 8 * n * XSB);
               f[0] = u2f(e.x), f[1] = u2f(e.y);
+              if (!ENTRIES) f[0] *= 0.0625f, f[1] *= 0.0625f;
+              if (ZEROS)
+#pragma unroll
+                for (int k = 0; k < 4; k++) sum[n][k] += z[k >> 1] * ones[n][k];
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[n][e] = fmaf((float)sum[n][e], sw[e >> 1] * f[e & 1], acc[n][e]);
@@ -343,9 +352,8 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
           x_at += 8 * NT * XSB;
         }
       }
-#pragma unroll
-      for (int n = 0; n < NT; n++) xq[n] += 128, xp[n] += 128;
-      now += p.record;
+      x_now += 128;
+      now += p.stage;
       if (now == ring_end) now = ring;
     }
     // The team's sums: one barrier a tile, since the next tile's go to the
@@ -358,87 +366,63 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
     if (p.log_kw == 0) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(warp >> p.log_kw), "r"(32 << p.log_kw) : "memory");
     const float *first = part + (flip * kW4Warps + (warp & ~(kw - 1))) * TILE;
-    if (p.split == 1) {
-      for (int i = share * 32 + lane; i < TILE; i += 32 << p.log_kw) {
-        float v = first[i];
-        for (int k = 1; k < kw; k++) v += first[k * TILE + i];
-        put(t, i, v);
-      }
-      flip ^= 1;
-    } else {
-      float here[MINE];
-#pragma unroll
-      for (int k = 0; k < MINE; k++) {
-        const int i = threadIdx.x + k * 32 * kW4Warps;
-        here[k] = 0.0f;
-        if (i < TILE) {
-          here[k] = first[i];
-          for (int o = 1; o < kw; o++) here[k] += first[o * TILE + i];
-        }
-      }
-      // The other CTAs' sums of the tile before have come: they are waited for a tile late.
-      if (far_tile >= 0) {
-        cluster_wait();
-        if (rank == 0) join_far();
-      } else {  // every CTA of the cluster has begun, before its memory is written
-        cluster_arrive();
-        cluster_wait();
-      }
-#pragma unroll
-      for (int k = 0; k < MINE; k++) {
-        const int i = threadIdx.x + k * 32 * kW4Warps;
-        if (rank == 0) kept[k] = here[k];
-        else if (i < TILE) store_first(s_addr(far + (flip * (p.split - 1) + rank - 1) * TILE + i), here[k]);
-      }
-      cluster_arrive();
-      far_tile = t;
-      flip ^= 1;
+    for (int i = share * 32 + lane; i < TILE; i += 32 << p.log_kw) {
+      float v = first[i];
+      for (int k = 1; k < kw; k++) v += first[k * TILE + i];
+      put(t, i, v);
     }
-  }
-  if (p.split > 1 && far_tile >= 0) {
-    cluster_wait();
-    if (rank == 0) join_far();
+    flip ^= 1;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Shared memory of a plan (teams, log_kw, split set); the vectors go to
-// shared memory if that fits.
+// Shared memory of a plan; the vectors go there if they fit.
 static void w4_layout_smem(const W4Args &a, W4Plan &p) {
   const int nt = a.n > 8 ? 2 : 1, nv = a.n < 8 * nt ? a.n : 8 * nt;
-  p.cta_quads = (p.quads + p.split - 1) / p.split;
-  const int xs = (128 * p.cta_quads / w4_segment(a) * 8 * nt * (a.zeros ? 8 : 4) + 127) / 128 * 128;
-  const int ring = (kW4Warps * w4_depth(nt) * p.record + 127) / 128 * 128;
-  const int part = 2 * kW4Warps * 16 * 8 * nt * 4, far = 2 * (p.split - 1) * 16 * 8 * nt * 4;
-  p.x_stride = 128 * p.cta_quads + 32;  // rows of eight lanes' reads fall on different banks
-  if ((int64_t)nv * p.x_stride + 128 + xs + ring + part + far > kW4Smem) p.x_stride = 0;
+  const int64_t xs = ((int64_t)a.cols / w4_segment(a) * 8 * nt * (a.zeros ? 8 : 4) + 127) / 128 * 128;
+  const int part = 2 * kW4Warps * 16 * 8 * nt * 4;
+  const auto ring = [&] { return (kW4Warps * w4_depth(nt) * p.stage + 127) / 128 * 128; };
+  p.vectors = W4_KEPT;
+  p.stage = p.record;
+  p.x_stride = 128 * p.quads + 32;  // rows of eight lanes' reads fall on different banks
+  int64_t entries = xs;
+  if ((int64_t)nv * p.x_stride + 128 + xs + ring() + part > kW4Smem) {
+    p.vectors = W4_PASSING;
+    p.stage += 8 * nt * 128;
+    p.x_stride = 0;
+    if (xs + ring() + part > kW4Smem) {
+      p.vectors = W4_ALL_PASSING;
+      p.stage += 128 / w4_segment(a) * 8 * nt * 4;
+      entries = 0;
+    }
+  }
   p.at_xs = (nv * p.x_stride + 127) / 128 * 128;
-  p.at_ring = p.at_xs + xs;
-  p.at_part = p.at_ring + ring;
-  p.at_far = p.at_part + part;
-  p.size = p.at_far + far;
+  p.at_ring = (int)(p.at_xs + entries);
+  p.at_part = p.at_ring + ring();
+  p.size = p.at_part + part;
 }
 
-// f<NT, SEG, ZEROS, XS, S32>() of the instance for a product.
-template <int NT, bool XS, bool S32, class F>
+// f<NT, SEG, ZEROS, VECTORS, S32>() of the instance for a product.
+template <int NT, int VECTORS, bool S32, class F>
 static cudaError_t w4_seg(int seg, bool zeros, F f) {
   if (zeros) {
-    if (seg == 128) return f.template operator()<NT, 128, true, XS, S32>();
-    if (seg == 64) return f.template operator()<NT, 64, true, XS, S32>();
-    return f.template operator()<NT, 32, true, XS, S32>();
+    if (seg == 128) return f.template operator()<NT, 128, true, VECTORS, S32>();
+    if (seg == 64) return f.template operator()<NT, 64, true, VECTORS, S32>();
+    return f.template operator()<NT, 32, true, VECTORS, S32>();
   }
-  if (seg == 128) return f.template operator()<NT, 128, false, XS, S32>();
-  if (seg == 64) return f.template operator()<NT, 64, false, XS, S32>();
-  return f.template operator()<NT, 32, false, XS, S32>();
+  if (seg == 128) return f.template operator()<NT, 128, false, VECTORS, S32>();
+  if (seg == 64) return f.template operator()<NT, 64, false, VECTORS, S32>();
+  return f.template operator()<NT, 32, false, VECTORS, S32>();
+}
+template <int NT, bool S32, class F>
+static cudaError_t w4_vec(int vectors, int seg, bool zeros, F f) {
+  if (vectors == W4_KEPT) return w4_seg<NT, W4_KEPT, S32>(seg, zeros, f);
+  return vectors == W4_PASSING ? w4_seg<NT, W4_PASSING, S32>(seg, zeros, f) : w4_seg<NT, W4_ALL_PASSING, S32>(seg, zeros, f);
 }
 template <class F>
-static cudaError_t w4_at(int nt, bool xs, bool s32, int seg, bool zeros, F f) {
-  if (nt > 1) {
-    if (xs) return s32 ? w4_seg<2, true, true>(seg, zeros, f) : w4_seg<2, true, false>(seg, zeros, f);
-    return s32 ? w4_seg<2, false, true>(seg, zeros, f) : w4_seg<2, false, false>(seg, zeros, f);
-  }
-  if (xs) return s32 ? w4_seg<1, true, true>(seg, zeros, f) : w4_seg<1, true, false>(seg, zeros, f);
-  return s32 ? w4_seg<1, false, true>(seg, zeros, f) : w4_seg<1, false, false>(seg, zeros, f);
+static cudaError_t w4_at(int nt, int vectors, bool s32, int seg, bool zeros, F f) {
+  if (nt > 1) return s32 ? w4_vec<2, true>(vectors, seg, zeros, f) : w4_vec<2, false>(vectors, seg, zeros, f);
+  return s32 ? w4_vec<1, true>(vectors, seg, zeros, f) : w4_vec<1, false>(vectors, seg, zeros, f);
 }
 
 struct W4Launch {
@@ -446,45 +430,34 @@ struct W4Launch {
   int type;
   const W4Plan &p;
   cudaStream_t st;
-  template <int NT, int SEG, bool ZEROS, bool XS, bool S32>
+  template <int NT, int SEG, bool ZEROS, int VECTORS, bool S32>
   cudaError_t operator()() const {
-    const int ctas = p.split > 1 ? p.teams * p.split : p.teams / (kW4Warps >> p.log_kw);
-    const dim3 grid(ctas, (unsigned)((a.n + 8 * NT - 1) / (8 * NT))), cl(p.split, 1, 1);
-    return launch_kc(k_w4<NT, SEG, ZEROS, XS, S32>, grid, 32 * kW4Warps, cl, p.size, st, a, p, type);
+    const dim3 grid(p.teams / (kW4Warps >> p.log_kw), (unsigned)((a.n + 8 * NT - 1) / (8 * NT)));
+    return launch_k(k_w4<NT, SEG, ZEROS, VECTORS, S32>, grid, 32 * kW4Warps, p.size, st, a, p, type);
   }
 };
 
 cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st) {
   const int tiles = (a.rows + 15) / 16;
   const bool s32 = a.scale_type == RK_ACT_F32;
-  W4Plan best{};
-  double least = 0;
-  // The time of a plan in stretches: a team's tiles, each its longest share and
-  // an end (about two stretches' instructions; another four for the exchange in
-  // a cluster); vectors that stay in global memory take four times as long.
-  const auto take = [&](int log_kw, int split) {
-    W4Plan p{};
-    p.quads = (a.cols + 127) / 128;
-    p.log_kw = log_kw;
-    p.split = split;
-    p.record = w4_record(a.group, s32, a.zeros);
-    p.log_width = w4_width(a.group) == 128 ? 7 : w4_width(a.group) == 64 ? 6 : 5;
-    w4_layout_smem(a, p);
-    if (p.size > kW4Smem) return;
-    const int units = split > 1 ? sms / split : sms * (kW4Warps >> log_kw);
-    const int rounds = (tiles + units - 1) / units;
-    const int share = (p.cta_quads + (1 << log_kw) - 1) >> log_kw;
-    const double cost = rounds * (share * (p.x_stride ? 1.0 : 4.0) + 2 + (split > 1 ? 4 : 0));
-    const int per_cta = kW4Warps >> log_kw;
-    p.teams = split > 1 ? (tiles < units ? tiles : units) : (tiles < units ? (tiles + per_cta - 1) / per_cta * per_cta : units);
-    if (least == 0 || cost < least) {
-      least = cost;
-      best = p;
+  W4Plan p{};
+  p.quads = (a.cols + 127) / 128;
+  p.record = w4_record(a.group, s32, a.zeros);
+  p.log_width = w4_width(a.group) == 128 ? 7 : w4_width(a.group) == 64 ? 6 : 5;
+  w4_layout_smem(a, p);
+  if (p.size > kW4Smem) return cudaErrorInvalidValue;
+  // Teams of the size that ends soonest, counted in stretches: the tiles of a
+  // team, each its longest share and an end, which costs about two stretches.
+  int least = 0x7fffffff;
+  for (int log_kw = 4; log_kw >= 0; log_kw--) {
+    const int per_cta = kW4Warps >> log_kw, units = sms * per_cta;
+    const int64_t cost = (int64_t)((tiles + units - 1) / units) * (((p.quads + (1 << log_kw) - 1) >> log_kw) + 2);
+    if (cost < least) {
+      least = (int)cost;
+      p.log_kw = log_kw;
+      p.teams = tiles < units ? (tiles + per_cta - 1) / per_cta * per_cta : units;
     }
-  };
-  for (int k = 4; k >= 0; k--) take(k, 1);
-  for (int s = 2; s <= 8; s *= 2) take(4, s);
-  if (least == 0) return cudaErrorInvalidValue;
+  }
   const int64_t width = 65535LL * 8;  // of grid.y
   for (int64_t v = 0; v < a.n; v += width) {
     W4Args b = a;
@@ -492,23 +465,23 @@ cudaError_t launch_w4_mulvec(const W4Args &a, int type, int sms, cudaStream_t st
     b.x += v * a.cols;
     b.x_scales += v * (a.cols / a.x_group);
     b.out = static_cast<char *>(a.out) + v * a.out_stride * (type == RK_ACT_F32 ? 4 : 2);
-    const cudaError_t e = w4_at(a.n > 8 ? 2 : 1, best.x_stride > 0, s32, w4_segment(a), a.zeros, W4Launch{b, type, best, st});
+    const cudaError_t e = w4_at(a.n > 8 ? 2 : 1, p.vectors, s32, w4_segment(a), a.zeros, W4Launch{b, type, p, st});
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
 struct W4Init {
-  template <int NT, int SEG, bool ZEROS, bool XS, bool S32>
+  template <int NT, int SEG, bool ZEROS, int VECTORS, bool S32>
   cudaError_t operator()() const {
-    return cudaFuncSetAttribute(k_w4<NT, SEG, ZEROS, XS, S32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4Smem);
+    return cudaFuncSetAttribute(k_w4<NT, SEG, ZEROS, VECTORS, S32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4Smem);
   }
 };
 
 cudaError_t init_w4_attributes() {
-  for (int i = 0; i < 16; i++)
+  for (int i = 0; i < 24; i++)
     for (int seg = 32; seg <= 128; seg *= 2) {
-      const cudaError_t e = w4_at(1 + (i & 1), (i & 2) != 0, (i & 4) != 0, seg, (i & 8) != 0, W4Init{});
+      const cudaError_t e = w4_at(1 + (i & 1), i / 8, (i & 2) != 0, seg, (i & 4) != 0, W4Init{});
       if (e != cudaSuccess) return e;
     }
   return cudaSuccess;
