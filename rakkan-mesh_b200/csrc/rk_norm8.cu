@@ -1,18 +1,195 @@
 // rk_norm8.cu — residual addition and RMSNorm with an 8-bit output.
+//
+//   h = x + residual,  u = h·w,  base = max|u| / 127 over a group,
+//   q = round(u / base),  scale = base / sqrt(mean(h²) + eps).
+// The integers do not depend on the row's norm (it cancels in u / base), so a
+// row is read once: h and u stay in registers, the integers are stored while
+// the sum of squares is still on its way through the CTA, and only the scales
+// wait for it. The bytes of x, residual, sum and q bound the call.
+//
+// A CTA takes a row, a thread K pieces of VEC neighbours (16 bytes, or single
+// values where rows or groups do not lie on 16-byte boundaries); a group is a
+// power of two of lanes, whose largest magnitude is found by shuffles, or the
+// whole row. Other groups take a kernel that keeps h in shared memory.
 #include "rk_act.cuh"
 #include "rk_serve.cuh"
 
 namespace rk {
 
-// A CTA per row, a warp per group in turn: h is formed, stored and squared
-// on the first reading, the groups' magnitudes and integers on the second.
-constexpr int kNormThreads = 256;
+template <int VEC>
+RK_DEV void norm_load(const float *p, float *v) {
+  if constexpr (VEC == 4) {
+    const float4 x = *reinterpret_cast<const float4 *>(p);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int VEC, class T>
+RK_DEV void norm_load(const T *p, float *v) {
+  if constexpr (VEC == 8) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const T *h = reinterpret_cast<const T *>(&w[i]);
+      v[2 * i] = act_load(h);
+      v[2 * i + 1] = act_load(h + 1);
+    }
+  } else {
+    v[0] = act_load(p);
+  }
+}
+template <int VEC>
+RK_DEV void norm_store(float *p, const float *v) {
+  if constexpr (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *p = v[0];
+}
+template <int VEC, class T>
+RK_DEV void norm_store(T *p, const float *v) {
+  if constexpr (VEC == 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      T *h = reinterpret_cast<T *>(&w[i]);
+      act_store(h, v[2 * i]);
+      act_store(h + 1, v[2 * i + 1]);
+    }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    act_store(p, v[0]);
+  }
+}
+
+RK_DEV float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+RK_DEV float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+// 1 / sqrt(mean + eps), both operations rounded once.
+RK_DEV float norm_recip(float ss, int cols, float eps) { return __frcp_rn(__fsqrt_rn(ss / (float)cols + eps)); }
+// base of a group's largest magnitude, and the factor of its values.
+RK_DEV float norm_base(float m, float &inv) {
+  float base = __fmul_rn(m, u2f(K_1_127));
+  if (base < u2f(K_TINY)) base = 0.0f;
+  inv = base > 0.0f ? __frcp_rn(base) : 0.0f;
+  return base;
+}
+
+// lanes: of a group (a power of two up to 32); 0: the group is the row.
+template <class T, int VEC, int K>
+__global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int lanes) {
+  __shared__ float sh[32], sh_max[32];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+  const T *res = static_cast<const T *>(a.residual) + (a.residual ? row * a.r_stride : 0);
+  const T *w = static_cast<const T *>(a.weight);
+  T *sum = static_cast<T *>(a.sum_out) + (a.sum_out ? row * a.s_stride : 0);
+  int8_t *q = a.q + row * a.cols;
+  float h[K][VEC], u[K][VEC], ss = 0.0f, top[K], base[K];
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int at = VEC * ((int)threadIdx.x + k * (int)blockDim.x);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) h[k][i] = u[k][i] = 0.0f;
+    if (at < a.cols) {
+      norm_load<VEC>(x + at, h[k]);
+      norm_load<VEC>(w + at, u[k]);
+    }
+  }
+  if (a.residual) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const int at = VEC * ((int)threadIdx.x + k * (int)blockDim.x);
+      if (at < a.cols) {
+        float r[VEC];
+        norm_load<VEC>(res + at, r);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) h[k][i] = __fadd_rn(h[k][i], r[i]);
+      }
+    }
+  }
+  float all = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int at = VEC * ((int)threadIdx.x + k * (int)blockDim.x);
+    top[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {
+      ss = fmaf(h[k][i], h[k][i], ss);
+      u[k][i] = __fmul_rn(h[k][i], u[k][i]);
+      top[k] = fmaxf(top[k], fabsf(u[k][i]));
+    }
+    if (a.sum_out && at < a.cols) norm_store<VEC>(sum + at, h[k]);
+    all = fmaxf(all, top[k]);
+  }
+  auto store = [&](int k, float inv) {
+    const int at = VEC * ((int)threadIdx.x + k * (int)blockDim.x);
+    if (at >= a.cols) return;
+    int v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; i++) v[i] = quant127(u[k][i], inv);
+    if constexpr (VEC == 1) {
+      q[at] = (int8_t)v[0];
+    } else {
+      uint32_t p[VEC / 4];
+#pragma unroll
+      for (int i = 0; i < VEC / 4; i++)
+        p[i] = (v[4 * i] & 255) | (v[4 * i + 1] & 255) << 8 | (v[4 * i + 2] & 255) << 16 | (uint32_t)v[4 * i + 3] << 24;
+      if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(q + at) = make_uint2(p[0], p[1]);
+      else *reinterpret_cast<uint32_t *>(q + at) = p[0];
+    }
+  };
+  ss = warp_sum(ss);
+  if (lanes == 0) all = warp_max(all);
+  if (lane == 0) {
+    sh[warp] = ss;
+    sh_max[warp] = all;
+  }
+  if (lanes) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      for (int o = 1; o < lanes; o <<= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+      float inv;
+      base[k] = norm_base(top[k], inv);
+      store(k, inv);
+    }
+  }
+  __syncthreads();
+  ss = lane < warps ? sh[lane] : 0.0f;
+  const float r = norm_recip(warp_sum(ss), a.cols, a.eps);
+  if (lanes == 0) {
+    float inv;
+    const float b = norm_base(warp_max(lane < warps ? sh_max[lane] : 0.0f), inv);
+#pragma unroll
+    for (int k = 0; k < K; k++) store(k, inv);
+    if (threadIdx.x == 0) a.scales[row] = __fmul_rn(b, r);
+  } else if (threadIdx.x % lanes == 0) {
+    float *scales = a.scales + row * (a.cols / a.group);
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const int piece = (int)threadIdx.x + k * (int)blockDim.x;
+      if (VEC * piece < a.cols) scales[piece / lanes] = __fmul_rn(base[k], r);
+    }
+  }
+}
+
+// Any group: h in shared memory where a row fits (else read again), a warp
+// per group in turn.
+constexpr int kNormThreads = 256, kNormShared = 12000;
 
 template <class T>
-__global__ void __launch_bounds__(kNormThreads) k_norm8_rows(Norm8Args a) {
-  __shared__ float sh[kNormThreads / 32];
+__global__ void __launch_bounds__(kNormThreads) k_norm8_any(Norm8Args a) {
+  __shared__ float sh[kNormThreads / 32], keep[kNormShared];
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool kept = a.cols <= kNormShared;
   const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
   const T *res = a.residual ? static_cast<const T *>(a.residual) + row * a.r_stride : nullptr;
   const T *w = static_cast<const T *>(a.weight);
@@ -20,42 +197,75 @@ __global__ void __launch_bounds__(kNormThreads) k_norm8_rows(Norm8Args a) {
   float ss = 0.0f;
   for (int j = threadIdx.x; j < a.cols; j += kNormThreads) {
     const float h = h_of(j);
+    if (kept) keep[j] = h;
     ss = fmaf(h, h, ss);
   }
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  ss = warp_sum(ss);
   if (lane == 0) sh[warp] = ss;
   __syncthreads();
   ss = 0.0f;
   for (int i = 0; i < kNormThreads / 32; i++) ss += sh[i];
-  const float r = __frcp_rn(__fsqrt_rn(ss / (float)a.cols + a.eps));
+  const float r = norm_recip(ss, a.cols, a.eps);
   const int groups = a.cols / a.group;
   for (int g = warp; g < groups; g += kNormThreads / 32) {
     float m = 0.0f;
     for (int j = lane; j < a.group; j += 32) {
       const int c = g * a.group + j;
-      m = fmaxf(m, fabsf(__fmul_rn(h_of(c), act_load(w + c))));
+      m = fmaxf(m, fabsf(__fmul_rn(kept ? keep[c] : h_of(c), act_load(w + c))));
     }
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float base = __fmul_rn(m, u2f(K_1_127));
-    if (base < u2f(K_TINY)) base = 0.0f;
-    const float inv = base > 0.0f ? __fdiv_rn(1.0f, base) : 0.0f;
+    float inv;
+    const float base = norm_base(warp_max(m), inv);
     for (int j = lane; j < a.group; j += 32) {
       const int c = g * a.group + j;
-      a.q[row * a.cols + c] = (int8_t)quant127(__fmul_rn(h_of(c), act_load(w + c)), inv);
+      a.q[row * a.cols + c] = (int8_t)quant127(__fmul_rn(kept ? keep[c] : h_of(c), act_load(w + c)), inv);
     }
     if (lane == 0) a.scales[row * groups + g] = __fmul_rn(base, r);
   }
   if (!a.sum_out) return;
   __syncthreads();  // sum_out may be x or the residual
   T *sum = static_cast<T *>(a.sum_out) + row * a.s_stride;
-  for (int j = threadIdx.x; j < a.cols; j += kNormThreads) act_store(sum + j, h_of(j));
+  for (int j = threadIdx.x; j < a.cols; j += kNormThreads) act_store(sum + j, kept ? keep[j] : h_of(j));
 }
 
-cudaError_t launch_add_rmsnorm_q8(const Norm8Args &a, int type, int, cudaStream_t st) {
+template <class T, int VEC>
+static cudaError_t norm_pieces(const Norm8Args &a, int sms, int lanes, cudaStream_t st, bool &taken) {
+  // Few rows: as many threads as pieces. Many: CTAs of up to 512, so that
+  // several share an SM and one's loads pass while another waits.
+  const int pieces = a.cols / VEC, most = a.rows >= 2 * sms ? 512 : 1024;
+  const auto threads = [&](int k) { return ((pieces + k - 1) / k + 31) / 32 * 32; };
+  taken = true;
+  if (threads(1) <= most) return launch_k(k_norm8<T, VEC, 1>, a.rows, threads(1), 0, st, a, lanes);
+  if (threads(2) <= most) return launch_k(k_norm8<T, VEC, 2>, a.rows, threads(2), 0, st, a, lanes);
+  if (threads(4) <= 512) return launch_k(k_norm8<T, VEC, 4>, a.rows, threads(4), 0, st, a, lanes);
+  if (threads(8) <= 512) return launch_k(k_norm8<T, VEC, 8>, a.rows, threads(8), 0, st, a, lanes);
+  taken = false;
+  return cudaSuccess;
+}
+
+template <class T>
+static cudaError_t norm_typed(const Norm8Args &a, int sms, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  const auto on16 = [](const void *p, int64_t stride) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % VEC == 0;
+  };
+  const bool vec = a.cols % VEC == 0 && on16(a.x, a.x_stride) && on16(a.weight, 0) && (!a.residual || on16(a.residual, a.r_stride)) &&
+                   (!a.sum_out || on16(a.sum_out, a.s_stride)) && (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
+  const auto lanes_of = [&](int v) {  // -1: no power of two of lanes
+    const int n = a.group % v ? 0 : a.group / v;
+    return a.group == a.cols ? 0 : n >= 1 && n <= 32 && (n & (n - 1)) == 0 ? n : -1;
+  };
+  bool taken = false;
+  cudaError_t e = cudaSuccess;
+  if (vec && lanes_of(VEC) >= 0) e = norm_pieces<T, VEC>(a, sms, lanes_of(VEC), st, taken);
+  else if (lanes_of(1) >= 0) e = norm_pieces<T, 1>(a, sms, lanes_of(1), st, taken);
+  return taken ? e : launch_k(k_norm8_any<T>, a.rows, kNormThreads, 0, st, a);
+}
+
+cudaError_t launch_add_rmsnorm_q8(const Norm8Args &a, int type, int sms, cudaStream_t st) {
   switch (type) {
-    case RK_ACT_F32: return launch_k(k_norm8_rows<float>, a.rows, kNormThreads, 0, st, a);
-    case RK_ACT_F16: return launch_k(k_norm8_rows<__half>, a.rows, kNormThreads, 0, st, a);
-    default: return launch_k(k_norm8_rows<__nv_bfloat16>, a.rows, kNormThreads, 0, st, a);
+    case RK_ACT_F32: return norm_typed<float>(a, sms, st);
+    case RK_ACT_F16: return norm_typed<__half>(a, sms, st);
+    default: return norm_typed<__nv_bfloat16>(a, sms, st);
   }
 }
 
