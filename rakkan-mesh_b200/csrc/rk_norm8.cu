@@ -16,30 +16,31 @@
 
 namespace rk {
 
-template <int VEC>
-RK_DEV void norm_load(const float *p, float *v) {
-  if constexpr (VEC == 4) {
-    const float4 x = *reinterpret_cast<const float4 *>(p);
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-  } else {
-    v[0] = *p;
-  }
-}
-template <int VEC, class T>
-RK_DEV void norm_load(const T *p, float *v) {
-  if constexpr (VEC == 8) {
-    const uint4 x = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+// VEC values as they lie in memory.
+template <class T, int VEC>
+struct Piece {
+  uint4 bits;
+  RK_DEV void load(const T *p) { bits = *reinterpret_cast<const uint4 *>(p); }
+  RK_DEV void values(float *v) const {
+    const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const T *h = reinterpret_cast<const T *>(&w[i]);
-      v[2 * i] = act_load(h);
-      v[2 * i + 1] = act_load(h + 1);
+      if constexpr (sizeof(T) == 4) {
+        v[i] = u2f(w[i]);
+      } else {
+        const T *h = reinterpret_cast<const T *>(&w[i]);
+        v[2 * i] = act_load(h);
+        v[2 * i + 1] = act_load(h + 1);
+      }
     }
-  } else {
-    v[0] = act_load(p);
   }
-}
+};
+template <class T>
+struct Piece<T, 1> {
+  T bits;
+  RK_DEV void load(const T *p) { bits = *p; }
+  RK_DEV void values(float *v) const { v[0] = act_load(&bits); }
+};
 template <int VEC>
 RK_DEV void norm_store(float *p, const float *v) {
   if constexpr (VEC == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -81,101 +82,104 @@ RK_DEV float norm_base(float m, float &inv) {
   return base;
 }
 
-// lanes: of a group (a power of two up to 32); 0: the group is the row.
+// lanes: of a group (a power of two up to 32); 0: the group is the row. A CTA
+// takes every gridDim.x-th row and loads the next one before it waits for a
+// row's sum (41.9 us for 4096x5120 bfloat16 with a CTA a row and no loads in
+// flight meanwhile).
 template <class T, int VEC, int K>
 __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int lanes) {
-  __shared__ float sh[32], sh_max[32];
-  const int64_t row = blockIdx.x;
+  __shared__ float sh[2][32], sh_max[2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-  const T *res = static_cast<const T *>(a.residual) + (a.residual ? row * a.r_stride : 0);
-  const T *w = static_cast<const T *>(a.weight);
-  T *sum = static_cast<T *>(a.sum_out) + (a.sum_out ? row * a.s_stride : 0);
-  int8_t *q = a.q + row * a.cols;
-  float h[K][VEC], u[K][VEC], ss = 0.0f, top[K], base[K];
+  const auto at_of = [&](int k) { return VEC * ((int)threadIdx.x + k * (int)blockDim.x); };
+  Piece<T, VEC> x[K], res[K], w[K];
+  const auto load = [&](int64_t row) {
 #pragma unroll
-  for (int k = 0; k < K; k++) {
-    const int at = VEC * ((int)threadIdx.x + k * (int)blockDim.x);
+    for (int k = 0; k < K; k++)
+      if (at_of(k) < a.cols) {
+        x[k].load(static_cast<const T *>(a.x) + row * a.x_stride + at_of(k));
+        if (a.residual) res[k].load(static_cast<const T *>(a.residual) + row * a.r_stride + at_of(k));
+      }
+  };
+  load(blockIdx.x);
 #pragma unroll
-    for (int i = 0; i < VEC; i++) h[k][i] = u[k][i] = 0.0f;
-    if (at < a.cols) {
-      norm_load<VEC>(x + at, h[k]);
-      norm_load<VEC>(w + at, u[k]);
-    }
-  }
-  if (a.residual) {
+  for (int k = 0; k < K; k++)
+    if (at_of(k) < a.cols) w[k].load(static_cast<const T *>(a.weight) + at_of(k));
+
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
+    int8_t *q = a.q + row * a.cols;
+    float u[K][VEC], ss = 0.0f, top[K], base[K], all = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      const int at = VEC * ((int)threadIdx.x + k * (int)blockDim.x);
-      if (at < a.cols) {
-        float r[VEC];
-        norm_load<VEC>(res + at, r);
+      top[k] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < VEC; i++) h[k][i] = __fadd_rn(h[k][i], r[i]);
+      for (int i = 0; i < VEC; i++) u[k][i] = 0.0f;
+      if (at_of(k) < a.cols) {
+        float h[VEC], f[VEC];
+        x[k].values(h);
+        if (a.residual) {
+          res[k].values(f);
+#pragma unroll
+          for (int i = 0; i < VEC; i++) h[i] = __fadd_rn(h[i], f[i]);
+        }
+        if (a.sum_out) norm_store<VEC>(static_cast<T *>(a.sum_out) + row * a.s_stride + at_of(k), h);
+        w[k].values(f);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          ss = fmaf(h[i], h[i], ss);
+          u[k][i] = __fmul_rn(h[i], f[i]);
+          top[k] = fmaxf(top[k], fabsf(u[k][i]));
+        }
+      }
+      all = fmaxf(all, top[k]);
+    }
+    if (row + gridDim.x < a.rows) load(row + gridDim.x);
+    auto store = [&](int k, float inv) {
+      const int at = at_of(k);
+      if (at >= a.cols) return;
+      int v[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; i++) v[i] = quant127(u[k][i], inv);
+      if constexpr (VEC == 1) {
+        q[at] = (int8_t)v[0];
+      } else {
+        uint32_t p[VEC / 4];
+#pragma unroll
+        for (int i = 0; i < VEC / 4; i++)
+          p[i] = (v[4 * i] & 255) | (v[4 * i + 1] & 255) << 8 | (v[4 * i + 2] & 255) << 16 | (uint32_t)v[4 * i + 3] << 24;
+        if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(q + at) = make_uint2(p[0], p[1]);
+        else *reinterpret_cast<uint32_t *>(q + at) = p[0];
+      }
+    };
+    ss = warp_sum(ss);
+    if (lanes == 0) all = warp_max(all);
+    if (lane == 0) {
+      sh[flip][warp] = ss;
+      sh_max[flip][warp] = all;
+    }
+    if (lanes) {
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        for (int o = 1; o < lanes; o <<= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+        float inv;
+        base[k] = norm_base(top[k], inv);
+        store(k, inv);
       }
     }
-  }
-  float all = 0.0f;
-#pragma unroll
-  for (int k = 0; k < K; k++) {
-    const int at = VEC * ((int)threadIdx.x + k * (int)blockDim.x);
-    top[k] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      ss = fmaf(h[k][i], h[k][i], ss);
-      u[k][i] = __fmul_rn(h[k][i], u[k][i]);
-      top[k] = fmaxf(top[k], fabsf(u[k][i]));
-    }
-    if (a.sum_out && at < a.cols) norm_store<VEC>(sum + at, h[k]);
-    all = fmaxf(all, top[k]);
-  }
-  auto store = [&](int k, float inv) {
-    const int at = VEC * ((int)threadIdx.x + k * (int)blockDim.x);
-    if (at >= a.cols) return;
-    int v[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; i++) v[i] = quant127(u[k][i], inv);
-    if constexpr (VEC == 1) {
-      q[at] = (int8_t)v[0];
-    } else {
-      uint32_t p[VEC / 4];
-#pragma unroll
-      for (int i = 0; i < VEC / 4; i++)
-        p[i] = (v[4 * i] & 255) | (v[4 * i + 1] & 255) << 8 | (v[4 * i + 2] & 255) << 16 | (uint32_t)v[4 * i + 3] << 24;
-      if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(q + at) = make_uint2(p[0], p[1]);
-      else *reinterpret_cast<uint32_t *>(q + at) = p[0];
-    }
-  };
-  ss = warp_sum(ss);
-  if (lanes == 0) all = warp_max(all);
-  if (lane == 0) {
-    sh[warp] = ss;
-    sh_max[warp] = all;
-  }
-  if (lanes) {
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-      for (int o = 1; o < lanes; o <<= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+    __syncthreads();  // one a row: the next row's sums go to the other half
+    ss = lane < warps ? sh[flip][lane] : 0.0f;
+    const float r = norm_recip(warp_sum(ss), a.cols, a.eps);
+    if (lanes == 0) {
       float inv;
-      base[k] = norm_base(top[k], inv);
-      store(k, inv);
-    }
-  }
-  __syncthreads();
-  ss = lane < warps ? sh[lane] : 0.0f;
-  const float r = norm_recip(warp_sum(ss), a.cols, a.eps);
-  if (lanes == 0) {
-    float inv;
-    const float b = norm_base(warp_max(lane < warps ? sh_max[lane] : 0.0f), inv);
+      const float b = norm_base(warp_max(lane < warps ? sh_max[flip][lane] : 0.0f), inv);
 #pragma unroll
-    for (int k = 0; k < K; k++) store(k, inv);
-    if (threadIdx.x == 0) a.scales[row] = __fmul_rn(b, r);
-  } else if (threadIdx.x % lanes == 0) {
-    float *scales = a.scales + row * (a.cols / a.group);
+      for (int k = 0; k < K; k++) store(k, inv);
+      if (threadIdx.x == 0) a.scales[row] = __fmul_rn(b, r);
+    } else if (threadIdx.x % lanes == 0) {
+      float *scales = a.scales + row * (a.cols / a.group);
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-      const int piece = (int)threadIdx.x + k * (int)blockDim.x;
-      if (VEC * piece < a.cols) scales[piece / lanes] = __fmul_rn(base[k], r);
+      for (int k = 0; k < K; k++)
+        if (at_of(k) < a.cols) scales[((int)threadIdx.x + k * (int)blockDim.x) / lanes] = __fmul_rn(base[k], r);
     }
   }
 }
@@ -229,15 +233,22 @@ __global__ void __launch_bounds__(kNormThreads) k_norm8_any(Norm8Args a) {
 
 template <class T, int VEC>
 static cudaError_t norm_pieces(const Norm8Args &a, int sms, int lanes, cudaStream_t st, bool &taken) {
-  // Few rows: as many threads as pieces. Many: CTAs of up to 512, so that
-  // several share an SM and one's loads pass while another waits.
+  // Few rows: as many threads as pieces. Many: CTAs of up to 512, several of
+  // which share an SM.
   const int pieces = a.cols / VEC, most = a.rows >= 2 * sms ? 512 : 1024;
   const auto threads = [&](int k) { return ((pieces + k - 1) / k + 31) / 32 * 32; };
+  // As many CTAs as the SMs hold at the registers that the bounds leave.
+  const auto ctas = [&](int t, int regs) {
+    const int n = 65536 / (regs * t), by_threads = 2048 / t;
+    const int64_t all = (int64_t)sms * (n < by_threads ? n : by_threads);
+    return (unsigned)(a.rows < all ? a.rows : all);
+  };
   taken = true;
-  if (threads(1) <= most) return launch_k(k_norm8<T, VEC, 1>, a.rows, threads(1), 0, st, a, lanes);
-  if (threads(2) <= most) return launch_k(k_norm8<T, VEC, 2>, a.rows, threads(2), 0, st, a, lanes);
-  if (threads(4) <= 512) return launch_k(k_norm8<T, VEC, 4>, a.rows, threads(4), 0, st, a, lanes);
-  if (threads(8) <= 512) return launch_k(k_norm8<T, VEC, 8>, a.rows, threads(8), 0, st, a, lanes);
+  int t;
+  if ((t = threads(1)) <= most) return launch_k(k_norm8<T, VEC, 1>, ctas(t, 64), t, 0, st, a, lanes);
+  if ((t = threads(2)) <= most) return launch_k(k_norm8<T, VEC, 2>, ctas(t, 64), t, 0, st, a, lanes);
+  if ((t = threads(4)) <= 512) return launch_k(k_norm8<T, VEC, 4>, ctas(t, 128), t, 0, st, a, lanes);
+  if ((t = threads(8)) <= 512) return launch_k(k_norm8<T, VEC, 8>, ctas(t, 128), t, 0, st, a, lanes);
   taken = false;
   return cudaSuccess;
 }
