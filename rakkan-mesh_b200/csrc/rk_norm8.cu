@@ -28,9 +28,9 @@ struct Piece {
       if constexpr (sizeof(T) == 4) {
         v[i] = u2f(w[i]);
       } else {
-        const T *h = reinterpret_cast<const T *>(&w[i]);
-        v[2 * i] = act_load(h);
-        v[2 * i + 1] = act_load(h + 1);
+        const float2 h = act_pair<T>(w[i]);
+        v[2 * i] = h.x;
+        v[2 * i + 1] = h.y;
       }
     }
   }
@@ -51,11 +51,7 @@ RK_DEV void norm_store(T *p, const float *v) {
   if constexpr (VEC == 8) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      T *h = reinterpret_cast<T *>(&w[i]);
-      act_store(h, v[2 * i]);
-      act_store(h + 1, v[2 * i + 1]);
-    }
+    for (int i = 0; i < 4; i++) w[i] = act_pack<T>(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
     act_store(p, v[0]);
@@ -72,8 +68,9 @@ RK_DEV float warp_max(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-// 1 / sqrt(mean + eps), both operations rounded once.
-RK_DEV float norm_recip(float ss, int cols, float eps) { return __frcp_rn(__fsqrt_rn(ss / (float)cols + eps)); }
+// 1 / sqrt(mean + eps) within a few units in the last place (the integers do
+// not depend on it).
+RK_DEV float norm_recip(float ss, float inv_cols, float eps) { return rsqrtf(fmaf(ss, inv_cols, eps)); }
 // base of a group's largest magnitude, and the factor of its values.
 RK_DEV float norm_base(float m, float &inv) {
   float base = __fmul_rn(m, u2f(K_1_127));
@@ -104,6 +101,17 @@ __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int 
 #pragma unroll
   for (int k = 0; k < K; k++)
     if (at_of(k) < a.cols) w[k].load(static_cast<const T *>(a.weight) + at_of(k));
+  // Values within ±127 of their base need no clamp; a thread with a NaN or an
+  // infinity among its h (then its squares' sum is one) or weights does.
+  bool odd_weights = false;
+#pragma unroll
+  for (int k = 0; k < K; k++)
+    if (at_of(k) < a.cols) {
+      float f[VEC];
+      w[k].values(f);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) odd_weights |= !(fabsf(f[i]) < INFINITY);
+    }
 
   int flip = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
@@ -134,19 +142,24 @@ __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int 
       all = fmaxf(all, top[k]);
     }
     if (row + gridDim.x < a.rows) load(row + gridDim.x);
+    const bool odd = odd_weights || !(ss < INFINITY);
     auto store = [&](int k, float inv) {
       const int at = at_of(k);
       if (at >= a.cols) return;
-      int v[VEC];
+      uint32_t v[VEC];
+      if (odd) {
 #pragma unroll
-      for (int i = 0; i < VEC; i++) v[i] = quant127(u[k][i], inv);
+        for (int i = 0; i < VEC; i++) v[i] = (uint32_t)quant127(u[k][i], inv);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = quant127_bits(u[k][i], inv);
+      }
       if constexpr (VEC == 1) {
         q[at] = (int8_t)v[0];
       } else {
         uint32_t p[VEC / 4];
 #pragma unroll
-        for (int i = 0; i < VEC / 4; i++)
-          p[i] = (v[4 * i] & 255) | (v[4 * i + 1] & 255) << 8 | (v[4 * i + 2] & 255) << 16 | (uint32_t)v[4 * i + 3] << 24;
+        for (int i = 0; i < VEC / 4; i++) p[i] = pack_bytes(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(q + at) = make_uint2(p[0], p[1]);
         else *reinterpret_cast<uint32_t *>(q + at) = p[0];
       }
@@ -168,7 +181,7 @@ __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int 
     }
     __syncthreads();  // one a row: the next row's sums go to the other half
     ss = lane < warps ? sh[flip][lane] : 0.0f;
-    const float r = norm_recip(warp_sum(ss), a.cols, a.eps);
+    const float r = norm_recip(warp_sum(ss), a.inv_cols, a.eps);
     if (lanes == 0) {
       float inv;
       const float b = norm_base(warp_max(lane < warps ? sh_max[flip][lane] : 0.0f), inv);
@@ -209,7 +222,7 @@ __global__ void __launch_bounds__(kNormThreads) k_norm8_any(Norm8Args a) {
   __syncthreads();
   ss = 0.0f;
   for (int i = 0; i < kNormThreads / 32; i++) ss += sh[i];
-  const float r = norm_recip(ss, a.cols, a.eps);
+  const float r = norm_recip(ss, a.inv_cols, a.eps);
   const int groups = a.cols / a.group;
   for (int g = warp; g < groups; g += kNormThreads / 32) {
     float m = 0.0f;

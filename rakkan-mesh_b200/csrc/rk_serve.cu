@@ -186,7 +186,7 @@ extern "C" int rk_add_rmsnorm_q8(rk_device *d, int type, int rows, int cols, int
   if (!aligned(x, es) || !aligned(residual, es) || !aligned(weight, es) || !aligned(sum_out, es) || !aligned(scales, 4))
     return bad("norm q8: a misaligned buffer");
   OnDevice on(d, stream);
-  Norm8Args a{rows, cols, group, x, residual, weight, sum_out, x_stride, r_stride, s_stride, eps, q, scales};
+  Norm8Args a{rows, cols, group, x, residual, weight, sum_out, x_stride, r_stride, s_stride, eps, 1.0f / (float)cols, q, scales};
   return on.done(on.e == cudaSuccess ? launch_add_rmsnorm_q8(a, type, on.sms, on.st) : on.e, "norm q8");
 }
 

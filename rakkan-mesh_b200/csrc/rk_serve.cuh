@@ -44,7 +44,7 @@ struct Norm8Args {
   const void *x, *residual, *weight;
   void *sum_out;
   int64_t x_stride, r_stride, s_stride;
-  float eps;
+  float eps, inv_cols;  // 1 / cols
   int8_t *q;
   float *scales;
 };
