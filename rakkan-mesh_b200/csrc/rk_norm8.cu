@@ -79,12 +79,12 @@ RK_DEV float norm_base(float m, float &inv) {
   return base;
 }
 
-// lanes: of a group (a power of two up to 32); 0: the group is the row. A CTA
+// log_lanes: of the lanes of a group (0 to 5); -1: the group is the row. A CTA
 // takes every gridDim.x-th row and loads the next one before it waits for a
 // row's sum (41.9 us for 4096x5120 bfloat16 with a CTA a row and no loads in
 // flight meanwhile).
 template <class T, int VEC, int K>
-__global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int lanes) {
+__global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int log_lanes) {
   __shared__ float sh[2][32], sh_max[2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const auto at_of = [&](int k) { return VEC * ((int)threadIdx.x + k * (int)blockDim.x); };
@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int 
     }
 
   int flip = 0;
+  const int groups = a.cols / a.group;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
     int8_t *q = a.q + row * a.cols;
     float u[K][VEC], ss = 0.0f, top[K], base[K], all = 0.0f;
@@ -165,15 +166,19 @@ __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int 
       }
     };
     ss = warp_sum(ss);
-    if (lanes == 0) all = warp_max(all);
+    if (log_lanes < 0) all = warp_max(all);
     if (lane == 0) {
       sh[flip][warp] = ss;
       sh_max[flip][warp] = all;
     }
-    if (lanes) {
+    if (log_lanes >= 0) {
+#pragma unroll
+      for (int o = 0; o < 5; o++)
+        if (o < log_lanes)
+#pragma unroll
+          for (int k = 0; k < K; k++) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1 << o));
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        for (int o = 1; o < lanes; o <<= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
         float inv;
         base[k] = norm_base(top[k], inv);
         store(k, inv);
@@ -182,17 +187,17 @@ __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int 
     __syncthreads();  // one a row: the next row's sums go to the other half
     ss = lane < warps ? sh[flip][lane] : 0.0f;
     const float r = norm_recip(warp_sum(ss), a.inv_cols, a.eps);
-    if (lanes == 0) {
+    if (log_lanes < 0) {
       float inv;
       const float b = norm_base(warp_max(lane < warps ? sh_max[flip][lane] : 0.0f), inv);
 #pragma unroll
       for (int k = 0; k < K; k++) store(k, inv);
       if (threadIdx.x == 0) a.scales[row] = __fmul_rn(b, r);
-    } else if (threadIdx.x % lanes == 0) {
-      float *scales = a.scales + row * (a.cols / a.group);
+    } else if ((threadIdx.x & ((1 << log_lanes) - 1)) == 0) {
+      float *scales = a.scales + row * groups;
 #pragma unroll
       for (int k = 0; k < K; k++)
-        if (at_of(k) < a.cols) scales[((int)threadIdx.x + k * (int)blockDim.x) / lanes] = __fmul_rn(base[k], r);
+        if (at_of(k) < a.cols) scales[((int)threadIdx.x + k * (int)blockDim.x) >> log_lanes] = __fmul_rn(base[k], r);
     }
   }
 }
@@ -274,14 +279,16 @@ static cudaError_t norm_typed(const Norm8Args &a, int sms, cudaStream_t st) {
   };
   const bool vec = a.cols % VEC == 0 && on16(a.x, a.x_stride) && on16(a.weight, 0) && (!a.residual || on16(a.residual, a.r_stride)) &&
                    (!a.sum_out || on16(a.sum_out, a.s_stride)) && (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
-  const auto lanes_of = [&](int v) {  // -1: no power of two of lanes
-    const int n = a.group % v ? 0 : a.group / v;
-    return a.group == a.cols ? 0 : n >= 1 && n <= 32 && (n & (n - 1)) == 0 ? n : -1;
+  const auto lanes_of = [&](int v) {  // log2; -1: the row; -2: no power of two of lanes
+    if (a.group == a.cols) return -1;
+    for (int k = 0; k <= 5; k++)
+      if (a.group == v << k) return k;
+    return -2;
   };
   bool taken = false;
   cudaError_t e = cudaSuccess;
-  if (vec && lanes_of(VEC) >= 0) e = norm_pieces<T, VEC>(a, sms, lanes_of(VEC), st, taken);
-  else if (lanes_of(1) >= 0) e = norm_pieces<T, 1>(a, sms, lanes_of(1), st, taken);
+  if (vec && lanes_of(VEC) >= -1) e = norm_pieces<T, VEC>(a, sms, lanes_of(VEC), st, taken);
+  else if (lanes_of(1) >= -1) e = norm_pieces<T, 1>(a, sms, lanes_of(1), st, taken);
   return taken ? e : launch_k(k_norm8_any<T>, a.rows, kNormThreads, 0, st, a);
 }
 
