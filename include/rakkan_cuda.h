@@ -533,11 +533,12 @@ typedef struct {
 } rk_kv8;
 /* Stores rows t < tokens of k and v ([kv_heads][head_size] each, rows
  * k_stride and v_stride elements apart, of type RK_ACT_*) at slots[t]
- * (below zero: the row is skipped). The rows of one page are consecutive in
- * the call, in ascending slots, and a page is in one such run only; what a
- * page below its run's first slot holds are earlier tokens, and what lies
- * behind the run is left as it is. For each page and head, with m the
- * largest finite magnitude of the run:
+ * (below zero: the row is skipped). The rows of one page follow one another
+ * in the call, with no skipped row between them, in ascending slots (of two rows
+ * with the same slot the later one stays), and a page is in one such run only (else its contents are
+ * unspecified). What a page below its run's first slot holds are earlier
+ * tokens, and what lies behind the run is left as it is. For each page and
+ * head, with m the largest finite magnitude of the run:
  *   scale = max(the page's scale if it holds earlier tokens, m * fl(1/127)),
  *           zero when below 2^-120;
  *   new values: clamp(RoundToEven(x * fl(1/scale)), +-127), NaN as 0;

@@ -144,9 +144,14 @@ cudaError_t launch_page_tables(const TablesArgs &a, int sms, cudaStream_t st) {
 // Append
 // ---------------------------------------------------------------------------
 // A run is the consecutive rows of one page. One CTA takes a run's part for
-// one kv head, of the keys or of the values: it finds the largest magnitude
-// (first reading), then scales, rounds and stores (second reading, from L2
-// or L1). A CTA looks for the runs that begin in its `chunk` of rows.
+// one kv head, of the keys or of the values: it finds the largest magnitude,
+// then scales, rounds and stores. The rows are read twice, the second time
+// from L1 (a page's part is 16 KB of bfloat16 at most at 64 tokens and head
+// size 128); the bytes of the rows and of the cache bound the call. Keys go
+// from 4 neighbours to a word; values, transposed, from 4 dimensions of 4
+// tokens to 4 words, with the tokens in the fast lanes, so that a page row's
+// words are stored side by side and no shared memory is needed. A CTA looks for
+// the runs that begin in its `chunk` of rows (at most 32).
 constexpr int kAppThreads = 128;
 
 RK_DEV float cta_max(float m, float *sh) {
@@ -161,64 +166,139 @@ RK_DEV float cta_max(float m, float *sh) {
   return m;
 }
 
+// Four neighbours of a row; vec: on their boundary of 8 or 16 bytes.
+RK_DEV float4 load4(const float *p, bool vec) {
+  if (vec) return *reinterpret_cast<const float4 *>(p);
+  return make_float4(p[0], p[1], p[2], p[3]);
+}
 template <class T>
-__global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int chunk) {
+RK_DEV float4 load4(const T *p, bool vec) {
+  if (!vec) return make_float4(act_load(p), act_load(p + 1), act_load(p + 2), act_load(p + 3));
+  const uint2 w = *reinterpret_cast<const uint2 *>(p);
+  const float2 a = act_pair<T>(w.x), b = act_pair<T>(w.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+// Their bytes; odd: infinities or NaN are among the run's values.
+RK_DEV uint32_t quant4(float4 x, float inv, bool odd) {
+  if (odd)
+    return pack_bytes((uint32_t)quant127(x.x, inv), (uint32_t)quant127(x.y, inv), (uint32_t)quant127(x.z, inv),
+                      (uint32_t)quant127(x.w, inv));
+  return pack_bytes(quant127_bits(x.x, inv), quant127_bits(x.y, inv), quant127_bits(x.z, inv), quant127_bits(x.w, inv));
+}
+RK_DEV uint32_t requant4(uint32_t w, float ratio) {
+  return pack_bytes(quant127_bits((float)(int8_t)w, ratio), quant127_bits((float)(int8_t)(w >> 8), ratio),
+                    quant127_bits((float)(int8_t)(w >> 16), ratio), quant127_bits((float)(int8_t)(w >> 24), ratio));
+}
+// Bytes [from, to) of a word.
+RK_DEV void store_bytes(int8_t *p, uint32_t w, int from, int to) {
+  if (from <= 0 && to >= 4) {
+    *reinterpret_cast<uint32_t *>(p) = w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (i >= from && i < to) p[i] = (int8_t)(w >> (8 * i));
+}
+
+template <class T>
+__global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int chunk, int log_block) {
   __shared__ float sh[kAppThreads / 32];
   const int head = blockIdx.y, lane = threadIdx.x & 31;
   const bool values = blockIdx.z != 0;
-  const int B = a.c.block, hs = a.c.head_size, H = a.c.kv_heads;
-  const int cap = a.c.blocks * B;
+  const int B = 1 << log_block, hs = a.c.head_size, hs4 = hs >> 2, H = a.c.kv_heads;
+  const int cap = a.c.blocks << log_block;
   const T *x = static_cast<const T *>(values ? a.v : a.k) + (int64_t)head * hs;
   const int64_t stride = values ? a.v_stride : a.k_stride;
+  const bool vec = stride % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
   int8_t *cache = values ? a.c.v : a.c.k;
   float *scales = values ? a.c.v_scale : a.c.k_scale;
-  const int t0 = blockIdx.x * chunk, t1 = min(a.tokens, t0 + chunk);
+  const int t0 = blockIdx.x * chunk;
 
-  for (int t = t0; t < t1; t++) {
-    const int slot = a.slots[t];
-    if (slot < 0) continue;
-    if (slot >= cap) {
-      if (threadIdx.x == 0 && head == 0 && !values) atomicExch(a.err, DEV_ERR_RANGE);
-      continue;
-    }
-    const int page = slot / B, first = slot % B;
-    if (t > 0) {
-      const int p = a.slots[t - 1];
-      if (p >= 0 && p < cap && p / B == page) continue;  // within a run that begins earlier
-    }
-    int rows = 1;  // of the run
+  // The rows at which runs begin, of this chunk.
+  const int mine = t0 + lane < a.tokens && lane < chunk ? a.slots[t0 + lane] : -1;
+  const int ahead = t0 + lane > 0 && mine >= 0 ? a.slots[t0 + lane - 1] : -1;
+  const bool fits = mine >= 0 && mine < cap;
+  if (mine >= cap && head == 0 && !values && threadIdx.x < 32) atomicExch(a.err, DEV_ERR_RANGE);
+  unsigned begins =
+      __ballot_sync(0xffffffffu, fits && !(ahead >= 0 && ahead < cap && ahead >> log_block == mine >> log_block));
+  for (; begins; begins &= begins - 1) {
+    const int t = t0 + __ffs(begins) - 1;
+    const int slot = __shfl_sync(0xffffffffu, mine, __ffs(begins) - 1);
+    const int page = slot >> log_block, first = slot & (B - 1);
+    int rows = 0;          // of the run
+    bool regular = true;   // its slots follow one another
     for (;;) {
-      const int u = t + rows + lane;
-      const int s = u < a.tokens ? a.slots[u] : -1;
-      const unsigned in = __ballot_sync(0xffffffffu, s >= 0 && s < cap && s / B == page);
-      if (in != 0xffffffffu) {
-        rows += __ffs(~in) - 1;
-        break;
-      }
-      rows += 32;
+      const int u = t + rows + lane, s = u < a.tokens ? a.slots[u] : -1;
+      const bool in = s >= 0 && s < cap && s >> log_block == page;
+      const unsigned in_run = __ballot_sync(0xffffffffu, in);
+      const int n = in_run == 0xffffffffu ? 32 : __ffs(~in_run) - 1;
+      regular &= __all_sync(0xffffffffu, lane >= n || s == slot + rows + lane);
+      rows += n;
+      if (n < 32) break;
     }
+
     float m = 0.0f;
-    for (int e = threadIdx.x; e < rows * hs; e += kAppThreads)
-      m = fmaxf(m, finite_abs(act_load(x + (int64_t)(t + e / hs) * stride + e % hs)));
+    bool odd = false;
+    for (int e = threadIdx.x; e < rows * hs4; e += kAppThreads) {
+      const float4 v = load4(x + (int64_t)(t + e / hs4) * stride + 4 * (e % hs4), vec);
+      const float top = fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)));
+      odd |= !(fabsf(v.x) < INFINITY) | !(fabsf(v.y) < INFINITY) | !(fabsf(v.z) < INFINITY) | !(fabsf(v.w) < INFINITY);
+      m = fmaxf(m, top);
+    }
     m = cta_max(m, sh);
+    odd = __syncthreads_or(odd);
     const int64_t ph = (int64_t)page * H + head;
     const float had = first > 0 ? scales[ph] : 0.0f;
     float scale = fmaxf(had, __fmul_rn(m, u2f(K_1_127)));
     if (scale < u2f(K_TINY)) scale = 0.0f;
     const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
     int8_t *pg = cache + ph * B * hs;
-    const int64_t step_o = values ? 1 : hs, step_d = values ? B : 1;  // of a token, of a dimension
-    if (had != scale) {
+
+    if (had != scale) {  // earlier rows, to the larger scale
       const float ratio = scale > 0.0f ? __fdiv_rn(had, scale) : 0.0f;
-      for (int e = threadIdx.x; e < first * hs; e += kAppThreads) {
-        int8_t *q = pg + (values ? (e % first) * step_o + (e / first) * step_d : e);
-        *q = (int8_t)quant127((float)*q, ratio);
+      if (!values) {
+        for (int e = threadIdx.x; e < first * hs4; e += kAppThreads) {
+          uint32_t *w = reinterpret_cast<uint32_t *>(pg) + e;
+          *w = requant4(*w, ratio);
+        }
+      } else {
+        const int words = (first + 3) >> 2;
+        for (int e = threadIdx.x; e < words * hs; e += kAppThreads) {
+          const int d = e / words, o = 4 * (e % words);
+          int8_t *p = pg + d * B + o;
+          store_bytes(p, requant4(*reinterpret_cast<const uint32_t *>(p), ratio), 0, first - o);
+        }
       }
     }
-    for (int e = threadIdx.x; e < rows * hs; e += kAppThreads) {
-      const int r = values ? e % rows : e / hs, d = values ? e / rows : e % hs;
-      const int o = a.slots[t + r] % B;
-      pg[o * step_o + d * step_d] = (int8_t)quant127(act_load(x + (int64_t)(t + r) * stride + d), inv);
+    if (!regular) {  // a row after the other: of rows of one slot, the last stays
+      for (int r = 0; r < rows; r++) {
+        const int o = a.slots[t + r] & (B - 1);
+        __syncthreads();
+        for (int d = threadIdx.x; d < hs; d += kAppThreads)
+          pg[values ? d * B + o : o * hs + d] = (int8_t)quant127(act_load(x + (int64_t)(t + r) * stride + d), inv);
+      }
+    } else if (!values) {
+      for (int e = threadIdx.x; e < rows * hs4; e += kAppThreads)
+        reinterpret_cast<uint32_t *>(pg + first * hs)[e] =
+            quant4(load4(x + (int64_t)(t + e / hs4) * stride + 4 * (e % hs4), vec), inv, odd);
+    } else {
+      // Words of four tokens, from the one that holds the run's first.
+      const int o0 = first & ~3, words = (first + rows + 3 - o0) >> 2;
+      __syncthreads();  // its bytes before the run have been written
+      for (int e = threadIdx.x; e < words * hs4; e += kAppThreads) {
+        const int o = o0 + 4 * (e % words), d = 4 * (e / words), r = o - first;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          w[j] = r + j >= 0 && r + j < rows ? quant4(load4(x + (int64_t)(t + r + j) * stride + d, vec), inv, odd) : 0;
+        // Byte i of the four rows: dimension d + i.
+        const uint32_t lo01 = __byte_perm(w[0], w[1], 0x5140), hi01 = __byte_perm(w[0], w[1], 0x7362);
+        const uint32_t lo23 = __byte_perm(w[2], w[3], 0x5140), hi23 = __byte_perm(w[2], w[3], 0x7362);
+        const uint32_t t4[4] = {__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632), __byte_perm(hi01, hi23, 0x5410),
+                                __byte_perm(hi01, hi23, 0x7632)};
+#pragma unroll
+        for (int i = 0; i < 4; i++) store_bytes(pg + (d + i) * B + o, t4[i], -r, rows - r);
+      }
     }
     __syncthreads();  // every thread has read the old scale
     if (threadIdx.x == 0) scales[ph] = scale;
@@ -228,12 +308,13 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
 cudaError_t launch_kv8_append(const AppendArgs &a, int type, int sms, cudaStream_t st) {
   const long long ctas = 2LL * a.tokens * a.c.kv_heads;
   int chunk = 1;  // rows a CTA looks through: more once every SM has several CTAs
-  while (chunk < a.c.block && ctas / chunk > 32LL * sms) chunk *= 2;
+  while (chunk < 32 && chunk < a.c.block && ctas / chunk > 32LL * sms) chunk *= 2;
   const dim3 grid((a.tokens + chunk - 1) / chunk, a.c.kv_heads, 2);
+  const int lb = a.c.block == 16 ? 4 : a.c.block == 32 ? 5 : a.c.block == 64 ? 6 : 7;
   switch (type) {
-    case RK_ACT_F32: return launch_k(k_kv8_append<float>, grid, kAppThreads, 0, st, a, chunk);
-    case RK_ACT_F16: return launch_k(k_kv8_append<__half>, grid, kAppThreads, 0, st, a, chunk);
-    default: return launch_k(k_kv8_append<__nv_bfloat16>, grid, kAppThreads, 0, st, a, chunk);
+    case RK_ACT_F32: return launch_k(k_kv8_append<float>, grid, kAppThreads, 0, st, a, chunk, lb);
+    case RK_ACT_F16: return launch_k(k_kv8_append<__half>, grid, kAppThreads, 0, st, a, chunk, lb);
+    default: return launch_k(k_kv8_append<__nv_bfloat16>, grid, kAppThreads, 0, st, a, chunk, lb);
   }
 }
 

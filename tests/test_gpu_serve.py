@@ -238,6 +238,34 @@ def test_append_many_rows_and_strides(torch, dev):
     np.testing.assert_array_equal(kv.v_scale.cpu().numpy(), vs)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_append_slots_with_gaps_and_repeats(torch, dev, t):
+    """Runs that skip offsets, and a slot given twice: the later row stays."""
+    rng = np.random.default_rng(17)
+    kv, host = cache(torch, dev, rng, 4, 2, 32, 48)
+    slots = [1, 4, 5, 31, 32 + 7, 32 + 7, 32 + 8, 64, 64, 96 + 3, 96 + 30]
+    x = [rng.normal(0, 2, (len(slots), 2, 48)).astype(np.float32) for _ in range(2)]
+    check_append(torch, dev, rng, kv, host, x, slots, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("first", [0, 1, 2, 3, 13])
+def test_append_unaligned_rows(torch, dev, first, t):
+    """Keys and values that begin off a 16-byte boundary, runs at every offset of a word of four tokens."""
+    rng = np.random.default_rng(18 + first)
+    kv, host = cache(torch, dev, rng, 3, 2, 16, 32)
+    slots = [(16 * (j // 16) + j % 16) for j in range(first, first + 22)]
+    wide = torch.from_numpy(rng.normal(0, 1, (22, 2 * 64 + 3)).astype(np.float32)).cuda().to(dtype(torch, t))
+    kn, vn = wide[:, 1:65].unflatten(1, (2, 32)), wide[:, 66:130].unflatten(1, (2, 32))
+    kv.append(kn, vn, ints(torch, slots))
+    k, v, ks, vs = host
+    vt = np.ascontiguousarray(v.transpose(0, 1, 3, 2))
+    append_plain(k, ks, kn.float().cpu().numpy(), slots, 16)
+    append_plain(vt, vs, vn.float().cpu().numpy(), slots, 16)
+    np.testing.assert_array_equal(kv.k.cpu().numpy(), k)
+    np.testing.assert_array_equal(kv.v.cpu().numpy(), vt.transpose(0, 1, 3, 2))
+
+
 def test_append_leaves_out_slots_behind_the_cache(torch, dev):
     rng = np.random.default_rng(8)
     kv, host = cache(torch, dev, rng, 2, 2, 16, 16)
