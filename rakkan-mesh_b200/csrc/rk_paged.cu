@@ -166,24 +166,55 @@ RK_DEV float cta_max(float m, float *sh) {
   return m;
 }
 
-// Four neighbours of a row; vec: on their boundary of 8 or 16 bytes.
-RK_DEV float4 load4(const float *p, bool vec) {
-  if (vec) return *reinterpret_cast<const float4 *>(p);
-  return make_float4(p[0], p[1], p[2], p[3]);
+// e / d and e % d for a divisor that many e share.
+struct Divisor {
+  uint32_t d, m;
+  RK_HD explicit Divisor(uint32_t n) : d(n), m(0xffffffffu / n + 1) {}  // d > 1, e·d < 2^32
+  RK_DEV uint32_t quotient(uint32_t e) const { return __umulhi(e, m); }
+  RK_DEV uint32_t rest(uint32_t e, uint32_t q) const { return e - q * d; }
+};
+
+// N neighbours of a row; vec: on a 16-byte boundary (N = 4 of 16 bits: of 8).
+template <int N>
+RK_DEV void load_n(const float *p, bool vec, float *v) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4 *>(p + i));
+      v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = __ldg(p + i);
+  }
 }
-template <class T>
-RK_DEV float4 load4(const T *p, bool vec) {
-  if (!vec) return make_float4(act_load(p), act_load(p + 1), act_load(p + 2), act_load(p + 3));
-  const uint2 w = *reinterpret_cast<const uint2 *>(p);
-  const float2 a = act_pair<T>(w.x), b = act_pair<T>(w.y);
-  return make_float4(a.x, a.y, b.x, b.y);
+template <int N, class T>
+RK_DEV void load_n(const T *p, bool vec, float *v) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = act_load(p + i);
+    return;
+  }
+  uint32_t w[N / 2];
+  if constexpr (N == 8) {
+    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+  } else {
+    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+    w[0] = x.x, w[1] = x.y;
+  }
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) {
+    const float2 f = act_pair<T>(w[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
 }
 // Their bytes; odd: infinities or NaN are among the run's values.
-RK_DEV uint32_t quant4(float4 x, float inv, bool odd) {
+RK_DEV uint32_t quant4(const float *x, float inv, bool odd) {
   if (odd)
-    return pack_bytes((uint32_t)quant127(x.x, inv), (uint32_t)quant127(x.y, inv), (uint32_t)quant127(x.z, inv),
-                      (uint32_t)quant127(x.w, inv));
-  return pack_bytes(quant127_bits(x.x, inv), quant127_bits(x.y, inv), quant127_bits(x.z, inv), quant127_bits(x.w, inv));
+    return pack_bytes((uint32_t)quant127(x[0], inv), (uint32_t)quant127(x[1], inv), (uint32_t)quant127(x[2], inv),
+                      (uint32_t)quant127(x[3], inv));
+  return pack_bytes(quant127_bits(x[0], inv), quant127_bits(x[1], inv), quant127_bits(x[2], inv), quant127_bits(x[3], inv));
 }
 RK_DEV uint32_t requant4(uint32_t w, float ratio) {
   return pack_bytes(quant127_bits((float)(int8_t)w, ratio), quant127_bits((float)(int8_t)(w >> 8), ratio),
@@ -205,11 +236,12 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
   __shared__ float sh[kAppThreads / 32];
   const int head = blockIdx.y, lane = threadIdx.x & 31;
   const bool values = blockIdx.z != 0;
-  const int B = 1 << log_block, hs = a.c.head_size, hs4 = hs >> 2, H = a.c.kv_heads;
+  const int B = 1 << log_block, hs = a.c.head_size, H = a.c.kv_heads;
   const int cap = a.c.blocks << log_block;
   const T *x = static_cast<const T *>(values ? a.v : a.k) + (int64_t)head * hs;
   const int64_t stride = values ? a.v_stride : a.k_stride;
-  const bool vec = stride % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
+  const Divisor by8(hs >> 3);  // hs / 8 is at least 2
+  const bool vec = stride * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   int8_t *cache = values ? a.c.v : a.c.k;
   float *scales = values ? a.c.v_scale : a.c.k_scale;
   const int t0 = blockIdx.x * chunk;
@@ -239,11 +271,16 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
 
     float m = 0.0f;
     bool odd = false;
-    for (int e = threadIdx.x; e < rows * hs4; e += kAppThreads) {
-      const float4 v = load4(x + (int64_t)(t + e / hs4) * stride + 4 * (e % hs4), vec);
-      const float top = fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)));
-      odd |= !(fabsf(v.x) < INFINITY) | !(fabsf(v.y) < INFINITY) | !(fabsf(v.z) < INFINITY) | !(fabsf(v.w) < INFINITY);
-      m = fmaxf(m, top);
+#pragma unroll 4
+    for (int e = threadIdx.x; e < rows * (hs >> 3); e += kAppThreads) {
+      const int r = by8.quotient(e);
+      float v[8];
+      load_n<8>(x + (int64_t)(t + r) * stride + 8 * by8.rest(e, r), vec, v);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        m = fmaxf(m, finite_abs(v[i]));
+        odd |= !(fabsf(v[i]) < INFINITY);
+      }
     }
     m = cta_max(m, sh);
     odd = __syncthreads_or(odd);
@@ -257,7 +294,7 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
     if (had != scale) {  // earlier rows, to the larger scale
       const float ratio = scale > 0.0f ? __fdiv_rn(had, scale) : 0.0f;
       if (!values) {
-        for (int e = threadIdx.x; e < first * hs4; e += kAppThreads) {
+        for (int e = threadIdx.x; e < first * hs / 4; e += kAppThreads) {
           uint32_t *w = reinterpret_cast<uint32_t *>(pg) + e;
           *w = requant4(*w, ratio);
         }
@@ -278,19 +315,31 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
           pg[values ? d * B + o : o * hs + d] = (int8_t)quant127(act_load(x + (int64_t)(t + r) * stride + d), inv);
       }
     } else if (!values) {
-      for (int e = threadIdx.x; e < rows * hs4; e += kAppThreads)
-        reinterpret_cast<uint32_t *>(pg + first * hs)[e] =
-            quant4(load4(x + (int64_t)(t + e / hs4) * stride + 4 * (e % hs4), vec), inv, odd);
+#pragma unroll 4
+      for (int e = threadIdx.x; e < rows * (hs >> 3); e += kAppThreads) {
+        const int r = by8.quotient(e);
+        float v[8];
+        load_n<8>(x + (int64_t)(t + r) * stride + 8 * by8.rest(e, r), vec, v);
+        reinterpret_cast<uint2 *>(pg + first * hs)[e] = make_uint2(quant4(v, inv, odd), quant4(v + 4, inv, odd));
+      }
     } else {
       // Words of four tokens, from the one that holds the run's first.
       const int o0 = first & ~3, words = (first + rows + 3 - o0) >> 2;
       __syncthreads();  // its bytes before the run have been written
-      for (int e = threadIdx.x; e < words * hs4; e += kAppThreads) {
-        const int o = o0 + 4 * (e % words), d = 4 * (e / words), r = o - first;
+      const Divisor by_words(max(words, 2));
+      for (int e = threadIdx.x; e < words * (hs >> 2); e += kAppThreads) {
+        const int n = words > 1 ? by_words.quotient(e) : e;
+        const int o = words > 1 ? o0 + 4 * by_words.rest(e, n) : o0, d = 4 * n, r = o - first;
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          w[j] = r + j >= 0 && r + j < rows ? quant4(load4(x + (int64_t)(t + r + j) * stride + d, vec), inv, odd) : 0;
+        for (int j = 0; j < 4; j++) {
+          w[j] = 0;
+          if (r + j >= 0 && r + j < rows) {
+            float v[4];
+            load_n<4>(x + (int64_t)(t + r + j) * stride + d, vec, v);
+            w[j] = quant4(v, inv, odd);
+          }
+        }
         // Byte i of the four rows: dimension d + i.
         const uint32_t lo01 = __byte_perm(w[0], w[1], 0x5140), hi01 = __byte_perm(w[0], w[1], 0x7362);
         const uint32_t lo23 = __byte_perm(w[2], w[3], 0x5140), hi23 = __byte_perm(w[2], w[3], 0x7362);
