@@ -1,5 +1,7 @@
 // rk_paged.cu — page tables from request lengths, and the append of new keys
 // and values into the 8-bit paged cache.
+#include <cstring>
+
 #include "rk_act.cuh"
 #include "rk_matvec.cuh"
 #include "rk_serve.cuh"
@@ -145,14 +147,17 @@ cudaError_t launch_page_tables(const TablesArgs &a, int sms, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // A run is the consecutive rows of one page. One CTA takes a run's part for
 // one kv head, of the keys or of the values: it finds the largest magnitude,
-// then scales, rounds and stores. The rows are read twice, the second time
-// from L1 (a page's part is 16 KB of bfloat16 at most at 64 tokens and head
-// size 128); the bytes of the rows and of the cache bound the call. Keys go
-// from 4 neighbours to a word; values, transposed, from 4 dimensions of 4
-// tokens to 4 words, with the tokens in the fast lanes, so that a page row's
-// words are stored side by side and no shared memory is needed. A CTA looks for
-// the runs that begin in its `chunk` of rows (at most 32).
-constexpr int kAppThreads = 128;
+// then scales, rounds and stores. The bytes of the rows and of the cache bound
+// the call. A run of up to 8192 values (a page of 64 tokens at head size 128) is
+// loaded once, into registers; longer ones and rows off 16-byte boundaries are
+// read twice, the second time from L1 or L2 (every run so: 32.5 us for the
+// prompts of 16 sequences, 8 heads of 128). Values are stored transposed: the
+// rounded bytes go through shared memory, from which 4 dimensions of 4 tokens
+// become 4 words, with the tokens in the fast lanes, so that a page row's words
+// are stored side by side. A CTA looks for the runs that begin in its `chunk`
+// of rows (at most 32).
+constexpr int kAppThreads = 128, kAppPieces = 8;  // a thread's pieces of eight values
+constexpr int kAppHeld = kAppThreads * kAppPieces * 8;
 
 RK_DEV float cta_max(float m, float *sh) {
 #pragma unroll
@@ -209,6 +214,12 @@ RK_DEV void load_n(const T *p, bool vec, float *v) {
     v[2 * i] = f.x, v[2 * i + 1] = f.y;
   }
 }
+// The larger of top and |w|, as bits: of two values of 16 bits, each half by itself.
+template <class T>
+RK_DEV uint32_t max_bits(uint32_t top, uint32_t w) {
+  if constexpr (sizeof(T) == 4) return max(top, w & 0x7fffffffu);
+  else return __vmaxu2(top, w & 0x7fff7fffu);
+}
 // Their bytes; odd: infinities or NaN are among the run's values.
 RK_DEV uint32_t quant4(const float *x, float inv, bool odd) {
   if (odd)
@@ -234,6 +245,7 @@ RK_DEV void store_bytes(int8_t *p, uint32_t w, int from, int to) {
 template <class T>
 __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int chunk, int log_block) {
   __shared__ float sh[kAppThreads / 32];
+  __shared__ __align__(16) uint32_t s_rows[(kAppHeld + 128 * 4) / 4];  // rounded values, rows hs + 4 bytes apart
   const int head = blockIdx.y, lane = threadIdx.x & 31;
   const bool values = blockIdx.z != 0;
   const int B = 1 << log_block, hs = a.c.head_size, H = a.c.kv_heads;
@@ -269,21 +281,57 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
       if (n < 32) break;
     }
 
+    // Held runs: magnitudes compare as their bits do, two of 16 bits at once,
+    // and an infinity or a NaN comes out on top; such a run is read again.
+    bool held = vec && regular && rows * hs <= kAppHeld, odd = false;
+    const int pieces = rows * (hs >> 3);
+    uint4 kept[kAppPieces][sizeof(T) / 2];
     float m = 0.0f;
-    bool odd = false;
-#pragma unroll 4
-    for (int e = threadIdx.x; e < rows * (hs >> 3); e += kAppThreads) {
-      const int r = by8.quotient(e);
-      float v[8];
-      load_n<8>(x + (int64_t)(t + r) * stride + 8 * by8.rest(e, r), vec, v);
+    if (held) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        m = fmaxf(m, finite_abs(v[i]));
-        odd |= !(fabsf(v[i]) < INFINITY);
+      for (int i = 0; i < kAppPieces; i++) {
+        const int e = threadIdx.x + i * kAppThreads;
+#pragma unroll
+        for (int j = 0; j < sizeof(T) / 2; j++) kept[i][j] = make_uint4(0, 0, 0, 0);
+        if (e < pieces) {
+          const int r = by8.quotient(e);
+          const uint4 *p = reinterpret_cast<const uint4 *>(x + (int64_t)(t + r) * stride + 8 * by8.rest(e, r));
+#pragma unroll
+          for (int j = 0; j < sizeof(T) / 2; j++) kept[i][j] = __ldg(p + j);
+        }
       }
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kAppPieces; i++)
+#pragma unroll
+        for (int j = 0; j < sizeof(T) / 2; j++) {
+          const uint4 w = kept[i][j];
+          top = max_bits<T>(max_bits<T>(max_bits<T>(max_bits<T>(top, w.x), w.y), w.z), w.w);
+        }
+      if (sizeof(T) == 2) top = max(top & 0xffff, top >> 16);
+      T value;
+      memcpy(&value, &top, sizeof(T));
+      m = act_load(&value);
+      odd = !(m < INFINITY);
+      if (odd) m = 0.0f;
+      held = !__syncthreads_or(odd);
+    }
+    if (!held) {
+      m = 0.0f;
+#pragma unroll 4
+      for (int e = threadIdx.x; e < pieces; e += kAppThreads) {
+        const int r = by8.quotient(e);
+        float v[8];
+        load_n<8>(x + (int64_t)(t + r) * stride + 8 * by8.rest(e, r), vec, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          m = fmaxf(m, finite_abs(v[i]));
+          odd |= !(fabsf(v[i]) < INFINITY);
+        }
+      }
+      odd = __syncthreads_or(odd);
     }
     m = cta_max(m, sh);
-    odd = __syncthreads_or(odd);
     const int64_t ph = (int64_t)page * H + head;
     const float had = first > 0 ? scales[ph] : 0.0f;
     float scale = fmaxf(had, __fmul_rn(m, u2f(K_1_127)));
@@ -307,6 +355,32 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
         }
       }
     }
+    // Values to the page: f(row, dimension) are four dimensions' bytes of a row.
+    // A word of the page is four tokens, the first and last perhaps in part.
+    auto to_page = [&](auto f) {
+      const int o0 = first & ~3, words = (first + rows + 3 - o0) >> 2;
+      const Divisor by_words(max(words, 2));
+      for (int e = threadIdx.x; e < words * (hs >> 2); e += kAppThreads) {
+        const int n = words > 1 ? by_words.quotient(e) : e;
+        const int o = words > 1 ? o0 + 4 * by_words.rest(e, n) : o0, d = 4 * n, r = o - first;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = r + j >= 0 && r + j < rows ? f(r + j, d) : 0;
+        // Byte i of the four rows: dimension d + i.
+        const uint32_t lo01 = __byte_perm(w[0], w[1], 0x5140), hi01 = __byte_perm(w[0], w[1], 0x7362);
+        const uint32_t lo23 = __byte_perm(w[2], w[3], 0x5140), hi23 = __byte_perm(w[2], w[3], 0x7362);
+        const uint32_t t4[4] = {__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632), __byte_perm(hi01, hi23, 0x5410),
+                                __byte_perm(hi01, hi23, 0x7632)};
+        int8_t *to = pg + (d << log_block) + o;
+        if (r >= 0 && r + 4 <= rows) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) *reinterpret_cast<uint32_t *>(to + (i << log_block)) = t4[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) store_bytes(to + (i << log_block), t4[i], -r, rows - r);
+        }
+      }
+    };
     if (!regular) {  // a row after the other: of rows of one slot, the last stays
       for (int r = 0; r < rows; r++) {
         const int o = a.slots[t + r] & (B - 1);
@@ -314,40 +388,51 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
         for (int d = threadIdx.x; d < hs; d += kAppThreads)
           pg[values ? d * B + o : o * hs + d] = (int8_t)quant127(act_load(x + (int64_t)(t + r) * stride + d), inv);
       }
+    } else if (held) {
+#pragma unroll
+      for (int i = 0; i < kAppPieces; i++) {
+        const int e = threadIdx.x + i * kAppThreads;
+        if (e < pieces) {
+          float v[8];
+          const uint32_t *w = reinterpret_cast<const uint32_t *>(kept[i]);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            if constexpr (sizeof(T) == 4) {
+              v[2 * j] = u2f(w[2 * j]), v[2 * j + 1] = u2f(w[2 * j + 1]);
+            } else {
+              const float2 f = act_pair<T>(w[j]);
+              v[2 * j] = f.x, v[2 * j + 1] = f.y;
+            }
+          }
+          const uint32_t w0 = quant4(v, inv, false), w1 = quant4(v + 4, inv, false);
+          if (!values) {
+            reinterpret_cast<uint2 *>(pg + first * hs)[e] = make_uint2(w0, w1);
+          } else {
+            const int r = by8.quotient(e), at = r * ((hs >> 2) + 1) + 2 * by8.rest(e, r);
+            s_rows[at] = w0;
+            s_rows[at + 1] = w1;
+          }
+        }
+      }
+      if (values) {
+        __syncthreads();
+        to_page([&](int r, int d) { return s_rows[r * ((hs >> 2) + 1) + (d >> 2)]; });
+      }
     } else if (!values) {
 #pragma unroll 4
-      for (int e = threadIdx.x; e < rows * (hs >> 3); e += kAppThreads) {
+      for (int e = threadIdx.x; e < pieces; e += kAppThreads) {
         const int r = by8.quotient(e);
         float v[8];
         load_n<8>(x + (int64_t)(t + r) * stride + 8 * by8.rest(e, r), vec, v);
         reinterpret_cast<uint2 *>(pg + first * hs)[e] = make_uint2(quant4(v, inv, odd), quant4(v + 4, inv, odd));
       }
     } else {
-      // Words of four tokens, from the one that holds the run's first.
-      const int o0 = first & ~3, words = (first + rows + 3 - o0) >> 2;
       __syncthreads();  // its bytes before the run have been written
-      const Divisor by_words(max(words, 2));
-      for (int e = threadIdx.x; e < words * (hs >> 2); e += kAppThreads) {
-        const int n = words > 1 ? by_words.quotient(e) : e;
-        const int o = words > 1 ? o0 + 4 * by_words.rest(e, n) : o0, d = 4 * n, r = o - first;
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          w[j] = 0;
-          if (r + j >= 0 && r + j < rows) {
-            float v[4];
-            load_n<4>(x + (int64_t)(t + r + j) * stride + d, vec, v);
-            w[j] = quant4(v, inv, odd);
-          }
-        }
-        // Byte i of the four rows: dimension d + i.
-        const uint32_t lo01 = __byte_perm(w[0], w[1], 0x5140), hi01 = __byte_perm(w[0], w[1], 0x7362);
-        const uint32_t lo23 = __byte_perm(w[2], w[3], 0x5140), hi23 = __byte_perm(w[2], w[3], 0x7362);
-        const uint32_t t4[4] = {__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632), __byte_perm(hi01, hi23, 0x5410),
-                                __byte_perm(hi01, hi23, 0x7632)};
-#pragma unroll
-        for (int i = 0; i < 4; i++) store_bytes(pg + (d + i) * B + o, t4[i], -r, rows - r);
-      }
+      to_page([&](int r, int d) {
+        float v[4];
+        load_n<4>(x + (int64_t)(t + r) * stride + d, vec, v);
+        return quant4(v, inv, odd);
+      });
     }
     __syncthreads();  // every thread has read the old scale
     if (threadIdx.x == 0) scales[ph] = scale;
