@@ -243,7 +243,7 @@ RK_DEV void store_bytes(int8_t *p, uint32_t w, int from, int to) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int chunk, int log_block) {
+__global__ void __launch_bounds__(kAppThreads, sizeof(T) == 4 ? 4 : 6) k_kv8_append(AppendArgs a, int chunk, int log_block) {
   __shared__ float sh[kAppThreads / 32];
   __shared__ __align__(16) uint32_t s_rows[(kAppHeld + 128 * 4) / 4];  // rounded values, rows hs + 4 bytes apart
   const int head = blockIdx.y, lane = threadIdx.x & 31;
@@ -269,16 +269,27 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
     const int t = t0 + __ffs(begins) - 1;
     const int slot = __shfl_sync(0xffffffffu, mine, __ffs(begins) - 1);
     const int page = slot >> log_block, first = slot & (B - 1);
+    const int64_t ph = (int64_t)page * H + head;
+    const float had = first > 0 ? scales[ph] : 0.0f;
     int rows = 0;          // of the run
     bool regular = true;   // its slots follow one another
-    for (;;) {
-      const int u = t + rows + lane, s = u < a.tokens ? a.slots[u] : -1;
-      const bool in = s >= 0 && s < cap && s >> log_block == page;
-      const unsigned in_run = __ballot_sync(0xffffffffu, in);
-      const int n = in_run == 0xffffffffu ? 32 : __ffs(~in_run) - 1;
-      regular &= __all_sync(0xffffffffu, lane >= n || s == slot + rows + lane);
+    for (bool more = true; more;) {
+      int s[4];  // one round trip for 128 rows
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int u = t + rows + 32 * i + lane;
+        s[i] = u < a.tokens ? a.slots[u] : -1;
+      }
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const unsigned in = __ballot_sync(0xffffffffu, s[i] >= 0 && s[i] < cap && s[i] >> log_block == page);
+        const int k = !more ? 0 : in == 0xffffffffu ? 32 : __ffs(~in) - 1;
+        regular &= __all_sync(0xffffffffu, lane >= k || s[i] == slot + rows + 32 * i + lane);
+        n += k;
+        more &= k == 32;
+      }
       rows += n;
-      if (n < 32) break;
     }
 
     // Held runs: magnitudes compare as their bits do, two of 16 bits at once,
@@ -332,8 +343,6 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a, int ch
       odd = __syncthreads_or(odd);
     }
     m = cta_max(m, sh);
-    const int64_t ph = (int64_t)page * H + head;
-    const float had = first > 0 ? scales[ph] : 0.0f;
     float scale = fmaxf(had, __fmul_rn(m, u2f(K_1_127)));
     if (scale < u2f(K_TINY)) scale = 0.0f;
     const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
