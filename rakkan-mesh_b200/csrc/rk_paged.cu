@@ -246,9 +246,10 @@ template <class T>
 __global__ void __launch_bounds__(kAppThreads, sizeof(T) == 4 ? 4 : 6) k_kv8_append(AppendArgs a, int chunk, int log_block) {
   __shared__ float sh[kAppThreads / 32];
   __shared__ __align__(16) uint32_t s_rows[(kAppHeld + 128 * 4) / 4];  // rounded values, rows hs + 4 bytes apart
-  const int head = blockIdx.y, lane = threadIdx.x & 31;
-  const bool values = blockIdx.z != 0;
-  const int B = 1 << log_block, hs = a.c.head_size, H = a.c.kv_heads;
+  // The CTAs of one run side by side: its rows lie together in memory.
+  const int hs = a.c.head_size, H = a.c.kv_heads, B = 1 << log_block, lane = threadIdx.x & 31;
+  const int part = blockIdx.x % (2 * H), head = part >> 1;
+  const bool values = part & 1;
   const int cap = a.c.blocks << log_block;
   const T *x = static_cast<const T *>(values ? a.v : a.k) + (int64_t)head * hs;
   const int64_t stride = values ? a.v_stride : a.k_stride;
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kAppThreads, sizeof(T) == 4 ? 4 : 6) k_kv8_app
   const bool vec = stride * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   int8_t *cache = values ? a.c.v : a.c.k;
   float *scales = values ? a.c.v_scale : a.c.k_scale;
-  const int t0 = blockIdx.x * chunk;
+  const int t0 = blockIdx.x / (2 * H) * chunk;
 
   // The rows at which runs begin, of this chunk.
   const int mine = t0 + lane < a.tokens && lane < chunk ? a.slots[t0 + lane] : -1;
@@ -452,7 +453,9 @@ cudaError_t launch_kv8_append(const AppendArgs &a, int type, int sms, cudaStream
   const long long ctas = 2LL * a.tokens * a.c.kv_heads;
   int chunk = 1;  // rows a CTA looks through: more once every SM has several CTAs
   while (chunk < 32 && chunk < a.c.block && ctas / chunk > 32LL * sms) chunk *= 2;
-  const dim3 grid((a.tokens + chunk - 1) / chunk, a.c.kv_heads, 2);
+  const long long ctas_all = (long long)((a.tokens + chunk - 1) / chunk) * 2 * a.c.kv_heads;
+  if (ctas_all > 0x7fffffff) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)ctas_all);
   const int lb = a.c.block == 16 ? 4 : a.c.block == 32 ? 5 : a.c.block == 64 ? 6 : 7;
   switch (type) {
     case RK_ACT_F32: return launch_k(k_kv8_append<float>, grid, kAppThreads, 0, st, a, chunk, lb);
