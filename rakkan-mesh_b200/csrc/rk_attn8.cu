@@ -4,8 +4,8 @@
 
 namespace rk {
 
-// Joins the parts of the unit that crosses into CTA blockIdx.x + 1. The CTAs
-// that a unit crosses into share its rows. A row of a few parts is one warp's:
+// Joins the parts of the unit that crosses into CTA blockIdx.x + 1 of the main
+// kernel. The CTAs of all its crossings share its rows. A row of a few parts is one warp's:
 // its lanes weigh the parts side by side and then add them up, four
 // dimensions a lane. A row of many is a CTA's, a share of the parts to each warp.
 constexpr int kJoinWarps = 4, kJoinFew = 8;
@@ -25,7 +25,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int
   const float *p0 = parts + 2LL * rec.first * size;
   auto part_of = [&](int i) { return p0 + (2LL * i + (i == 0)) * size; };
   const bool few = n <= kJoinFew;
-  const int nth = b - rec.first - 1, step = n - 1;
+  const int nth = (b - rec.first - 1) * gridDim.y + blockIdx.y, step = (n - 1) * gridDim.y;
   const int row0 = few ? nth * kJoinWarps + warp : nth, row_step = few ? step * kJoinWarps : step;
   const int my0 = few ? 0 : warp * 32, my_step = few ? 32 : 32 * kJoinWarps;  // parts of this warp
   for (int row = row0; row < rec.rows; row += row_step) {
@@ -126,7 +126,8 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   // for them before it reads.
   const bool pdl = g_pdl;
   g_pdl = true;
-  e = launch_k(k_attn8_join, g.ctas - 1, 32 * kJoinWarps, 0, st, a, type, g);
+  // Units of up to 64 rows are joined by eight CTAs for each crossing.
+  e = launch_k(k_attn8_join, dim3(g.ctas - 1, rows ? 8 : 1), 32 * kJoinWarps, 0, st, a, type, g);
   g_pdl = pdl;
   return e;
 }

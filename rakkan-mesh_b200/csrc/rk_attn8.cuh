@@ -44,6 +44,8 @@
 // that crosses CTAs leaves its parts in the workspace, and a second kernel
 // joins them.
 #pragma once
+#include <type_traits>
+
 #include "rk_act.cuh"
 #include "rk_matvec.cuh"
 #include "rk_serve.cuh"
@@ -380,46 +382,65 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     char *ring = sm + wt * 2 * Shape::TILE;
     const int *table = a.table + (int64_t)req * a.max_blocks;
     const uint32_t page_bytes = (uint32_t)(H * HS) << lb;
-    const int8_t *k_head = a.c.k + (((int64_t)head * HS) << lb), *v_head = a.c.v + (((int64_t)head * HS) << lb);
-    int page[2];
+    // A lane's piece of 16 bytes: of the keys, 32 side by side; of the values,
+    // dimension lane / 2, half lane % 2 of the tile's tokens.
+    const int8_t *k_lane = a.c.k + (((int64_t)head * HS) << lb) + 16 * lane;
+    const int8_t *v_lane = a.c.v + (((int64_t)head * HS + (lane >> 1)) << lb) + 16 * (lane & 1);
+    const int key_piece = (16 * lane) ^ key_swizzle<HS>(16 * lane / HS);
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    const uint32_t my_pieces = (rw == 4 ? 0x11111111u : 0x55555555u) << wr;
+    int page[2];  // -1: outside the cache
     float ks = 0.0f, vs = 0.0f;  // scales of the next tile, of the page of this lane's tokens
     bool live = false;
-    auto usable = [&](int p) { return p >= 0 && p < a.c.blocks; };
     auto look_up = [&](int t) {
       page[0] = page[1] = -1;
       if (t < t_end) {
         const int tok = (q.tile0 + t) * TT;
         page[0] = __ldg(table + (tok >> lb));
-        page[1] = lb >= 5 ? page[0] : tok + 16 <= reach ? __ldg(table + (tok >> lb) + 1) : -1;
-        if (!usable(page[0]) || (tok + 16 <= reach && !usable(page[1]))) atomicExch(a.err, DEV_ERR_RANGE);
+        bool wrong = (unsigned)page[0] >= (unsigned)a.c.blocks;
+        if (wrong) page[0] = -1;
+        page[1] = page[0];
+        if (lb == 4) {
+          page[1] = tok + 16 <= reach ? __ldg(table + (tok >> lb) + 1) : 0;
+          if ((unsigned)page[1] >= (unsigned)a.c.blocks) wrong = true, page[1] = -1;
+        }
+        if (wrong) atomicExch(a.err, DEV_ERR_RANGE);
+      }
+    };
+    // The copies of a tile: piece i of a lane, by constant offsets.
+    auto copy_pieces = [&](auto log, uint32_t dst, const int8_t *k0, const int8_t *k1, const int8_t *v0) {
+      constexpr int LB = decltype(log)::value;
+#pragma unroll
+      for (int i = 0; i < KS; i++) {
+        if (rw > 1 && !(my_pieces >> i & 1)) continue;
+        const int8_t *k = LB > 4 || (KS % 2 ? 32 * i + lane < HS : 2 * i < KS) ? k0 : k1;
+        copy16(dst + key_piece + 512 * i, k + 512 * i);
+        copy16(dst + Shape::KBYTES + 16 * lane + 512 * i, v0 + (16 << LB) * i);
       }
     };
     auto copy_tile = [&](int t, int stage) {  // page[] is the tile's
       if (t < t_end) {
-        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + stage * Shape::TILE);
-        const int tok = (q.tile0 + t) * TT, in_page = tok & ((1 << lb) - 1);
-        const int64_t p0 = usable(page[0]) ? (int64_t)((uint64_t)(uint32_t)page[0] * page_bytes) : 0;
-        const int8_t *k0 = k_head + p0 + in_page * HS, *k1 = k0, *v0 = v_head + p0 + in_page + 16 * (lane & 1);
-        if (lb == 4) {
-          const int64_t p1 = usable(page[1]) ? (int64_t)((uint64_t)(uint32_t)page[1] * page_bytes) : 0;
-          k1 = k_head + p1 - 16 * HS;
-          if (lane & 1) v0 = v_head + p1;
-        }
-        v0 += (lane >> 1) << lb;
-#pragma unroll
-        for (int i = 0; i < KS; i++) {
-          if ((i & (rw - 1)) != wr) continue;
-          const int at = 16 * (32 * i + lane);  // of the tile's keys
-          copy16(dst + (at ^ key_swizzle<HS>(at / HS)), ((KS % 2 ? at < 16 * HS : 2 * i < KS) ? k0 : k1) + at);
-          copy16(dst + Shape::KBYTES + at, v0 + ((16 * i) << lb));
+        const uint32_t dst = ring_at + stage * Shape::TILE;
+        const int in_page = ((q.tile0 + t) * TT) & ((1 << lb) - 1);
+        const int64_t p0 = (int64_t)((uint64_t)(uint32_t)max(page[0], 0) * page_bytes);
+        const int8_t *k0 = k_lane + p0 + in_page * HS, *v0 = v_lane + p0 + in_page;
+        if (lb == 6) {
+          copy_pieces(std::integral_constant<int, 6>(), dst, k0, k0, v0);
+        } else if (lb == 5) {
+          copy_pieces(std::integral_constant<int, 5>(), dst, k0, k0, v0);
+        } else if (lb == 7) {
+          copy_pieces(std::integral_constant<int, 7>(), dst, k0, k0, v0);
+        } else {
+          const int64_t p1 = (int64_t)((uint64_t)(uint32_t)max(page[1], 0) * page_bytes);
+          copy_pieces(std::integral_constant<int, 4>(), dst, k0, k_lane + p1 - 16 * HS, lane & 1 ? v_lane + p1 - 16 : v0);
         }
       }
       copy_commit();
     };
     auto load_scales = [&](int t) {
       const int p = page[r >> 2];
-      live = t < t_end && usable(p);
-      const int64_t ph = live ? (int64_t)p * H + head : 0;
+      live = t < t_end && p >= 0;
+      const int64_t ph = (int64_t)max(p, 0) * H + head;
       ks = live ? __ldg(a.c.k_scale + ph) : 0.0f;
       vs = live ? __ldg(a.c.v_scale + ph) : 0.0f;
     };
