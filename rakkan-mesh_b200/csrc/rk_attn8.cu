@@ -4,15 +4,29 @@
 
 namespace rk {
 
-// Joins the parts of the unit that crosses into CTA blockIdx.x + 1 of the main
-// kernel. The CTAs of all its crossings share its rows. A row of a few parts is one warp's:
-// its lanes weigh the parts side by side and then add them up, four
-// dimensions a lane. A row of many is a CTA's, a share of the parts to each warp.
+RK_DEV float warp_top(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+RK_DEV float warp_total(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Joins the parts of the unit that crosses into CTA c of the main kernel
+// (c = blockIdx.x + 1). The CTAs of all its crossings share its rows. A row of a
+// few parts is one warp's, a row of many all four's: a warp's lanes read its
+// parts' (m, M, l) side by side, then the sums, four dimensions a lane, with
+// all loads under way at once; each step is a round trip to L2, and there is
+// little else to the call.
 constexpr int kJoinWarps = 4, kJoinFew = 8;
 
+template <int J>  // pieces of 128 dimensions
 __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int type, A8Grid grid) {
-  __shared__ float4 s_v[kJoinWarps][2][32];
-  __shared__ float s_l[kJoinWarps];
+  __shared__ float4 s_v[kJoinWarps][J][32];
+  __shared__ float s_st[kJoinWarps][3];
   griddep_wait();
   const A8Record *records = static_cast<const A8Record *>(a.ws);
   const float *parts = reinterpret_cast<const float *>(records + grid.ctas);
@@ -27,68 +41,80 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int
   const bool few = n <= kJoinFew;
   const int nth = (b - rec.first - 1) * gridDim.y + blockIdx.y, step = (n - 1) * gridDim.y;
   const int row0 = few ? nth * kJoinWarps + warp : nth, row_step = few ? step * kJoinWarps : step;
-  const int my0 = few ? 0 : warp * 32, my_step = few ? 32 : 32 * kJoinWarps;  // parts of this warp
+  const int my0 = few ? 0 : warp, my_step = few ? 1 : kJoinWarps;  // parts of this warp
   for (int row = row0; row < rec.rows; row += row_step) {
     float mm = -INFINITY, MM = -INFINITY, ll = 0.0f;
-    for (int i = lane; i < n; i += 32) {
-      const float *s = part_of(i) + 64 * hs + 4 * row;
-      mm = fmaxf(mm, s[0]);
-      MM = fmaxf(MM, s[1]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-      MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, o));
-    }
-    const float msafe = mm == -INFINITY ? 0.0f : mm, Msafe = MM == -INFINITY ? 0.0f : MM;
-    float4 v[2] = {};
-    for (int i0 = my0; i0 < n; i0 += my_step) {
-      const int k = min(32, n - i0);
-      float g = 0.0f;
+    float4 v[J] = {};
+    for (int i0 = my0; i0 < n; i0 += 32 * my_step) {
+      const int k = min(32, (n - i0 + my_step - 1) / my_step);
+      float m = -INFINITY, M = -INFINITY, l = 0.0f;
       if (lane < k) {
-        const float *s = part_of(i0 + lane) + 64 * hs + 4 * row;
-        g = exp2f(s[1] - Msafe);
-        ll += s[2] * exp2f(s[0] - msafe);
+        const float4 s = *reinterpret_cast<const float4 *>(part_of(i0 + lane * my_step) + 64 * hs + 4 * row);
+        m = s.x, M = s.y, l = s.z;
       }
-#pragma unroll 8
-      for (int i = 0; i < k; i++) {
-        const float w = __shfl_sync(0xffffffffu, g, i);
-        const float *p = part_of(i0 + i) + row * hs;
+      const float m1 = fmaxf(mm, warp_top(m)), M1 = fmaxf(MM, warp_top(M));
+      const float ms = m1 == -INFINITY ? 0.0f : m1, Ms = M1 == -INFINITY ? 0.0f : M1;
+      const float g = exp2f(M - Ms), old = exp2f(MM - Ms);
+      ll = ll * exp2f(mm - ms) + warp_total(l * exp2f(m - ms));
+      mm = m1, MM = M1;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const int d = 4 * lane + 128 * j;
-          if (d >= hs) break;
-          const float4 x = *reinterpret_cast<const float4 *>(p + d);
-          v[j].x = fmaf(x.x, w, v[j].x);
-          v[j].y = fmaf(x.y, w, v[j].y);
-          v[j].z = fmaf(x.z, w, v[j].z);
-          v[j].w = fmaf(x.w, w, v[j].w);
+      for (int j = 0; j < J; j++) v[j].x *= old, v[j].y *= old, v[j].z *= old, v[j].w *= old;
+      for (int i1 = 0; i1 < k; i1 += 8) {
+        float4 x[8][J];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+          for (int j = 0; j < J; j++) {
+            const int d = 4 * lane + 128 * j;
+            x[i][j] = i1 + i < k && d < hs ? *reinterpret_cast<const float4 *>(part_of(i0 + (i1 + i) * my_step) + row * hs + d)
+                                           : make_float4(0, 0, 0, 0);
+          }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float w = __shfl_sync(0xffffffffu, g, min(i1 + i, 31));
+#pragma unroll
+          for (int j = 0; j < J; j++)
+            if (i1 + i < k) {
+              v[j].x = fmaf(x[i][j].x, w, v[j].x);
+              v[j].y = fmaf(x[i][j].y, w, v[j].y);
+              v[j].z = fmaf(x[i][j].z, w, v[j].z);
+              v[j].w = fmaf(x[i][j].w, w, v[j].w);
+            }
         }
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
     if (!few) {
       __syncthreads();
-      s_v[warp][0][lane] = v[0];
-      s_v[warp][1][lane] = v[1];
-      if (lane == 0) s_l[warp] = ll;
+#pragma unroll
+      for (int j = 0; j < J; j++) s_v[warp][j][lane] = v[j];
+      if (lane == 0) s_st[warp][0] = mm, s_st[warp][1] = MM, s_st[warp][2] = ll;
       __syncthreads();
       if (warp > 0) continue;
-      for (int w = 1; w < kJoinWarps; w++) {
-        ll += s_l[w];
+      float m1 = mm, M1 = MM;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
+      for (int w = 1; w < kJoinWarps; w++) m1 = fmaxf(m1, s_st[w][0]), M1 = fmaxf(M1, s_st[w][1]);
+      const float ms = m1 == -INFINITY ? 0.0f : m1, Ms = M1 == -INFINITY ? 0.0f : M1;
+      ll = 0.0f;
+#pragma unroll
+      for (int j = 0; j < J; j++) v[j] = make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; w++) {
+        ll += s_st[w][2] * exp2f(s_st[w][0] - ms);
+        const float g = exp2f(s_st[w][1] - Ms);
+#pragma unroll
+        for (int j = 0; j < J; j++) {
           const float4 x = s_v[w][j][lane];
-          v[j].x += x.x, v[j].y += x.y, v[j].z += x.z, v[j].w += x.w;
+          v[j].x = fmaf(x.x, g, v[j].x), v[j].y = fmaf(x.y, g, v[j].y);
+          v[j].z = fmaf(x.z, g, v[j].z), v[j].w = fmaf(x.w, g, v[j].w);
         }
       }
+      mm = m1, MM = M1;
     }
-    const float scale = ll == 0.0f ? 0.0f : exp2f(Msafe - 14.0f - msafe) / ll;
+    const float scale = ll == 0.0f ? 0.0f : exp2f((MM == -INFINITY ? 0.0f : MM) - 14.0f - (mm == -INFINITY ? 0.0f : mm)) / ll;
     const int qrow = rec.row0 + row;
     const int64_t oi = (int64_t)(rec.q0 + qrow / G) * a.out_stride + (int64_t)(rec.head * G + qrow % G) * hs;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < J; j++) {
       const int d = 4 * lane + 128 * j;
       if (d >= hs) break;
       o_store(a.out, type, oi + d, v[j].x * scale);
@@ -127,7 +153,7 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   const bool pdl = g_pdl;
   g_pdl = true;
   // Units of up to 64 rows are joined by eight CTAs for each crossing.
-  e = launch_k(k_attn8_join, dim3(g.ctas - 1, rows ? 8 : 1), 32 * kJoinWarps, 0, st, a, type, g);
+  e = launch_k(hs > 128 ? k_attn8_join<2> : k_attn8_join<1>, dim3(g.ctas - 1, rows ? 8 : 1), 32 * kJoinWarps, 0, st, a, type, g);
   g_pdl = pdl;
   return e;
 }
