@@ -141,7 +141,7 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   const int terms = type == RK_ACT_F32 || (type == RK_ACT_F16 && !rows) ? 2 : 1;
   const int nt = terms == 1 && rows && hs <= 128 ? 2 : 1;
   A8Grid g{sms * a8_ctas(hs, terms, nt), 4, a.c.block == 16 ? 4 : a.c.block == 32 ? 5 : a.c.block == 64 ? 6 : 7,
-           a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0};
+           a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0, G > 1 ? 0xffffffffu / G + 1 : 0};
   // Short tables: a unit's tiles are few for one CTA, and without units cut in
   // two there is nothing to join.
   const bool whole = (int64_t)a.max_blocks * a.c.block <= 512;

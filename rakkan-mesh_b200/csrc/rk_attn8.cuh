@@ -56,6 +56,10 @@ constexpr int kA8Warps = 4;
 constexpr int kA8Threads = 32 * kA8Warps;
 
 constexpr int kA8Tile = 32;  // tokens
+// What a unit's beginning and end cost a CTA, in tiles (about 5 us against 0.6
+// us a tile where memory bounds them; 12 measured best of 0 to 14): CTAs that begin a second unit get so
+// many tiles less.
+constexpr int kA8Begin = 12;
 template <int HS>
 struct A8Shape {
   static constexpr int KS = HS / 16;        // 16-long steps over a head
@@ -85,6 +89,7 @@ struct A8Grid {
   int min_tiles;  // fewest tiles worth a CTA; 0: a CTA takes whole units
   int log_block;  // of the page's tokens
   bool vec_q;     // rows of q lie on 16-byte boundaries
+  uint32_t by_group;  // ceil(2^32 / G), for quotients (0: G is 1)
 };
 
 RK_DEV uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
@@ -276,6 +281,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   __shared__ int s_req;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   const int G = a.heads / a.c.kv_heads, H = a.c.kv_heads, lb = grid.log_block;
+  const auto token_of = [&](int row) { return grid.by_group ? (int)__umulhi(row, grid.by_group) : row; };
   griddep_trigger();
 
   // The run of tiles (or of whole units) of this CTA: a scan over the
@@ -283,7 +289,9 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   const bool by_unit = grid.min_tiles == 0;
   const int per_t = (a.n + kA8Threads - 1) / kA8Threads;
   const int i0 = min(a.n, tid * per_t), i1 = min(a.n, i0 + per_t);
-  auto size_of = [&](const A8Req &q) { return (long long)H * q.units * (by_unit ? 1 : q.tiles); };
+  // A unit counts kA8Begin tiles more than it has, in front of them.
+  auto length_of = [&](const A8Req &q) { return by_unit ? 1 : q.tiles + kA8Begin; };
+  auto size_of = [&](const A8Req &q) { return (long long)H * q.units * length_of(q); };
   long long mine = 0;
   for (int i = i0; i < i1; i++) mine += size_of(a8_req<HS, R>(a, lb, i));
   long long incl = mine;
@@ -303,10 +311,8 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   const long long begin = per * blockIdx.x, end = min(total, begin + per);
   A8Record *records = static_cast<A8Record *>(a.ws);
   float *parts = reinterpret_cast<float *>(records + grid.ctas);
-  if (begin >= end) {
-    if (tid == 0 && !by_unit) records[blockIdx.x].first = -1;
-    return;
-  }
+  if (tid == 0 && !by_unit) records[blockIdx.x].first = -1;
+  if (begin >= end) return;
   if (begin >= excl && begin < excl + mine) {
     long long p = excl;
     for (int i = i0; i < i1; i++) {
@@ -330,11 +336,13 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       base += size_of(q);
       q = a8_req<HS, R>(a, lb, ++req);
     }
-    const int step = by_unit ? 1 : q.tiles;
-    const int u = (int)(at - base) / step;
+    const int step = length_of(q);
+    const int u = (uint32_t)(at - base) / (uint32_t)step;
     const int head = u / q.units, rg = u % q.units;
     const long long u0 = base + (long long)u * step, u1 = u0 + step;
-    const int t0 = (int)(at - u0), t1 = by_unit ? q.tiles : (int)(min(end, u1) - u0);
+    const int t0 = by_unit ? 0 : max(0, (int)(at - u0) - kA8Begin);
+    const int t1 = by_unit ? q.tiles : (int)(min(end, u1) - u0) - kA8Begin;
+    if (t1 <= 0) break;  // the run ends before the unit's first tile
     const int rw = q.rw, tw = kA8Warps / rw, wr = warp % rw, wt = warp / rw;
     const int row0 = (rg * rw + wr) * R;        // of the request's nq·G rows (token-major)
     const int all_rows = q.nq * G;
@@ -354,7 +362,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         high[n][e] = 0x7fffffff;
         low[n][e] = -1;
         if (row < all_rows) {
-          const int pos = pos0 + row / G;
+          const int pos = pos0 + token_of(row);
           high[n][e] = max(-1, min(pos, q.len - 1));
           if (a.window > 0 && pos >= a.window) low[n][e] = pos - a.window;
           high_max = max(high_max, high[n][e]);
@@ -369,8 +377,8 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       low_max = max(low_max, __shfl_xor_sync(0xffffffffu, low_max, o));
     }
     // The same of the whole unit: the tiles that its warps go through together.
-    const int reach = max(-1, min(pos0 + (unit_row0 + unit_rows - 1) / G, q.len - 1));
-    const int pos_first = pos0 + unit_row0 / G;
+    const int reach = max(-1, min(pos0 + token_of(unit_row0 + unit_rows - 1), q.len - 1));
+    const int pos_first = pos0 + token_of(unit_row0);
     const int t_first = a.window > 0 && pos_first >= a.window
                             ? max(t0, min(q.len, pos_first - a.window + 1) / TT - q.tile0) : t0;
     const int t_end = min(t1, reach / TT + (reach >= 0) - q.tile0);
@@ -457,39 +465,45 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     for (int n = 0; n < NT; n++) {
       const int row = row0 + 8 * n + r;
       const bool have = row < all_rows;
-      const int64_t qi = have ? (int64_t)(q.q0 + row / G) * a.q_stride + (int64_t)(head * G + row % G) * HS : 0;
-      float top = 0.0f, v[KS][4];
-      bool wrong = false;
+      const int tq = have ? token_of(row) : 0;
+      const int64_t qi = have ? (q.q0 + tq) * a.q_stride + (head * G + row - tq * G) * HS : 0;
+      float v[KS][4];
 #pragma unroll
       for (int s = 0; s < KS; s++) v[s][0] = v[s][1] = v[s][2] = v[s][3] = 0.0f;
       if (have) by_stretch<HS>(c, LoadQuery<HS>{a.q, qi, type, grid.vec_q, v[0]});
+      // The largest magnitude, as bits: infinities and NaN come out on top.
+      uint32_t most = 0;
 #pragma unroll
       for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-          top = fmaxf(top, fabsf(v[s][b]));
-          wrong |= !(fabsf(v[s][b]) < INFINITY);
-        }
+        for (int b = 0; b < 4; b++) most = max(most, f2u(v[s][b]) & 0x7fffffffu);
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      wrong = (__ballot_sync(0xffffffffu, wrong) >> (lane & 28) & 15) != 0;
-      // The row as integers of DIGITS signed bytes, its largest at the top.
-      constexpr float LIMIT = DIGITS == 2 ? 127 * 257 : 127 * 65793;
-      top = fmaxf(top, u2f(27u << 23));  // 2^-100: the quotients stay finite
+      for (int o = 1; o < 4; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      // The row as integers of DIGITS signed bytes, its largest at the top. (Of
+      // a row that is not finite any integers: its factor makes its scores NaN.)
+      // Three bytes hold 127·65793; two less, since the product's rounding may add one.
+      constexpr float LIMIT = DIGITS == 2 ? 127 * 257 : 127 * 65793 - 2;
+      const float top = fmaxf(u2f(most), u2f(27u << 23));  // 2^-100: the quotients stay finite
       const float up = LIMIT / top;
-      const float fr = wrong ? u2f(kCanonNaN) : (top / LIMIT) * (a.scale * 1.44269504088896f);
+      const float fr = most >= 0x7f800000u ? u2f(kCanonNaN) : (top * (1.0f / LIMIT)) * (a.scale * 1.44269504088896f);
       f[n][0] = __shfl_sync(0xffffffffu, fr, 8 * c);
       f[n][1] = __shfl_sync(0xffffffffu, fr, 8 * c + 4);
 #pragma unroll
       for (int s = 0; s < KS; s++) {
-        int w[4];
+        uint32_t w[4];
 #pragma unroll
-        for (int b = 0; b < 4; b++) w[b] = wrong ? 0 : __float2int_rn(fminf(LIMIT, fmaxf(-LIMIT, v[s][b] * up)));
+        for (int b = 0; b < 4; b++)
+          w[b] = DIGITS == 2 ? f2u(fmaf(v[s][b], up, 12582912.0f)) : (uint32_t)__float2int_rn(v[s][b] * up);
+        // The lowest byte as a signed one; the rest is a multiple of 256: the
+        // next byte of w + 128, and that of w + 128 + 128·256.
+        qb[n][DIGITS - 1][s] = pack_bytes(w[0], w[1], w[2], w[3]);
 #pragma unroll
-        for (int x = DIGITS - 1; x >= 0; x--) {  // the lowest byte first, as a signed one; the rest is a multiple of 256
-          qb[n][x][s] = prmt(prmt(w[0], w[1], 0x0040), prmt(w[2], w[3], 0x0040), 0x5410);
+        for (int b = 0; b < 4; b++) w[b] += 0x80u;
+        qb[n][DIGITS - 2][s] = prmt(prmt(w[0], w[1], 0x0051), prmt(w[2], w[3], 0x0051), 0x5410);
+        if constexpr (DIGITS == 3) {
 #pragma unroll
-          for (int b = 0; b < 4; b++) w[b] = (w[b] + 128) >> 8;
+          for (int b = 0; b < 4; b++) w[b] += 0x8000u;
+          qb[n][0][s] = prmt(prmt(w[0], w[1], 0x0062), prmt(w[2], w[3], 0x0062), 0x5410);
         }
       }
       if (KS % 2)
@@ -676,7 +690,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         }
       }
     __syncthreads();
-    const bool starts = by_unit || at == u0, ends = by_unit || u1 <= end;
+    const bool starts = t0 == 0, ends = u1 <= end;
     float *part = parts + (2LL * blockIdx.x + (starts ? 1 : 0)) * a8_part_floats(HS);
     for (int row = warp; row < unit_rows; row += kA8Warps) {
       const int tile = row / R, rr = row % R;
@@ -691,12 +705,12 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       for (int w = 0; w < kA8Warps; w++) {
         if (w >= tw) break;
         const float *s = s_st + ((tile + w * rw) * R + rr) * 4;
-        ll += s[2] * exp2f(s[0] - msafe);
-        g[w] = exp2f(s[1] - Msafe);
+        ll += s[2] * ex2(s[0] - msafe);
+        g[w] = ex2(s[1] - Msafe);
       }
-      const int qrow = unit_row0 + row;
-      const float scale = ll == 0.0f ? 0.0f : exp2f(Msafe - 14.0f - msafe) / ll;
-      const int64_t oi = (int64_t)(q.q0 + qrow / G) * a.out_stride + (int64_t)(head * G + qrow % G) * HS;
+      const int qrow = unit_row0 + row, tq = token_of(qrow);
+      const float scale = ll == 0.0f ? 0.0f : ex2(Msafe - 14.0f - msafe) / ll;
+      const int64_t oi = (q.q0 + tq) * a.out_stride + (head * G + qrow - tq * G) * HS;
       for (int d = lane; d < HS; d += 32) {
         float v = 0.0f;
 #pragma unroll
@@ -714,9 +728,9 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         s[2] = ll;
       }
     }
-    if (at == begin && tid == 0 && !by_unit) {
+    if (!starts && tid == 0) {  // the CTA's first unit, begun in another one
       A8Record rec;
-      rec.first = starts ? -1 : (int)(u0 / per);
+      rec.first = (int)((u0 + kA8Begin) / per);
       rec.last = (int)((u1 - 1) / per);
       rec.req = req;
       rec.head = head;
