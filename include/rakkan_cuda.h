@@ -562,7 +562,10 @@ int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const voi
  * (float32: as two, 22 bits); weights below 2^-126 of the largest count as
  * zero.
  * workspace: rk_kv8_attention_workspace() bytes, 16-byte aligned, used during the
- * call's kernels only; calls that may run at once need one each. */
+ * call's kernels only; calls that may run at once (on different streams, or
+ * captured into graphs that may) need one each. A table of at most
+ * RK_KV8_NO_WORKSPACE tokens (max_blocks * block) needs none. */
+#define RK_KV8_NO_WORKSPACE 512
 int64_t rk_kv8_attention_workspace(rk_device *d, const rk_kv8 *c, int heads);
 int rk_kv8_attention(rk_device *d, const rk_kv8 *c, int type, int n, int heads, int tokens, const void *q,
                      int64_t q_stride, const int32_t *q_start, const int32_t *lens, const int32_t *table,

@@ -144,7 +144,7 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
            a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0, G > 1 ? 0xffffffffu / G + 1 : 0};
   // Short tables: a unit's tiles are few for one CTA, and without units cut in
   // two there is nothing to join.
-  const bool whole = (int64_t)a.max_blocks * a.c.block <= 512;
+  const bool whole = (int64_t)a.max_blocks * a.c.block <= RK_KV8_NO_WORKSPACE;
   if (whole) g.min_tiles = 0;
   cudaError_t e = terms == 2 ? attn8_main_two(a, type, g, st) : A8<1>::at(hs, A8<1>::Launch{a, type, nt, g, st});
   if (e != cudaSuccess || whole) return e;

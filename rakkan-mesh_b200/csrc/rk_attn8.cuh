@@ -649,6 +649,10 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         // Tokens 8c .. 8c + 7 of two dimensions.
         const uint2 v0 = *reinterpret_cast<const uint2 *>(vt + (16 * d + r) * TT + 8 * c);
         const uint2 v1 = *reinterpret_cast<const uint2 *>(vt + (16 * d + 8 + r) * TT + 8 * c);
+        // Float32 results: a tile's sums of their own, added outside. The
+        // products' adder does not round, and over thousands of tokens that
+        // shows (6.7e-6 of the result over 4600).
+        float part[NT][4] = {};
 #pragma unroll
         for (int s = 0; s < 2; s++) {
           uint32_t va[4];
@@ -657,8 +661,13 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int x = TERMS - 1; x >= 0; x--) mma16816(o[n][d], va, pb[s][n][x][0], pb[s][n][x][1]);
+            for (int x = TERMS - 1; x >= 0; x--) mma16816(TERMS == 2 ? part[n] : o[n][d], va, pb[s][n][x][0], pb[s][n][x][1]);
         }
+        if (TERMS == 2)
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) o[n][d][x] += part[n][x];
       }
     }
     copy_wait<0>();

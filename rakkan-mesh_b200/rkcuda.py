@@ -23,6 +23,7 @@ MAX_COLS, MAX_ROWS = 1 << 18, 1 << 20
 NOALLOC_MAX_COLS = 32768
 ACT_F32, ACT_F16, ACT_BF16 = 0, 1, 2
 MAX_REQUESTS = 16384
+KV8_NO_WORKSPACE = 512
 
 # Every symbol include/rakkan_cuda.h declares.
 EXPORTS = [
@@ -855,9 +856,13 @@ def _torch():
         # reads NULL as the device's own, so the legacy stream's handle is passed.
         _t = types.SimpleNamespace(
             torch=torch, stream=lambda index: torch._C._cuda_getCurrentRawStream(index) or 1,
+            capturing=torch.cuda.is_current_stream_capturing,
             act={torch.float32: ACT_F32, torch.float16: ACT_F16, torch.bfloat16: ACT_BF16},
             f32=torch.float32, i32=torch.int32, i8=torch.int8, u8=torch.uint8)
     return _t
+
+
+_workspaces = {}  # by device and stream
 
 
 def _refuse(msg):
@@ -866,7 +871,7 @@ def _refuse(msg):
 
 def _tensor(x, index, dtype, what, shape=None):
     """A contiguous tensor of the dtype on the device (and of the shape): its address."""
-    if not x.is_cuda or x.get_device() != index:
+    if x.get_device() != index:
         _refuse(f"{what}: a tensor on {x.device}, not on cuda:{index}")
     if x.dtype is not dtype:
         _refuse(f"{what}: a tensor of {x.dtype}, not of {dtype}")
@@ -877,26 +882,23 @@ def _tensor(x, index, dtype, what, shape=None):
     return x.data_ptr()
 
 
-def _rows(x, index, dtype, what, shape):
-    """A tensor of rows that are contiguous inside and lie a stride apart: its address and that stride."""
-    if not x.is_cuda or x.get_device() != index:
+def _rows(x, index, dtype, what, shape, width):
+    """A tensor of rows of `width` values that are contiguous inside and lie a
+    stride apart: its address and that stride."""
+    if x.get_device() != index:
         _refuse(f"{what}: a tensor on {x.device}, not on cuda:{index}")
     if x.dtype is not dtype:
         _refuse(f"{what}: a tensor of {x.dtype}, not of {dtype}")
     if x.shape != shape:
         _refuse(f"{what}: shape {tuple(x.shape)}, not {tuple(shape)}")
-    if not x.is_contiguous():
-        want = 1
-        for size, stride in zip(reversed(shape[1:]), reversed(x.stride()[1:])):
-            if size != 1 and stride != want:
-                _refuse(f"{what}: rows that are not contiguous inside (strides {x.stride()})")
-            want *= size
-        if shape[0] > 1:
-            return x.data_ptr(), x.stride(0)
-    width = 1
-    for size in shape[1:]:
-        width *= size
-    return x.data_ptr(), width
+    if x.is_contiguous():
+        return x.data_ptr(), width
+    want, strides = 1, x.stride()
+    for size, stride in zip(reversed(shape[1:]), reversed(strides[1:])):
+        if size != 1 and stride != want:
+            _refuse(f"{what}: rows that are not contiguous inside (strides {strides})")
+        want *= size
+    return x.data_ptr(), strides[0] if shape[0] > 1 else width
 
 
 def device_check(dev):
@@ -973,9 +975,9 @@ class PagedKV8:
         if act is None:
             _refuse(f"kv8 append: keys of {k.dtype}")
         n = slots.numel()
-        shape = (n, self.kv_heads, self.head_size)
-        kp, ks = _rows(k, i, k.dtype, "kv8 append: k", shape)
-        vp, vs = _rows(v, i, k.dtype, "kv8 append: v", shape)
+        shape, width = (n, self.kv_heads, self.head_size), self.kv_heads * self.head_size
+        kp, ks = _rows(k, i, k.dtype, "kv8 append: k", shape, width)
+        vp, vs = _rows(v, i, k.dtype, "kv8 append: v", shape, width)
         sp = _tensor(slots, i, t.i32, "kv8 append: slots", (n,))
         rc = _lib.rk_kv8_append(self.dev.h, self.at, act, n, kp, ks, vp, vs, sp, t.stream(i))
         if rc:
@@ -995,25 +997,34 @@ class PagedKV8:
             _refuse(f"kv8 attention: queries of shape {tuple(q.shape)}, head size {self.head_size}")
         shape = q.shape
         tokens, heads = shape[0], shape[1]
+        width = heads * self.head_size
         n, max_blocks = table.shape
-        qp, qs = _rows(q, i, q.dtype, "kv8 attention: q", shape)
+        qp, qs = _rows(q, i, q.dtype, "kv8 attention: q", shape, width)
         if out is None:
-            out = t.torch.empty(shape, dtype=q.dtype, device=q.device)
-        op, os_ = _rows(out, i, q.dtype, "kv8 attention: out", shape)
+            out = t.torch.empty_like(q, memory_format=t.torch.contiguous_format)
+            op, os_ = out.data_ptr(), width
+        else:
+            op, os_ = _rows(out, i, q.dtype, "kv8 attention: out", shape, width)
         tp = _tensor(table, i, t.i32, "kv8 attention: table")
         lp = _tensor(lens, i, t.i32, "kv8 attention: lens", (n,))
         sp = None if q_start is None else _tensor(q_start, i, t.i32, "kv8 attention: q_start", (n + 1,))
-        need = self._ws.get(heads)
-        if need is None:
-            need = _lib.rk_kv8_attention_workspace(self.dev.h, self.at, heads)
-            if need < 0:
-                _check(need)
-            self._ws[heads] = need
-        # A workspace of each call's own, from torch's allocator: it belongs to
-        # the stream (or to the graph being captured) that uses it.
-        ws = t.torch.empty(need, dtype=t.u8, device=q.device) if need else None
+        stream, ws, need = t.stream(i), None, 0
+        if max_blocks * self.block > KV8_NO_WORKSPACE:
+            need = self._ws.get(heads)
+            if need is None:
+                need = _lib.rk_kv8_attention_workspace(self.dev.h, self.at, heads)
+                if need < 0:
+                    _check(need)
+                self._ws[heads] = need
+            # One workspace a stream, whose calls follow one another; in a
+            # capture one of the graph's own, which may run beside others.
+            ws = None if t.capturing() else _workspaces.get((i, stream))
+            if ws is None or ws.numel() < need:
+                ws = t.torch.empty(need, dtype=t.u8, device=q.device)
+                if not t.capturing():
+                    _workspaces[i, stream] = ws
         rc = _lib.rk_kv8_attention(self.dev.h, self.at, act, n, heads, tokens, qp, qs, sp, lp, tp, max_blocks, scale, window,
-                                   op, os_, ws.data_ptr() if need else None, need, t.stream(i))
+                                   op, os_, ws.data_ptr() if need else None, need, stream)
         if rc:
             _check(rc)
         return out
@@ -1030,17 +1041,21 @@ def add_rmsnorm_q8(dev, x, weight, eps, group=32, residual=None, sum_out=None):
         _refuse(f"norm q8: x of {x.dtype} and {x.dim()} dimensions")
     shape = x.shape
     rows, cols = shape
-    xp, xs = _rows(x, i, x.dtype, "norm q8: x", shape)
+    xp, xs = _rows(x, i, x.dtype, "norm q8: x", shape, cols)
     wp = _tensor(weight, i, x.dtype, "norm q8: weight", (cols,))
-    rp, rs = (None, cols) if residual is None else _rows(residual, i, x.dtype, "norm q8: residual", shape)
-    if sum_out is None and residual is not None:
-        sum_out = t.torch.empty(shape, dtype=x.dtype, device=x.device)
-    sp, ss = (None, cols) if sum_out is None else _rows(sum_out, i, x.dtype, "norm q8: sum_out", shape)
+    rp, rs = (None, cols) if residual is None else _rows(residual, i, x.dtype, "norm q8: residual", shape, cols)
+    if sum_out is not None:
+        sp, ss = _rows(sum_out, i, x.dtype, "norm q8: sum_out", shape, cols)
+    elif residual is not None:
+        sum_out = t.torch.empty_like(x, memory_format=t.torch.contiguous_format)
+        sp, ss = sum_out.data_ptr(), cols
+    else:
+        sp, ss = None, cols
     if group < 0 or group and cols % group:
         _refuse(f"norm q8: groups of {group} in {cols} columns")
-    q = t.torch.empty(shape, dtype=t.i8, device=x.device)
-    scales = t.torch.empty((rows, cols // (group or cols)), dtype=t.f32, device=x.device)
-    rc = lib().rk_add_rmsnorm_q8(dev.h, act, rows, cols, group, xp, xs, rp, rs, wp, eps, sp, ss, q.data_ptr(), scales.data_ptr(),
+    q = t.torch.empty_like(x, dtype=t.i8, memory_format=t.torch.contiguous_format)
+    scales = x.new_empty((rows, cols // group if group else 1), dtype=t.f32)
+    rc = _lib.rk_add_rmsnorm_q8(dev.h, act, rows, cols, group, xp, xs, rp, rs, wp, eps, sp, ss, q.data_ptr(), scales.data_ptr(),
                                  t.stream(i))
     if rc:
         _check(rc)
@@ -1080,11 +1095,11 @@ class W4Matrix:
         if groups < 1 or self.cols % groups:
             _refuse(f"w4: {groups} scales a vector for {self.cols} columns")
         if out is None:
-            out = t.torch.empty((n, self.rows), dtype=t.f32 if dtype is None else dtype, device=x.device)
+            out = x.new_empty((n, self.rows), dtype=t.f32 if dtype is None else dtype)
         act = t.act.get(out.dtype)
         if act is None:
             _refuse(f"w4: an output of {out.dtype}")
-        op, os_ = _rows(out, i, out.dtype, "w4: out", (n, self.rows))
+        op, os_ = _rows(out, i, out.dtype, "w4: out", (n, self.rows), self.rows)
         rc = _lib.rk_w4_mulvec(self.h, n, xp, sp, self.cols // groups, act, op, os_, t.stream(i))
         if rc:
             _check(rc)

@@ -505,17 +505,23 @@ def test_attention_offsets_past_32_bits(torch, dev):
 
 
 def test_attention_workspace_is_checked(torch, dev):
+    """Wide tables need the workspace, whole and aligned; those of 512 tokens none."""
     import ctypes as C
     kv = rk.PagedKV8.new(dev, 2, 1, 16, 32)
     need = rk.lib().rk_kv8_attention_workspace(dev.h, kv.at, 2)
-    assert need >= 0
-    q = torch.zeros((1, 2, 32), device="cuda")
-    table, lens = ints(torch, [[0]]), ints(torch, [3])
-    if need:
-        for ws, size in ((None, need), (q.data_ptr(), need - 1), (q.data_ptr() + 4, need)):
-            rc = rk.lib().rk_kv8_attention(dev.h, kv.at, 0, 1, 2, 1, q.data_ptr(), 64, None, lens.data_ptr(), table.data_ptr(), 1,
-                                           C.c_float(0), 0, q.data_ptr(), 64, ws, size, None)
-            assert rc == rk.RK_ERR_ARGS
+    assert need > 0
+    q, lens = torch.zeros((1, 2, 32), device="cuda"), ints(torch, [3])
+
+    def call(width, ws, size):
+        table = torch.zeros((1, width), dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()  # the call runs on the device's own stream
+        return rk.lib().rk_kv8_attention(dev.h, kv.at, 0, 1, 2, 1, q.data_ptr(), 64, None, lens.data_ptr(), table.data_ptr(), width,
+                                         C.c_float(0), 0, q.data_ptr(), 64, ws, size, None)
+    for ws, size in ((None, need), (q.data_ptr(), need - 1), (q.data_ptr() + 4, need)):
+        assert call(33, ws, size) == rk.RK_ERR_ARGS
+    assert call(32, None, 0) == rk.RK_OK
+    rk.device_check(dev)
+    torch.cuda.synchronize()
 
 
 # ---- norm --------------------------------------------------------------
