@@ -525,7 +525,9 @@ int rk_page_tables(rk_device *d, int n, int block, const int32_t *ctx_lens, cons
  * the key k[p][h][o][head_size] * k_scale[p][h] and the value
  * v[p][h][head_size][o] * v_scale[p][h] (values are transposed within a
  * page). block is 16, 32, 64 or 128 tokens, head_size a multiple of 16 up to
- * 128, or 256; blocks * block fits in 31 bits. k and v are 16-byte aligned. */
+ * 128, or 256; blocks * block fits in 31 bits. k and v are 16-byte aligned. A
+ * call takes at most RK_KV8_MAX_ROWS rows (and 2^31 - 1 rows times heads). */
+#define RK_KV8_MAX_ROWS (1 << 22)
 typedef struct {
     int8_t *k, *v;          /* [blocks][kv_heads][block][head_size], [blocks][kv_heads][head_size][block] */
     float *k_scale, *v_scale; /* [blocks][kv_heads] */

@@ -134,14 +134,15 @@ int64_t attn8_workspace(const rk_kv8 &c, int, int sms) {
 cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStream_t st) {
   const int hs = a.c.head_size, G = a.heads / a.c.kv_heads;
   // Two tiles of 8 rows a warp halve the conversions a row costs, once the
-  // requests have more than 8 rows a kv head on average. float16 takes two
-  // terms below that, where they cost little beside the loads: one term's
-  // rounding is not far below the output's own.
+  // requests have more than 16 rows a kv head on average (16 requests over 2048
+  // tokens, G = 4: 40.2 us with them and 37.1 without at 16 rows, 52.6 and 60.0
+  // at 32). float16 takes two terms up to 8 rows, where they cost little beside
+  // the loads: one term's rounding is not far below the output's own.
   const bool rows = (int64_t)a.tokens * G > 8LL * a.n;
   const int terms = type == RK_ACT_F32 || (type == RK_ACT_F16 && !rows) ? 2 : 1;
-  const int nt = terms == 1 && rows && hs <= 128 ? 2 : 1;
+  const int nt = terms == 1 && (int64_t)a.tokens * G > 16LL * a.n && hs <= 128 ? 2 : 1;
   A8Grid g{sms * a8_ctas(hs, terms, nt), 4, a.c.block == 16 ? 4 : a.c.block == 32 ? 5 : a.c.block == 64 ? 6 : 7,
-           a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0, G > 1 ? 0xffffffffu / G + 1 : 0};
+           a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0, G > 1 && (int64_t)a.tokens * G * G < 1LL << 32 ? 0xffffffffu / G + 1 : 0};
   // Short tables: a unit's tiles are few for one CTA, and without units cut in
   // two there is nothing to join.
   const bool whole = (int64_t)a.max_blocks * a.c.block <= RK_KV8_NO_WORKSPACE;

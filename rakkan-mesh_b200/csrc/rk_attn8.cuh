@@ -65,7 +65,16 @@ struct A8Shape {
   static constexpr int KS = HS / 16;        // 16-long steps over a head
   static constexpr int PITCH = HS + 4;      // floats between rows of a merge buffer
   static constexpr int KBYTES = kA8Tile * HS, TILE = 2 * KBYTES;  // of a tile: keys [32][HS], values [HS][32]
-  static constexpr int RING = 4 * 2 * TILE; // of a CTA: two tiles a warp
+};
+// Shared memory of a CTA: the rings of two tiles (of one warp, or of at least
+// two that share a tile where a warp has two tiles of rows), then those warps'
+// queries; between two units, the merge buffers.
+template <int HS, int NT, int DIGITS>
+struct A8Smem {
+  static constexpr int RINGS = kA8Warps / NT * 2 * A8Shape<HS>::TILE;
+  static constexpr int QUERY = NT > 1 ? NT * DIGITS * (HS / 16 + HS / 16 % 2) * 128 : 0;  // of a warp
+  static constexpr int MERGE = kA8Warps * 8 * NT * (A8Shape<HS>::PITCH + 4) * 4;
+  static constexpr int ALL = RINGS + kA8Warps * QUERY > MERGE ? RINGS + kA8Warps * QUERY : MERGE;
 };
 // CTAs of an SM, by their registers and shared memory (TERMS float16 terms,
 // NT tiles of 8 rows a warp).
@@ -89,7 +98,7 @@ struct A8Grid {
   int min_tiles;  // fewest tiles worth a CTA; 0: a CTA takes whole units
   int log_block;  // of the page's tokens
   bool vec_q;     // rows of q lie on 16-byte boundaries
-  uint32_t by_group;  // ceil(2^32 / G), for quotients (0: G is 1)
+  uint32_t by_group;  // ceil(2^32 / G), for quotients below 2^32 / G (0: divide)
 };
 
 RK_DEV uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
@@ -262,7 +271,7 @@ RK_DEV A8Req a8_req(const Attn8Args &a, int lb, int i) {
   q.tiles = max(1, q.len / TT + (q.len % TT != 0) - q.tile0);
   const long long rows = (long long)q.nq * (a.heads / a.c.kv_heads);
   const int rts = (int)((rows + R - 1) / R);
-  q.rw = rts >= 4 ? 4 : rts >= 2 ? 2 : 1;
+  q.rw = rts >= 4 ? 4 : rts >= 2 || R > 8 ? 2 : 1;
   q.units = (rts + q.rw - 1) / q.rw;
   return q;
 }
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   using Shape = A8Shape<HS>;
   constexpr int TT = kA8Tile, KS = Shape::KS, PITCH = Shape::PITCH, R = 8 * NT, ND = HS / 8;
   constexpr int DIGITS = TERMS + 1;  // signed bytes of a query
-  static_assert(kA8Warps * R * (PITCH + 4) * 4 <= Shape::RING, "the merge buffers fit the rings");
+  using Smem = A8Smem<HS, NT, DIGITS>;
   extern __shared__ __align__(128) char sm[];
   // The rings; between two units, the merge buffers [warps][R][PITCH] and [warps][R][4].
   float *s_o = reinterpret_cast<float *>(sm), *s_st = s_o + kA8Warps * R * PITCH;
@@ -281,7 +290,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   __shared__ int s_req;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   const int G = a.heads / a.c.kv_heads, H = a.c.kv_heads, lb = grid.log_block;
-  const auto token_of = [&](int row) { return grid.by_group ? (int)__umulhi(row, grid.by_group) : row; };
+  const auto token_of = [&](int row) { return grid.by_group ? (int)__umulhi(row, grid.by_group) : row / G; };
   griddep_trigger();
 
   // The run of tiles (or of whole units) of this CTA: a scan over the
@@ -337,7 +346,8 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       q = a8_req<HS, R>(a, lb, ++req);
     }
     const int step = length_of(q);
-    const int u = (uint32_t)(at - base) / (uint32_t)step;
+    const long long in = at - base;
+    const int u = in >> 32 ? (int)(in / step) : (int)((uint32_t)in / (uint32_t)step);
     const int head = u / q.units, rg = u % q.units;
     const long long u0 = base + (long long)u * step, u1 = u0 + step;
     const int t0 = by_unit ? 0 : max(0, (int)(at - u0) - kA8Begin);
@@ -458,8 +468,9 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     copy_tile(t, 0);
     look_up(t + tw);
 
-    // Query fragments.
-    uint32_t qb[NT][DIGITS][KS + KS % 2];
+    // Query fragments: in registers, or (two tiles of rows) in shared memory.
+    uint32_t qb[NT > 1 ? 1 : NT][DIGITS][KS + KS % 2];
+    uint2 *const q_mine = reinterpret_cast<uint2 *>(sm + Smem::RINGS + warp * Smem::QUERY) + lane;
     float f[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -496,19 +507,25 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
           w[b] = DIGITS == 2 ? f2u(fmaf(v[s][b], up, 12582912.0f)) : (uint32_t)__float2int_rn(v[s][b] * up);
         // The lowest byte as a signed one; the rest is a multiple of 256: the
         // next byte of w + 128, and that of w + 128 + 128·256.
-        qb[n][DIGITS - 1][s] = pack_bytes(w[0], w[1], w[2], w[3]);
+        qb[NT > 1 ? 0 : n][DIGITS - 1][s] = pack_bytes(w[0], w[1], w[2], w[3]);
 #pragma unroll
         for (int b = 0; b < 4; b++) w[b] += 0x80u;
-        qb[n][DIGITS - 2][s] = prmt(prmt(w[0], w[1], 0x0051), prmt(w[2], w[3], 0x0051), 0x5410);
+        qb[NT > 1 ? 0 : n][DIGITS - 2][s] = prmt(prmt(w[0], w[1], 0x0051), prmt(w[2], w[3], 0x0051), 0x5410);
         if constexpr (DIGITS == 3) {
 #pragma unroll
           for (int b = 0; b < 4; b++) w[b] += 0x8000u;
-          qb[n][0][s] = prmt(prmt(w[0], w[1], 0x0062), prmt(w[2], w[3], 0x0062), 0x5410);
+          qb[NT > 1 ? 0 : n][0][s] = prmt(prmt(w[0], w[1], 0x0062), prmt(w[2], w[3], 0x0062), 0x5410);
         }
       }
       if (KS % 2)
 #pragma unroll
-        for (int x = 0; x < DIGITS; x++) qb[n][x][KS] = 0;
+        for (int x = 0; x < DIGITS; x++) qb[NT > 1 ? 0 : n][x][KS] = 0;
+      if constexpr (NT > 1)
+#pragma unroll
+        for (int x = 0; x < DIGITS; x++)
+#pragma unroll
+          for (int s = 0; s < KS; s += 2)
+            q_mine[((n * DIGITS + x) * ((KS + 1) / 2) + s / 2) * 32] = make_uint2(qb[0][x][s], qb[0][x][s + 1]);
     }
 
     float o[NT][ND / 2][4], m[NT][2], M[NT][2], l[NT][2];
@@ -549,7 +566,12 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int x = 0; x < DIGITS; x++) mma16832(si[x][n], ka, qb[n][x][k], qb[n][x][k + 1]);
+            for (int x = 0; x < DIGITS; x++) {
+              uint2 b;
+              if constexpr (NT > 1) b = q_mine[((n * DIGITS + x) * ((KS + 1) / 2) + k / 2) * 32];
+              else b = make_uint2(qb[n][x][k], qb[n][x][k + 1]);
+              mma16832(si[x][n], ka, b.x, b.y);
+            }
         }
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -780,10 +802,10 @@ struct A8 {
   struct Init {
     template <int HS>
     cudaError_t operator()() const {
-      cudaError_t e = cudaFuncSetAttribute(k_attn8<HS, TERMS, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8Shape<HS>::RING);
+      cudaError_t e = cudaFuncSetAttribute(k_attn8<HS, TERMS, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8Smem<HS, 1, TERMS + 1>::ALL);
       if constexpr (two_tiles<HS>())
         if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(k_attn8<HS, TERMS, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8Shape<HS>::RING);
+          e = cudaFuncSetAttribute(k_attn8<HS, TERMS, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, A8Smem<HS, 2, TERMS + 1>::ALL);
       return e;
     }
   };
@@ -795,8 +817,8 @@ struct A8 {
     template <int HS>
     cudaError_t operator()() const {
       if constexpr (two_tiles<HS>())
-        if (nt == 2) return launch_k(k_attn8<HS, TERMS, 2>, g.ctas, kA8Threads, A8Shape<HS>::RING, st, a, type, g);
-      return launch_k(k_attn8<HS, TERMS, 1>, g.ctas, kA8Threads, A8Shape<HS>::RING, st, a, type, g);
+        if (nt == 2) return launch_k(k_attn8<HS, TERMS, 2>, g.ctas, kA8Threads, (A8Smem<HS, 2, TERMS + 1>::ALL), st, a, type, g);
+      return launch_k(k_attn8<HS, TERMS, 1>, g.ctas, kA8Threads, (A8Smem<HS, 1, TERMS + 1>::ALL), st, a, type, g);
     }
   };
   static cudaError_t init() {

@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(kTabThreads) k_page_tables(TablesArgs a) {
 }
 
 cudaError_t launch_page_tables(const TablesArgs &a, int sms, cudaStream_t st) {
-  const int want = (a.max_tokens + kTabThreads - 1) / kTabThreads;
-  const int grid = want < 1 ? 1 : want > 2 * sms ? 2 * sms : want;
+  const long long want = ((long long)a.max_tokens + kTabThreads - 1) / kTabThreads;
+  const int grid = want < 1 ? 1 : want > 2 * sms ? 2 * sms : (int)want;
   return launch_k(k_page_tables, grid, kTabThreads, sizeof(int) * (2 * (size_t)a.n + 1), st, a);
 }
 

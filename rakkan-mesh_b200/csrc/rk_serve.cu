@@ -114,7 +114,7 @@ extern "C" int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens
   if (!d) return bad("kv8 append: null argument");
   if (int rc = check_cache(c)) return rc;
   if (!act_type(type)) return bad("kv8 append: unknown type %d", type);
-  if (tokens < 0) return bad("kv8 append: %d tokens", tokens);
+  if (tokens < 0 || tokens > RK_KV8_MAX_ROWS) return bad("kv8 append: %d rows (at most %d)", tokens, RK_KV8_MAX_ROWS);
   if (tokens == 0) return RK_OK;
   if (!k || !v || !slots) return bad("kv8 append: null argument");
   const int64_t width = (int64_t)c->kv_heads * c->head_size;
@@ -147,6 +147,8 @@ extern "C" int rk_kv8_attention(rk_device *d, const rk_kv8 *c, int type, int n, 
   if (heads < 1 || heads % c->kv_heads) return bad("kv8 attention: %d heads over %d kv heads", heads, c->kv_heads);
   if (n < 0 || n > RK_MAX_REQUESTS) return bad("kv8 attention: %d requests (at most %d)", n, RK_MAX_REQUESTS);
   if (tokens < 0 || max_blocks < 0 || window < 0) return bad("kv8 attention: a negative size");
+  if (tokens > RK_KV8_MAX_ROWS || (int64_t)tokens * heads > 0x7fffffff)
+    return bad("kv8 attention: %d rows of %d heads (at most %d rows, 2^31 - 1 in all)", tokens, heads, RK_KV8_MAX_ROWS);
   if (!q_start && tokens < n) return bad("kv8 attention: %d rows for %d requests of one each", tokens, n);
   if (!(scale >= 0.0f) || scale > 3.0e38f) return bad("kv8 attention: scale %g", (double)scale);
   if (n == 0 || tokens == 0) return RK_OK;

@@ -55,7 +55,7 @@ def test_bad_caches_are_refused(wrong):
 
 @pytest.mark.parametrize("wrong", [dict(d=None), dict(type=3), dict(type=-1), dict(tokens=-1), dict(k=None), dict(v=None),
                                    dict(slots=None), dict(ks=127), dict(vs=0), dict(ks=-128), dict(k=P + 2),
-                                   dict(slots=P + 1), dict(type=rk.ACT_F16, v=P + 1)], ids=str)
+                                   dict(slots=P + 1), dict(type=rk.ACT_F16, v=P + 1), dict(tokens=(1 << 22) + 1)], ids=str)
 def test_append_refuses(wrong):
     refused(append(kv8(), **wrong), "kv8")
 
@@ -70,7 +70,8 @@ def test_append_of_nothing_is_nothing():
                                    dict(lens=None), dict(table=None), dict(out=None), dict(qs=255), dict(os=1),
                                    dict(width=-1), dict(window=-1), dict(scale=-1.0), dict(scale=float("nan")),
                                    dict(scale=float("inf")), dict(q=P + 1), dict(lens=P + 2), dict(start=P + 2),
-                                   dict(table=P + 3), dict(out=P + 1)], ids=str)
+                                   dict(table=P + 3), dict(out=P + 1), dict(tokens=(1 << 22) + 1),
+                                   dict(tokens=1 << 20, heads=1 << 12, qs=1 << 18, os=1 << 18)], ids=str)
 def test_attention_refuses(wrong):
     refused(attention(kv8(), **wrong), "kv8")
 
