@@ -131,6 +131,13 @@ RK_DEV void mma16832(int *c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same from sums of zero.
+RK_DEV void mma16832_first(int *c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+
 RK_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -153,6 +160,22 @@ RK_DEV uint32_t pack_rest(float a, float b, uint32_t p) {
   return pack_h2(a - __low2float(h), b - __high2float(h));
 }
 
+// Shared memory by 32-bit addresses.
+RK_DEV uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+RK_DEV uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+RK_DEV uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
 RK_DEV void copy16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -168,18 +191,18 @@ RK_DEV int key_swizzle(int row) { return HS % 128 == 0 ? (row & 1) << 6 : 0; }
 // A lane's words of one key row: word s is step s's four bytes. Whole 64-byte
 // stretches as 16 bytes a lane, then 32 as 8, then 16 as 4.
 template <int HS>
-RK_DEV void load_row(const char *row, int swizzle, int c, uint32_t *w) {
+RK_DEV void load_row(uint32_t row, int swizzle, int c, uint32_t *w) {
   constexpr int N64 = HS / 64, R = HS % 64;
 #pragma unroll
   for (int i = 0; i < N64; i++) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(row + ((64 * i) ^ swizzle) + 16 * c);
+    const uint4 v = lds128(row + (i % 2 ? (64 ^ swizzle) + 64 * (i - 1) : swizzle + 64 * i) + 16 * c);
     w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
   }
   if constexpr (R >= 32) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(row + 64 * N64 + 8 * c);
+    const uint2 v = lds64(row + 64 * N64 + 8 * c);
     w[4 * N64] = v.x, w[4 * N64 + 1] = v.y;
   }
-  if constexpr (R % 32 != 0) w[HS / 16 - 1] = *reinterpret_cast<const uint32_t *>(row + HS - 16 + 4 * c);
+  if constexpr (R % 32 != 0) w[HS / 16 - 1] = lds32(row + HS - 16 + 4 * c);
 }
 // A lane's values of a query row, in load_row's order: 16, 8 and 4
 // neighbours, as 16-byte pieces where the rows allow it.
@@ -471,6 +494,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     // Query fragments: in registers, or (two tiles of rows) in shared memory.
     uint32_t qb[NT > 1 ? 1 : NT][DIGITS][KS + KS % 2];
     uint2 *const q_mine = reinterpret_cast<uint2 *>(sm + Smem::RINGS + warp * Smem::QUERY) + lane;
+    const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(q_mine);
     float f[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -548,7 +572,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       const int tok0 = (q.tile0 + t) * TT;
       if (tok0 > high_max) continue;  // in reach of other warps' rows only
 
-      const char *kt = ring + it * Shape::TILE, *vt = kt + Shape::KBYTES;
+      const uint32_t kt = ring_at + it * Shape::TILE + (8 * (r >> 1) + (r & 1)) * HS, vt = ring_at + it * Shape::TILE + Shape::KBYTES + r * TT + 8 * c;
       float sc[2][NT][4];
 #pragma unroll
       for (int s = 0; s < 2; s++) {
@@ -556,10 +580,10 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         uint32_t kw[2][KS + KS % 2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          load_row<HS>(kt + (8 * (r >> 1) + 4 * s + 2 * j + (r & 1)) * HS, key_swizzle<HS>(r), c, kw[j]);
+          load_row<HS>(kt + (4 * s + 2 * j) * HS, key_swizzle<HS>(r), c, kw[j]);
           if (KS % 2) kw[j][KS] = 0;
         }
-        int si[DIGITS][NT][4] = {};
+        int si[DIGITS][NT][4];
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
           const uint32_t ka[4] = {kw[0][k], kw[1][k], kw[0][k + 1], kw[1][k + 1]};
@@ -568,9 +592,10 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
 #pragma unroll
             for (int x = 0; x < DIGITS; x++) {
               uint2 b;
-              if constexpr (NT > 1) b = q_mine[((n * DIGITS + x) * ((KS + 1) / 2) + k / 2) * 32];
+              if constexpr (NT > 1) b = lds64(q_at + ((n * DIGITS + x) * ((KS + 1) / 2) + k / 2) * 256);
               else b = make_uint2(qb[n][x][k], qb[n][x][k + 1]);
-              mma16832(si[x][n], ka, b.x, b.y);
+              if (k == 0) mma16832_first(si[x][n], ka, b.x, b.y);
+              else mma16832(si[x][n], ka, b.x, b.y);
             }
         }
 #pragma unroll
@@ -669,8 +694,8 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
 #pragma unroll
       for (int d = 0; d < ND / 2; d++) {
         // Tokens 8c .. 8c + 7 of two dimensions.
-        const uint2 v0 = *reinterpret_cast<const uint2 *>(vt + (16 * d + r) * TT + 8 * c);
-        const uint2 v1 = *reinterpret_cast<const uint2 *>(vt + (16 * d + 8 + r) * TT + 8 * c);
+        const uint2 v0 = lds64(vt + 16 * d * TT);
+        const uint2 v1 = lds64(vt + (16 * d + 8) * TT);
         // Float32 results: a tile's sums of their own, added outside. The
         // products' adder does not round, and over thousands of tokens that
         // shows (6.7e-6 of the result over 4600).
