@@ -37,9 +37,9 @@
 // rightly.
 //
 // Work. A unit is a request's kv head and up to four tiles of query rows; its
-// keys are cut into tiles of 32 tokens. The tiles of all units in a row are dealt out in equal runs, one to a CTA, so that lengths
-// need not be alike and one long request fills the GPU as well as many short
-// ones. Within a CTA the warps take different row tiles of the same tokens
+// keys are cut into tiles of 32 tokens. The tiles of all units in a row are dealt
+// out in runs of equal work, one to a CTA, so that lengths need not be alike
+// and one long request fills the GPU as well as many short ones. Within a CTA the warps take different row tiles of the same tokens
 // (their loads meet in L1) or, where there are fewer, different tokens. A unit
 // that crosses CTAs leaves its parts in the workspace, and a second kernel
 // joins them.
@@ -56,9 +56,10 @@ constexpr int kA8Warps = 4;
 constexpr int kA8Threads = 32 * kA8Warps;
 
 constexpr int kA8Tile = 32;  // tokens
-// What a unit's beginning and end cost a CTA, in tiles (about 5 us against 0.6
-// us a tile where memory bounds them; 12 measured best of 0 to 14): CTAs that begin a second unit get so
-// many tiles less.
+// What a unit's beginning and end cost a CTA, in tiles of one warp (about 5 us
+// against 0.6 us a tile where memory bounds them): a CTA that begins a second
+// unit gets so many fewer. 12 measured best for single tokens: 32 sequences of
+// 4096 tokens 47.0 us, 47.9 with 6 and 48.2 with 20; 8 x 64 rows 71.1, 72.2 and 69.5.
 constexpr int kA8Begin = 12;
 template <int HS>
 struct A8Shape {
@@ -95,7 +96,7 @@ __host__ __device__ inline int64_t a8_part_floats(int hs) { return 64LL * (hs + 
 
 struct A8Grid {
   int ctas;       // CTAs of the main kernel
-  int min_tiles;  // fewest tiles worth a CTA; 0: a CTA takes whole units
+  int min_tiles;  // fewest warp tiles worth a CTA; 0: a CTA takes whole units
   int log_block;  // of the page's tokens
   bool vec_q;     // rows of q lie on 16-byte boundaries
   uint32_t by_group;  // ceil(2^32 / G), for quotients below 2^32 / G (0: divide)
@@ -321,8 +322,9 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
   const bool by_unit = grid.min_tiles == 0;
   const int per_t = (a.n + kA8Threads - 1) / kA8Threads;
   const int i0 = min(a.n, tid * per_t), i1 = min(a.n, i0 + per_t);
-  // A unit counts kA8Begin tiles more than it has, in front of them.
-  auto length_of = [&](const A8Req &q) { return by_unit ? 1 : q.tiles + kA8Begin; };
+  // A unit's length: its tiles, each as many warp tiles as it has row tiles,
+  // and kA8Begin in front of them.
+  auto length_of = [&](const A8Req &q) { return by_unit ? 1 : q.tiles * q.rw + kA8Begin; };
   auto size_of = [&](const A8Req &q) { return (long long)H * q.units * length_of(q); };
   long long mine = 0;
   for (int i = i0; i < i1; i++) mine += size_of(a8_req<HS, R>(a, lb, i));
@@ -373,10 +375,16 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     const int u = in >> 32 ? (int)(in / step) : (int)((uint32_t)in / (uint32_t)step);
     const int head = u / q.units, rg = u % q.units;
     const long long u0 = base + (long long)u * step, u1 = u0 + step;
-    const int t0 = by_unit ? 0 : max(0, (int)(at - u0) - kA8Begin);
-    const int t1 = by_unit ? q.tiles : (int)(min(end, u1) - u0) - kA8Begin;
+    // A tile is that CTA's in whose run it begins.
+    const int rw = q.rw, log_rw = rw >> 1, tw = kA8Warps / rw;
+    const int t0 = by_unit ? 0 : (max(0, (int)(at - u0) - kA8Begin) + rw - 1) >> log_rw;
+    const int t1 = by_unit ? q.tiles : ((int)(min(end, u1) - u0) - kA8Begin + rw - 1) >> log_rw;
     if (t1 <= 0) break;  // the run ends before the unit's first tile
-    const int rw = q.rw, tw = kA8Warps / rw, wr = warp % rw, wt = warp / rw;
+    if (t0 >= q.tiles) {  // and begins behind the start of its last
+      at = u1;
+      continue;
+    }
+    const int wr = warp % rw, wt = warp / rw;
     const int row0 = (rg * rw + wr) * R;        // of the request's nq·G rows (token-major)
     const int all_rows = q.nq * G;
 
@@ -746,7 +754,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         }
       }
     __syncthreads();
-    const bool starts = t0 == 0, ends = u1 <= end;
+    const bool starts = t0 == 0, ends = t1 == q.tiles;
     float *part = parts + (2LL * blockIdx.x + (starts ? 1 : 0)) * a8_part_floats(HS);
     for (int row = warp; row < unit_rows; row += kA8Warps) {
       const int tile = row / R, rr = row % R;
@@ -787,7 +795,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     if (!starts && tid == 0) {  // the CTA's first unit, begun in another one
       A8Record rec;
       rec.first = (int)((u0 + kA8Begin) / per);
-      rec.last = (int)((u1 - 1) / per);
+      rec.last = (int)((u1 - rw) / per);
       rec.req = req;
       rec.head = head;
       rec.row0 = unit_row0;
