@@ -39,10 +39,10 @@
 // Work. A unit is a request's kv head and up to four tiles of query rows; its
 // keys are cut into tiles of 32 tokens. The tiles of all units in a row are dealt
 // out in runs of equal work, one to a CTA, so that lengths need not be alike
-// and one long request fills the GPU as well as many short ones. Within a CTA the warps take different row tiles of the same tokens
-// (their loads meet in L1) or, where there are fewer, different tokens. A unit
-// that crosses CTAs leaves its parts in the workspace, and a second kernel
-// joins them.
+// and one long request fills the GPU as well as many short ones. Within a CTA
+// the warps take different row tiles of the same tokens, which they copy
+// together, or, where there are fewer, different tokens. A unit that crosses
+// CTAs leaves its parts in the workspace, and a second kernel joins them.
 #pragma once
 #include <type_traits>
 
@@ -437,7 +437,6 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     const int8_t *v_lane = a.c.v + (((int64_t)head * HS + (lane >> 1)) << lb) + 16 * (lane & 1);
     const int key_piece = (16 * lane) ^ key_swizzle<HS>(16 * lane / HS);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-    const uint32_t my_pieces = (rw == 4 ? 0x11111111u : 0x55555555u) << wr;
     int page[2];  // -1: outside the cache
     float ks = 0.0f, vs = 0.0f;  // scales of the next tile, of the page of this lane's tokens
     bool live = false;
@@ -456,15 +455,21 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         if (wrong) atomicExch(a.err, DEV_ERR_RANGE);
       }
     };
-    // The copies of a tile: piece i of a lane, by constant offsets.
+    // The copies of a tile: piece i of a lane, by constant offsets where the
+    // warp copies all, every rw-th by a loop.
     auto copy_pieces = [&](auto log, uint32_t dst, const int8_t *k0, const int8_t *k1, const int8_t *v0) {
       constexpr int LB = decltype(log)::value;
-#pragma unroll
-      for (int i = 0; i < KS; i++) {
-        if (rw > 1 && !(my_pieces >> i & 1)) continue;
+      auto copy_piece = [&](int i) {
         const int8_t *k = LB > 4 || (KS % 2 ? 32 * i + lane < HS : 2 * i < KS) ? k0 : k1;
         copy16(dst + key_piece + 512 * i, k + 512 * i);
         copy16(dst + Shape::KBYTES + 16 * lane + 512 * i, v0 + (16 << LB) * i);
+      };
+      if (rw == 1) {
+#pragma unroll
+        for (int i = 0; i < KS; i++) copy_piece(i);
+      } else {
+#pragma unroll 1
+        for (int i = wr; i < KS; i += rw) copy_piece(i);
       }
     };
     auto copy_tile = [&](int t, int stage) {  // page[] is the tile's
