@@ -6,28 +6,31 @@
 // The cache is read once for the query heads of a kv head. At one token a
 // request that read bounds the call (one byte a value, 4·G flop for it with
 // G query heads a kv head), and CUDA cores cannot keep up with it from G = 4
-// on; so both products run on mma.m16n8k16 with the integers as float16
-// (exact), and no shared memory lies between a load and its product: each
-// warp streams its own tiles from global memory into the registers that the
-// products read.
+// on; so both products run on the tensor cores, the scores on the bytes as they
+// are, the weighted values with the bytes as float16 (exact). Each warp streams
+// its own tiles through two slots of shared memory (cp.async), one under way
+// while it works on the other: tiles loaded into registers instead took 78.6
+// us for one token of 32 sequences of up to 4096 tokens (97,000 in all, 8 kv
+// heads of 128, G = 4), which takes 44.2 now: 4.5 TB/s. With 16384 tokens each it is 5.9.
+// With many rows a request the instructions around the products bound it, some
+// 1000 for 16 rows by 32 tokens: 512 rows over 8192 tokens 391 us, 170 TFLOP/s.
 //
 // Fragments. Keys and transposed values are the 16-row operand, queries and
 // weights the 8-column one: a tile of 8 query rows then fills the columns,
 // and half as many products and registers do as with queries in the rows
-// (91 us that way). A 16-long step of a product may
-// take its terms in any order as long as both operands agree. Lane
-// (r, c) = (lane / 4, lane % 4) holds terms {2c, 2c+1, 2c+8, 2c+9} of a step;
-// they are given to four neighbouring bytes, so that a lane's bytes of
-// several steps are one 16-, 8- or 4-byte load: of a key row, dimensions; of a
-// transposed value row, tokens. (A step of bytes is 32 long: two such groups.) The scores come out as (token, query); a
-// transposing move of 8x8 registers makes them the second product's column
-// operand, which fixes the token of each key row.
+// (91 us that way, with tiles in registers). A step of a product may
+// take its terms in any order as long as both operands agree. So of a step of
+// two 16-long halves lane (r, c) = (lane / 4, lane % 4) is given four neighbouring
+// bytes of each, and its bytes of several steps are one 16-, 8- or 4-byte
+// load: of a key row, dimensions; of a transposed value row, tokens. The scores
+// come out as (token, query); a transposing move of 8x8 registers makes them
+// the second product's column operand, which fixes the token of each key row.
 //
 // Precision. The scores' product is mma.m16n8k32 on signed bytes: the keys
 // as they are, a row of queries as integers of two signed bytes (16-bit types,
 // the row's largest at 32639: off by at most 2^-16 of it) or three (float32,
 // 2^-24), each its own exact product, joined in float32. (float16 products
-// would want the keys converted, 160 of some 900 instructions a tile.) The
+// would want the keys converted: 58.3 us in place of 48.9 at the time.) The
 // softmax weights are float16, one term for 16-bit types (2^-12 of itself:
 // an eighth of bfloat16's own rounding of the result, and half of float16's
 // on average over tokens) and two for float32 (22 bits), with the value scale
@@ -58,8 +61,9 @@ constexpr int kA8Threads = 32 * kA8Warps;
 constexpr int kA8Tile = 32;  // tokens
 // What a unit's beginning and end cost a CTA, in tiles of one warp (about 5 us
 // against 0.6 us a tile where memory bounds them): a CTA that begins a second
-// unit gets so many fewer. 12 measured best for single tokens: 32 sequences of
-// 4096 tokens 47.0 us, 47.9 with 6 and 48.2 with 20; 8 x 64 rows 71.1, 72.2 and 69.5.
+// unit gets so many fewer. 12 measured best for single tokens: of 6, 12 and 20
+// one token of the 32 sequences took 47.9, 47.0 and 48.2 us, and 8 x 64 rows
+// over up to 2048 tokens 72.2, 71.1 and 69.5.
 constexpr int kA8Begin = 12;
 template <int HS>
 struct A8Shape {

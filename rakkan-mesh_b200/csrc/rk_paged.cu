@@ -15,7 +15,8 @@ namespace rk {
 // of the step. A step is a few kilobytes, so the call is all latency: one
 // launch, in which every CTA makes both sums for itself from L2 (8 bytes a
 // request) instead of waiting for another CTA's, and then writes its share
-// of the rows, each thread finding its row's request by bisection.
+// of the rows, each thread finding its row's request by bisection. A step of
+// 1024 requests of up to 96 new tokens takes 5.6 us, one of one request 3.6.
 constexpr int kTabThreads = 512;
 
 RK_DEV long long warp_scan(long long v, int lane) {
@@ -150,8 +151,9 @@ cudaError_t launch_page_tables(const TablesArgs &a, int sms, cudaStream_t st) {
 // then scales, rounds and stores. The bytes of the rows and of the cache bound
 // the call. A run of up to 8192 values (a page of 64 tokens at head size 128) is
 // loaded once, into registers; longer ones and rows off 16-byte boundaries are
-// read twice, the second time from L1 or L2 (every run so: 32.5 us for the
-// prompts of 16 sequences, 8 heads of 128). Values are stored transposed: the
+// read twice, the second time from L1 or L2. The prompts of 16 sequences (8470
+// tokens, 8 heads of 128, bfloat16) take 21.5 us, 2.4 TB/s, and 32.5 with every
+// run read twice; what is left is each run's chain of load, maximum, store. Values are stored transposed: the
 // rounded bytes go through shared memory, from which 4 dimensions of 4 tokens
 // become 4 words, with the tokens in the fast lanes, so that a page row's words
 // are stored side by side. A CTA looks for the runs that begin in its `chunk`

@@ -31,6 +31,9 @@
 // ten column pairs a warp, and the last wave of CTAs left SMs idle.) The
 // float32 sums of a tile's shares meet in shared memory, in order, while the
 // warps are at the next tile.
+// 28672x4096 takes 14.4 us by one vector (4.3 TB/s; some 4 us are the launch,
+// the vectors and the last tile), 128256x4096 44.4 us (6.1 TB/s, 0.93 of a plain
+// copy's rate), 4096x14336 by 16 vectors in groups of 32 15.8 us.
 #include "rk_act.cuh"
 #include "rk_serve.cuh"
 
