@@ -117,10 +117,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int
     for (int j = 0; j < J; j++) {
       const int d = 4 * lane + 128 * j;
       if (d >= hs) break;
-      o_store(a.out, type, oi + d, v[j].x * scale);
-      o_store(a.out, type, oi + d + 1, v[j].y * scale);
-      o_store(a.out, type, oi + d + 2, v[j].z * scale);
-      o_store(a.out, type, oi + d + 3, v[j].w * scale);
+      o_store4(a.out, type, oi + d, make_float4(v[j].x * scale, v[j].y * scale, v[j].z * scale, v[j].w * scale), grid.vec_out);
     }
   }
 }
@@ -142,7 +139,9 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   const int terms = type == RK_ACT_F32 || (type == RK_ACT_F16 && !rows) ? 2 : 1;
   const int nt = terms == 1 && (int64_t)a.tokens * G > 16LL * a.n && hs <= 128 ? 2 : 1;
   A8Grid g{sms * a8_ctas(hs, terms, nt), 4, a.c.block == 16 ? 4 : a.c.block == 32 ? 5 : a.c.block == 64 ? 6 : 7,
-           a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0, G > 1 && (int64_t)a.tokens * G * G < 1LL << 32 ? 0xffffffffu / G + 1 : 0};
+           a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0,
+           a.out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & (type == RK_ACT_F32 ? 15 : 7)) == 0,
+           G > 1 && (int64_t)a.tokens * G * G < 1LL << 32 ? 0xffffffffu / G + 1 : 0};
   // Short tables: a unit's tiles are few for one CTA, and without units cut in
   // two there is nothing to join.
   const bool whole = (int64_t)a.max_blocks * a.c.block <= RK_KV8_NO_WORKSPACE;

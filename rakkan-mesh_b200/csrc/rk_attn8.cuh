@@ -103,6 +103,7 @@ struct A8Grid {
   int min_tiles;  // fewest warp tiles worth a CTA; 0: a CTA takes whole units
   int log_block;  // of the page's tokens
   bool vec_q;     // rows of q lie on 16-byte boundaries
+  bool vec_out;   // four neighbours of out on a boundary of their size
   uint32_t by_group;  // ceil(2^32 / G), for quotients below 2^32 / G (0: divide)
 };
 
@@ -268,6 +269,19 @@ RK_DEV void o_store(void *o, int type, int64_t i, float v) {
   if (type == RK_ACT_F32) static_cast<float *>(o)[i] = v;
   else if (type == RK_ACT_F16) static_cast<__half *>(o)[i] = __float2half_rn(v);
   else static_cast<__nv_bfloat16 *>(o)[i] = __float2bfloat16_rn(v);
+}
+// Four neighbours; vec: on a boundary of their size.
+RK_DEV void o_store4(void *o, int type, int64_t i, float4 v, bool vec) {
+  if (!vec) {
+    o_store(o, type, i, v.x), o_store(o, type, i + 1, v.y);
+    o_store(o, type, i + 2, v.z), o_store(o, type, i + 3, v.w);
+  } else if (type == RK_ACT_F32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(o) + i) = v;
+  } else {
+    const uint2 w = type == RK_ACT_F16 ? make_uint2(act_pack<__half>(v.x, v.y), act_pack<__half>(v.z, v.w))
+                                       : make_uint2(act_pack<__nv_bfloat16>(v.x, v.y), act_pack<__nv_bfloat16>(v.z, v.w));
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + i) = w;
+  }
 }
 
 // A request's share of the work.
@@ -784,15 +798,17 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       const int qrow = unit_row0 + row, tq = token_of(qrow);
       const float scale = ll == 0.0f ? 0.0f : ex2(Msafe - 14.0f - msafe) / ll;
       const int64_t oi = (q.q0 + tq) * a.out_stride + (head * G + qrow - tq * G) * HS;
-      for (int d = lane; d < HS; d += 32) {
-        float v = 0.0f;
+      for (int d = 4 * lane; d < HS; d += 128) {
+        float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < kA8Warps; w++) {
           if (w >= tw) break;
-          v = fmaf(s_o[((tile + w * rw) * R + rr) * PITCH + d], g[w], v);
+          const float4 x = *reinterpret_cast<const float4 *>(s_o + ((tile + w * rw) * R + rr) * PITCH + d);
+          v.x = fmaf(x.x, g[w], v.x), v.y = fmaf(x.y, g[w], v.y);
+          v.z = fmaf(x.z, g[w], v.z), v.w = fmaf(x.w, g[w], v.w);
         }
-        if (starts && ends) o_store(a.out, type, oi + d, v * scale);
-        else part[row * HS + d] = v;
+        if (starts && ends) o_store4(a.out, type, oi + d, make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale), grid.vec_out);
+        else *reinterpret_cast<float4 *>(part + row * HS + d) = v;
       }
       if (!(starts && ends) && lane == 0) {
         float *s = part + 64 * HS + 4 * row;

@@ -396,6 +396,26 @@ def test_attention_window(torch, dev, window, block):
     attention_case(torch, dev, window, 4, 2, 64, block, [30, 40, 300], [30, 2, 64], "bf16", window=window)
 
 
+@pytest.mark.parametrize("new", [None, [20, 7]], ids=str)
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_attention_rows_off_boundaries(torch, dev, t, new):
+    """Rows of q and out one value off any boundary, an odd stride apart: the same bits."""
+    rng = np.random.default_rng(14)
+    kv, _ = cache(torch, dev, rng, 60, 2, 32, 80)
+    starts = None if new is None else ints(torch, [0, 20, 27])
+    rows = 2 if new is None else 27
+    q = torch.from_numpy(rng.normal(0, 1, (rows, 6, 80))).cuda().to(dtype(torch, t))
+    table = torch.arange(60, dtype=torch.int32, device="cuda").view(2, 30)
+    lens = ints(torch, [900, 33])
+    want = kv.attention(q, table, lens, q_start=starts)
+    wide = torch.full((2, rows, 483), 77.0, dtype=q.dtype, device="cuda")
+    q2, out = (wide[i, :, 1:481].unflatten(1, (6, 80)) for i in range(2))
+    q2.copy_(q)
+    kv.attention(q2, table, lens, q_start=starts, out=out)
+    assert bool(torch.equal(out, want))
+    assert bool((wide[1, :, 0] == 77).all()) and bool((wide[1, :, 481:] == 77).all())
+
+
 def test_attention_rows_without_a_token(torch, dev):
     """Lengths of zero and below, and queries in front of the first token, give zeros."""
     attention_case(torch, dev, 1, 4, 2, 32, 16, [0, 5, -4, 0], [2, 9, 3, 0], "f32")
