@@ -779,42 +779,48 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     __syncthreads();
     const bool starts = t0 == 0, ends = t1 == q.tiles;
     float *part = parts + (2LL * blockIdx.x + (starts ? 1 : 0)) * a8_part_floats(HS);
-    for (int row = warp; row < unit_rows; row += kA8Warps) {
-      const int tile = row / R, rr = row % R;
-      float mm = -INFINITY, MM = -INFINITY;
+    // Rows warp, warp + 4, ..., at most 16: lane i makes the i-th's factors.
+    const int my_row = warp + kA8Warps * lane;
+    float my_g[kA8Warps] = {}, my_scale = 0.0f;
+    int64_t my_at = 0;
+    if (my_row < unit_rows) {
+      const float4 *s = reinterpret_cast<const float4 *>(s_st) + my_row;
+      float mm = -INFINITY, MM = -INFINITY, ll = 0.0f;
       for (int w = 0; w < tw; w++) {
-        mm = fmaxf(mm, s_st[((tile + w * rw) * R + rr) * 4]);
-        MM = fmaxf(MM, s_st[((tile + w * rw) * R + rr) * 4 + 1]);
+        mm = fmaxf(mm, s[w * rw * R].x);
+        MM = fmaxf(MM, s[w * rw * R].y);
       }
       const float msafe = mm == -INFINITY ? 0.0f : mm, Msafe = MM == -INFINITY ? 0.0f : MM;
-      float ll = 0.0f, g[kA8Warps];
 #pragma unroll
       for (int w = 0; w < kA8Warps; w++) {
         if (w >= tw) break;
-        const float *s = s_st + ((tile + w * rw) * R + rr) * 4;
-        ll += s[2] * ex2(s[0] - msafe);
-        g[w] = ex2(s[1] - Msafe);
+        const float4 x = s[w * rw * R];
+        ll += x.z * ex2(x.x - msafe);
+        my_g[w] = ex2(x.y - Msafe);
       }
-      const int qrow = unit_row0 + row, tq = token_of(qrow);
-      const float scale = ll == 0.0f ? 0.0f : ex2(Msafe - 14.0f - msafe) / ll;
-      const int64_t oi = (q.q0 + tq) * a.out_stride + (head * G + qrow - tq * G) * HS;
+      my_scale = ll == 0.0f ? 0.0f : ex2(Msafe - 14.0f - msafe) / ll;
+      const int qrow = unit_row0 + my_row, tq = token_of(qrow);
+      my_at = (q.q0 + tq) * a.out_stride + (head * G + qrow - tq * G) * HS;
+      if (!(starts && ends)) reinterpret_cast<float4 *>(part + 64 * HS)[my_row] = make_float4(mm, MM, ll, 0.0f);
+    }
+    for (int i = 0, row = warp; row < unit_rows; i++, row += kA8Warps) {
+      const int64_t oi = __shfl_sync(0xffffffffu, my_at, i);
+      const float scale = __shfl_sync(0xffffffffu, my_scale, i);
+      float g[kA8Warps];
+#pragma unroll
+      for (int w = 0; w < kA8Warps; w++) g[w] = __shfl_sync(0xffffffffu, my_g[w], i);
+      const float *so_row = s_o + row * PITCH;
       for (int d = 4 * lane; d < HS; d += 128) {
         float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < kA8Warps; w++) {
           if (w >= tw) break;
-          const float4 x = *reinterpret_cast<const float4 *>(s_o + ((tile + w * rw) * R + rr) * PITCH + d);
+          const float4 x = *reinterpret_cast<const float4 *>(so_row + w * rw * R * PITCH + d);
           v.x = fmaf(x.x, g[w], v.x), v.y = fmaf(x.y, g[w], v.y);
           v.z = fmaf(x.z, g[w], v.z), v.w = fmaf(x.w, g[w], v.w);
         }
         if (starts && ends) o_store4(a.out, type, oi + d, make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale), grid.vec_out);
         else *reinterpret_cast<float4 *>(part + row * HS + d) = v;
-      }
-      if (!(starts && ends) && lane == 0) {
-        float *s = part + 64 * HS + 4 * row;
-        s[0] = mm;
-        s[1] = MM;
-        s[2] = ll;
       }
     }
     if (!starts && tid == 0) {  // the CTA's first unit, begun in another one
