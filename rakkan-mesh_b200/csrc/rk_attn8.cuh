@@ -210,37 +210,36 @@ RK_DEV void load_row(uint32_t row, int swizzle, int c, uint32_t *w) {
   }
   if constexpr (R % 32 != 0) w[HS / 16 - 1] = lds32(row + HS - 16 + 4 * c);
 }
-// A lane's values of a query row, in load_row's order: 16, 8 and 4
-// neighbours, as 16-byte pieces where the rows allow it.
+// A lane's values of a query row as they lie in memory, in load_row's order:
+// 16, 8 and 4 neighbours, as 16-byte pieces where the rows allow it. float32
+// fills the four words of a word's values, 16-bit types the first two.
 template <int N>
-RK_DEV void load_values(const float *q, bool vec, float *v) {
-  if (vec) {
+RK_DEV void load_bits(const float *q, bool vec, uint32_t (*w)[4]) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 x = __ldg(reinterpret_cast<const float4 *>(q + i));
-      v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+  for (int i = 0; i < N / 4; i++) {
+    if (vec) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4 *>(q) + i);
+      w[i][0] = x.x, w[i][1] = x.y, w[i][2] = x.z, w[i][3] = x.w;
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; b++) w[i][b] = f2u(__ldg(q + 4 * i + b));
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = __ldg(q + i);
   }
 }
-template <bool BF16>
-RK_DEV float half_value(uint32_t bits16) {
-  return BF16 ? u2f(bits16 << 16) : __half2float(__ushort_as_half((unsigned short)bits16));
-}
-template <int N, bool BF16>
-RK_DEV void load_values16(const uint16_t *q, bool vec, float *v) {
-  if (vec) {  // 8-byte pieces: N = 4 has no more
+template <int N, int W>
+RK_DEV void load_bits(const uint16_t *q, bool vec, uint32_t (*w)[W]) {
+  if (!vec) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const uint2 x = __ldg(reinterpret_cast<const uint2 *>(q + i));
-      v[i] = half_value<BF16>(x.x & 0xffff), v[i + 1] = half_value<BF16>(x.x >> 16);
-      v[i + 2] = half_value<BF16>(x.y & 0xffff), v[i + 3] = half_value<BF16>(x.y >> 16);
+    for (int i = 0; i < N; i += 2) w[i / 4][i / 2 % 2] = __ldg(q + i) | (uint32_t)__ldg(q + i + 1) << 16;
+  } else if constexpr (N >= 8) {
+#pragma unroll
+    for (int i = 0; i < N / 8; i++) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4 *>(q) + i);
+      w[2 * i][0] = x.x, w[2 * i][1] = x.y, w[2 * i + 1][0] = x.z, w[2 * i + 1][1] = x.w;
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = half_value<BF16>(__ldg(q + i));
+    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(q));
+    w[0][0] = x.x, w[0][1] = x.y;
   }
 }
 template <int HS, class F>
@@ -251,18 +250,14 @@ RK_DEV void by_stretch(int c, F f) {  // f<N>(first dimension, first word)
   if constexpr (R >= 32) f.template operator()<8>(64 * N64 + 8 * c, 4 * N64);
   if constexpr (R % 32 != 0) f.template operator()<4>(HS - 16 + 4 * c, HS / 16 - 1);
 }
-template <int HS>
+template <class T, int W>
 struct LoadQuery {
-  const void *q;
-  int64_t at;
-  int type;
+  const T *q;
   bool vec;
-  float *v;
+  uint32_t (*bits)[W];
   template <int N>
   RK_DEV void operator()(int d, int word) const {
-    if (type == RK_ACT_F32) load_values<N>(static_cast<const float *>(q) + at + d, vec, v + 4 * word);
-    else if (type == RK_ACT_F16) load_values16<N, false>(static_cast<const uint16_t *>(q) + at + d, vec, v + 4 * word);
-    else load_values16<N, true>(static_cast<const uint16_t *>(q) + at + d, vec, v + 4 * word);
+    load_bits<N>(q + d, vec, bits + word);
   }
 };
 RK_DEV void o_store(void *o, int type, int64_t i, float v) {
@@ -516,6 +511,25 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       ks = live ? __ldg(a.c.k_scale + ph) : 0.0f;
       vs = live ? __ldg(a.c.v_scale + ph) : 0.0f;
     };
+    // The queries' loads, under way while the first tile is looked up.
+    constexpr int QW = TERMS == 1 ? 2 : 4;  // one term: 16-bit types only
+    uint32_t qbits[NT][KS][QW];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const int row = row0 + 8 * n + r;
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int b = 0; b < QW; b++) qbits[n][s][b] = 0;
+      if (row < all_rows) {
+        const int tq = token_of(row);
+        const int64_t qi = (q.q0 + tq) * a.q_stride + (head * G + row - tq * G) * HS;
+        if constexpr (TERMS == 2)
+          if (type == RK_ACT_F32) by_stretch<HS>(c, LoadQuery<float, QW>{static_cast<const float *>(a.q) + qi, grid.vec_q, qbits[n]});
+        if (TERMS == 1 || type != RK_ACT_F32)
+          by_stretch<HS>(c, LoadQuery<uint16_t, QW>{static_cast<const uint16_t *>(a.q) + qi, grid.vec_q, qbits[n]});
+      }
+    }
     int t = t_first + wt;
     look_up(t);
     load_scales(t);
@@ -529,14 +543,21 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     float f[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-      const int row = row0 + 8 * n + r;
-      const bool have = row < all_rows;
-      const int tq = have ? token_of(row) : 0;
-      const int64_t qi = have ? (q.q0 + tq) * a.q_stride + (head * G + row - tq * G) * HS : 0;
       float v[KS][4];
 #pragma unroll
-      for (int s = 0; s < KS; s++) v[s][0] = v[s][1] = v[s][2] = v[s][3] = 0.0f;
-      if (have) by_stretch<HS>(c, LoadQuery<HS>{a.q, qi, type, grid.vec_q, v[0]});
+      for (int s = 0; s < KS; s++) {
+        if constexpr (TERMS == 2)
+          if (type == RK_ACT_F32) {
+#pragma unroll
+            for (int b = 0; b < 4; b++) v[s][b] = u2f(qbits[n][s][b]);
+            continue;
+          }
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const float2 x = type == RK_ACT_F16 ? act_pair<__half>(qbits[n][s][b]) : act_pair<__nv_bfloat16>(qbits[n][s][b]);
+          v[s][2 * b] = x.x, v[s][2 * b + 1] = x.y;
+        }
+      }
       // The largest magnitude, as bits: infinities and NaN come out on top.
       uint32_t most = 0;
 #pragma unroll
