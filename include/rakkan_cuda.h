@@ -537,9 +537,9 @@ typedef struct {
  * k_stride and v_stride elements apart, of type RK_ACT_*) at slots[t]
  * (below zero: the row is skipped). The rows of one page follow one another
  * in the call, with no skipped row between them, in ascending slots (of two rows
- * with the same slot the later one stays), and a page is in one such run only (else its contents are
- * unspecified). What a page below its run's first slot holds are earlier
- * tokens, and what lies behind the run is left as it is. For each page and
+ * with the same slot the later one stays), and a page is in one such run only
+ * (else its contents are unspecified). What a page below its run's first slot
+ * holds are earlier tokens, and what lies behind the run is left as it is. For each page and
  * head, with m the largest finite magnitude of the run:
  *   scale = max(the page's scale if it holds earlier tokens, m * fl(1/127)),
  *           zero when below 2^-120;
@@ -560,9 +560,9 @@ int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const voi
  * out_stride elements apart; rows of no request are neither read nor
  * written. Scores, sums and weighted values are held in float32, keys and
  * values enter exactly. A row of queries enters as integers of 16 bits
- * (float32: 24) of its largest magnitude, a softmax weight as float16
- * (float32: as two, 22 bits); weights below 2^-126 of the largest count as
- * zero.
+ * (float32: 24) of its largest magnitude, a softmax weight (times its page's
+ * value scale) as float16 (float32: as two, 22 bits), to within 2^-38 of the
+ * largest such: smaller ones count as zero.
  * workspace: rk_kv8_attention_workspace() bytes, 16-byte aligned, used during the
  * call's kernels only; calls that may run at once (on different streams, or
  * captured into graphs that may) need one each. A table of at most

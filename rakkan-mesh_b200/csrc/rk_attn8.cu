@@ -132,9 +132,10 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   const int hs = a.c.head_size, G = a.heads / a.c.kv_heads;
   // Two tiles of 8 rows a warp halve the conversions a row costs, once the
   // requests have more than 16 rows a kv head on average (16 requests over 2048
-  // tokens, G = 4: 40.2 us with them and 37.1 without at 16 rows, 52.6 and 60.0
-  // at 32). float16 takes two terms up to 8 rows, where they cost little beside
-  // the loads: one term's rounding is not far below the output's own.
+  // tokens, G = 4: 34.0 us with them and 29.8 without at 16 rows, 39.2 and
+  // 44.7 at 20, 65.5 and 75.9 at 64). float16 takes two terms up to 8 rows, where
+  // they cost little beside the loads: one term's rounding is not far below the
+  // output's own.
   const bool rows = (int64_t)a.tokens * G > 8LL * a.n;
   const int terms = type == RK_ACT_F32 || (type == RK_ACT_F16 && !rows) ? 2 : 1;
   const int nt = terms == 1 && (int64_t)a.tokens * G > 16LL * a.n && hs <= 128 ? 2 : 1;

@@ -11,9 +11,9 @@
 // its own tiles through two slots of shared memory (cp.async), one under way
 // while it works on the other: tiles loaded into registers instead took 78.6
 // us for one token of 32 sequences of up to 4096 tokens (97,000 in all, 8 kv
-// heads of 128, G = 4), which takes 44.2 now: 4.5 TB/s. With 16384 tokens each it is 5.9.
+// heads of 128, G = 4), which takes 42.8 now: 4.7 TB/s. With 16384 tokens each it is 6.1.
 // With many rows a request the instructions around the products bound it, some
-// 1000 for 16 rows by 32 tokens: 512 rows over 8192 tokens 391 us, 170 TFLOP/s.
+// 1000 for 16 rows by 32 tokens: 512 rows over 8192 tokens 365 us, 180 TFLOP/s.
 //
 // Fragments. Keys and transposed values are the 16-row operand, queries and
 // weights the 8-column one: a tile of 8 query rows then fills the columns,
@@ -61,9 +61,9 @@ constexpr int kA8Threads = 32 * kA8Warps;
 constexpr int kA8Tile = 32;  // tokens
 // What a unit's beginning and end cost a CTA, in tiles of one warp (about 5 us
 // against 0.6 us a tile where memory bounds them): a CTA that begins a second
-// unit gets so many fewer. 12 measured best for single tokens: of 6, 12 and 20
-// one token of the 32 sequences took 47.9, 47.0 and 48.2 us, and 8 x 64 rows
-// over up to 2048 tokens 72.2, 71.1 and 69.5.
+// unit gets so many fewer. With 6, 9, 12 and 16 one token of the 32 sequences
+// takes 43.1, 43.1, 42.6 and 43.4 us, 8 x 64 rows over up to 2048 tokens 55.5,
+// 54.7, 53.9 and 54.0.
 constexpr int kA8Begin = 12;
 template <int HS>
 struct A8Shape {
