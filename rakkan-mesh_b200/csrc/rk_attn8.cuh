@@ -11,9 +11,9 @@
 // its own tiles through two slots of shared memory (cp.async), one under way
 // while it works on the other: tiles loaded into registers instead took 78.6
 // us for one token of 32 sequences of up to 4096 tokens (97,000 in all, 8 kv
-// heads of 128, G = 4), which takes 42.8 now: 4.7 TB/s. With 16384 tokens each it is 6.1.
+// heads of 128, G = 4), which takes 42.8 now: 4.7 TB/s. With 16384 tokens each it is 6.0.
 // With many rows a request the instructions around the products bound it, some
-// 1000 for 16 rows by 32 tokens: 512 rows over 8192 tokens 365 us, 180 TFLOP/s.
+// 1000 for 16 rows by 32 tokens: 512 rows over 8192 tokens 366 us, 182 TFLOP/s.
 //
 // Fragments. Keys and transposed values are the 16-row operand, queries and
 // weights the 8-column one: a tile of 8 query rows then fills the columns,
