@@ -559,10 +559,13 @@ int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const voi
  * NaN. q and out are [tokens][heads][head_size] of `type`, rows q_stride and
  * out_stride elements apart; rows of no request are neither read nor
  * written. Scores, sums and weighted values are held in float32, keys and
- * values enter exactly. A row of queries enters as integers of 16 bits
- * (float32: 24) of its largest magnitude, a softmax weight (times its page's
- * value scale) as float16 (float32: as two, 22 bits), to within 2^-38 of the
- * largest such: smaller ones count as zero.
+ * values enter exactly. A row of queries enters as integers of 24 bits of its
+ * largest magnitude (of 2^-100, if that is larger; bfloat16: of 16 bits), a
+ * softmax weight (times its page's value scale) as two float16, 22 bits
+ * (bfloat16: as one), to within 2^-38 of the largest such: smaller ones count
+ * as zero. The kernel's tiles go by tokens / n, so a q far larger than the
+ * step's rows costs time, and the order of sums with it; the precision goes by
+ * the type alone.
  * workspace: rk_kv8_attention_workspace() bytes, 16-byte aligned, used during the
  * call's kernels only; calls that may run at once (on different streams, or
  * captured into graphs that may) need one each. A table of at most

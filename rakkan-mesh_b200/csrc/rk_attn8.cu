@@ -133,12 +133,14 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   // Two tiles of 8 rows a warp halve the conversions a row costs, once the
   // requests have more than 16 rows a kv head on average (16 requests over 2048
   // tokens, G = 4: 34.0 us with them and 29.8 without at 16 rows, 39.2 and
-  // 44.7 at 20, 65.5 and 75.9 at 64). float16 takes two terms up to 8 rows, where
-  // they cost little beside the loads: one term's rounding is not far below the
-  // output's own.
+  // 44.7 at 20, 65.5 and 75.9 at 64, bfloat16; float32 49.7 and 54.8 at 20, 85.0
+  // and 95.2 at 64).
   const bool rows = (int64_t)a.tokens * G > 8LL * a.n;
-  const int terms = type == RK_ACT_F32 || (type == RK_ACT_F16 && !rows) ? 2 : 1;
-  const int nt = terms == 1 && (int64_t)a.tokens * G > 16LL * a.n && hs <= 128 ? 2 : 1;
+  const int nt = (int64_t)a.tokens * G > 16LL * a.n && hs <= 128 ? 2 : 1;
+  // The precision goes by the type alone, so that a row's does not depend on
+  // what else the call holds. One term's rounding (2^-12 of a weight) is an
+  // eighth of bfloat16's of the output, but not far below float16's own.
+  const int terms = type == RK_ACT_BF16 ? 1 : 2;
   A8Grid g{sms * a8_ctas(hs, terms, nt), 4, a.c.block == 16 ? 4 : a.c.block == 32 ? 5 : a.c.block == 64 ? 6 : 7,
            a.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0,
            a.out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & (type == RK_ACT_F32 ? 15 : 7)) == 0,
@@ -147,7 +149,7 @@ cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStre
   // two there is nothing to join.
   const bool whole = (int64_t)a.max_blocks * a.c.block <= RK_KV8_NO_WORKSPACE;
   if (whole) g.min_tiles = 0;
-  cudaError_t e = terms == 2 ? attn8_main_two(a, type, g, st) : A8<1>::at(hs, A8<1>::Launch{a, type, nt, g, st});
+  cudaError_t e = terms == 2 ? attn8_main_two(a, type, nt, g, st) : A8<1>::at(hs, A8<1>::Launch{a, type, nt, g, st});
   if (e != cudaSuccess || whole) return e;
   // The join may be placed while the main kernel's last CTAs run; it waits
   // for them before it reads.

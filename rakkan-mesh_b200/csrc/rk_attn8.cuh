@@ -27,14 +27,19 @@
 // the second product's column operand, which fixes the token of each key row.
 //
 // Precision. The scores' product is mma.m16n8k32 on signed bytes: the keys
-// as they are, a row of queries as integers of two signed bytes (16-bit types,
-// the row's largest at 32639: off by at most 2^-16 of it) or three (float32,
-// 2^-24), each its own exact product, joined in float32. (float16 products
-// would want the keys converted: 58.3 us in place of 48.9 at the time.) The
-// softmax weights are float16, one term for 16-bit types (2^-12 of itself:
-// an eighth of bfloat16's own rounding of the result, and half of float16's
-// on average over tokens) and two for float32 (22 bits), with the value scale
-// in the weight: w_t = 2^(s_t - M + E + 14) f for vs = f 2^E, M within a power of two
+// as they are, a row of queries as integers of two signed bytes (bfloat16,
+// the row's largest at 32639: off by at most 2^-16 of it) or three (float32 and
+// float16, 2^-24), each its own exact product, joined in float32. (float16
+// products would want the keys converted: 58.3 us in place of 48.9 at the time.)
+// The softmax weights are float16, one term for bfloat16 (2^-12 of itself:
+// an eighth of bfloat16's own rounding of the result) and two for the others
+// (22 bits): float16's rounding of the result is 2^-11, and one term raised
+// the error of float16 pieces from 2.1e-4 to 2.8e-4. The type alone decides:
+// what a row gives does not lose precision by what else the call holds. (8 x 64
+// rows of float16 over up to 2048 tokens take 69 us, 54 with one term.) With
+// one term the products' own sums run over all tiles; their adder does not
+// round, which costs 7e-6 of the result over 4600 tokens, against bfloat16's
+// 2e-3. The value scale is in the weight: w_t = 2^(s_t - M + E + 14) f for vs = f 2^E, M within a power of two
 // of the running maximum of s_t + E + 1 and so w_t < 2^16. The denominator has
 // a reference of its own (m), so that pages of any two scales are weighed
 // rightly.
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       vs = live ? __ldg(a.c.v_scale + ph) : 0.0f;
     };
     // The queries' loads, under way while the first tile is looked up.
-    constexpr int QW = TERMS == 1 ? 2 : 4;  // one term: 16-bit types only
+    constexpr int QW = TERMS == 1 ? 2 : 4;  // one term: bfloat16 only
     uint32_t qbits[NT][KS][QW];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -554,7 +559,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
           }
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-          const float2 x = type == RK_ACT_F16 ? act_pair<__half>(qbits[n][s][b]) : act_pair<__nv_bfloat16>(qbits[n][s][b]);
+          const float2 x = TERMS == 2 ? act_pair<__half>(qbits[n][s][b]) : act_pair<__nv_bfloat16>(qbits[n][s][b]);
           v[s][2 * b] = x.x, v[s][2 * b + 1] = x.y;
         }
       }
@@ -748,9 +753,9 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
         // Tokens 8c .. 8c + 7 of two dimensions.
         const uint2 v0 = lds64(vt + 16 * d * TT);
         const uint2 v1 = lds64(vt + (16 * d + 8) * TT);
-        // Float32 results: a tile's sums of their own, added outside. The
-        // products' adder does not round, and over thousands of tokens that
-        // shows (6.7e-6 of the result over 4600).
+        // Two terms: a tile's sums of their own, added outside. The products'
+        // adder does not round, and over thousands of tokens that shows
+        // (6.7e-6 of a float32 result over 4600).
         float part[NT][4] = {};
 #pragma unroll
         for (int s = 0; s < 2; s++) {
@@ -880,10 +885,9 @@ struct A8 {
     }
     return cudaErrorInvalidValue;
   }
-  // Two tiles of 8 rows a warp where the registers allow it: one term, heads
-  // up to 128.
+  // Two tiles of 8 rows a warp where the registers allow it: heads up to 128.
   template <int HS>
-  static constexpr bool two_tiles() { return TERMS == 1 && HS <= 128; }
+  static constexpr bool two_tiles() { return HS <= 128; }
   struct Init {
     template <int HS>
     cudaError_t operator()() const {
@@ -915,6 +919,6 @@ struct A8 {
 };
 
 cudaError_t attn8_init_two();
-cudaError_t attn8_main_two(const Attn8Args &a, int type, A8Grid g, cudaStream_t st);
+cudaError_t attn8_main_two(const Attn8Args &a, int type, int nt, A8Grid g, cudaStream_t st);
 
 }  // namespace rk

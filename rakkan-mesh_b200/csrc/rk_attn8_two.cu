@@ -5,8 +5,8 @@
 namespace rk {
 
 cudaError_t attn8_init_two() { return A8<2>::init(); }
-cudaError_t attn8_main_two(const Attn8Args &a, int type, A8Grid g, cudaStream_t st) {
-  return A8<2>::at(a.c.head_size, A8<2>::Launch{a, type, 1, g, st});
+cudaError_t attn8_main_two(const Attn8Args &a, int type, int nt, A8Grid g, cudaStream_t st) {
+  return A8<2>::at(a.c.head_size, A8<2>::Launch{a, type, nt, g, st});
 }
 
 }  // namespace rk

@@ -793,3 +793,25 @@ def test_binding_refuses_tensors(torch, dev):
         assert e.value.code == rk.RK_ERR_ARGS
     m.free()
     rk.device_check(dev)
+
+
+# ---- calls beside the ordinary ones ------------------------------------
+
+
+@pytest.mark.parametrize("new,spare", [([1, 1, 1], 0), ([1, 1, 1], 253), ([1, 1, 1, 64], 0), ([2, 40], 0)], ids=str)
+def test_attention_precision_goes_by_type_alone(torch, dev, new, spare):
+    """float16 queries enter with 24 bits and their weights with 22 whatever else the call holds: alone, in a buffer far
+    larger than its rows, beside a prompt. So the float32 bound holds with float16's own rounding on top. (The value
+    scales lie half a step beside a float16, where a weight held in one float16 is off by 2^-12.)"""
+    rng = np.random.default_rng(30)
+    kv, _ = cache(torch, dev, rng, 40, 2, 16, 64)
+    kv.v_scale.fill_(1 + 0.98 * 2.0 ** -11)
+    lens = [90, 33, 100, 150][:len(new)]
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(int).tolist()
+    q = torch.from_numpy(rng.normal(0, 1, (starts[-1] + spare, 4, 64))).cuda().half()
+    table = torch.arange(40, dtype=torch.int32, device="cuda").view(4, 10)[:len(new)].contiguous()
+    got = kv.attention(q, table, ints(torch, lens), q_start=ints(torch, starts))[:starts[-1]]
+    want, *more = (x[:starts[-1]] for x in attention_exact(torch, kv, q.float(), table, lens, starts, 1 / 8, 0))
+    most = attention_bound("f32", want, *more)
+    off, allowed = (got.double() - want).abs(), most + HALF["f16"] * (want.abs() + most) + 2.0 ** -25
+    assert bool((off <= allowed).all()), (off / allowed).max().item()
