@@ -556,8 +556,10 @@ int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const voi
  * over the tokens t up to the query's own position and, when window > 0, the
  * last `window` of those (its own among them); scale 0 is 1/sqrt(head_size).
  * A query that sees no token gives zeros; one with a NaN or infinity gives
- * NaN. q and out are [tokens][heads][head_size] of `type`, rows q_stride and
- * out_stride elements apart; rows of no request are neither read nor
+ * NaN. Entries of pages that no query of a request sees (in front of its
+ * windows, behind its length) are not followed. q and out are
+ * [tokens][heads][head_size] of `type`, rows q_stride and out_stride elements
+ * apart; rows of no request are neither read nor
  * written. Scores, sums and weighted values are held in float32, keys and
  * values enter exactly. A row of queries enters as integers of 24 bits of its
  * largest magnitude (of 2^-100, if that is larger; bfloat16: of 16 bits), a

@@ -438,14 +438,16 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     // The same of the whole unit: the tiles that its warps go through together.
     const int reach = max(-1, min(pos0 + token_of(unit_row0 + unit_rows - 1), q.len - 1));
     const int pos_first = pos0 + token_of(unit_row0);
-    const int t_first = a.window > 0 && pos_first >= a.window
-                            ? max(t0, min(q.len, pos_first - a.window + 1) / TT - q.tile0) : t0;
+    const int seen = a.window > 0 && pos_first >= a.window ? min(q.len, pos_first - a.window + 1) : 0;  // its first token
+    const int t_first = max(t0, seen / TT - q.tile0);
     const int t_end = min(t1, reach / TT + (reach >= 0) - q.tile0);
 
     // A group of rw warps shares the tiles t_first + wt, + tw, ..., and copies
     // each together while it works on the one before. page[h] is the page of
     // the copied tile's tokens 16h.. (one page from 32 tokens on). A page
-    // outside the cache is left out: page 0 is copied in its place, and masked.
+    // outside the cache is left out: page 0 is copied in its place, and masked;
+    // so is a page of 16 tokens that no row of the unit sees (in front of the
+    // windows or behind the last row), whose entry is not read.
     char *ring = sm + wt * 2 * Shape::TILE;
     const int *table = a.table + (int64_t)req * a.max_blocks;
     const uint32_t page_bytes = (uint32_t)(H * HS) << lb;
@@ -455,19 +457,23 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
     const int8_t *v_lane = a.c.v + (((int64_t)head * HS + (lane >> 1)) << lb) + 16 * (lane & 1);
     const int key_piece = (16 * lane) ^ key_swizzle<HS>(16 * lane / HS);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-    int page[2];  // -1: outside the cache
+    int page[2];  // -1: left out
     float ks = 0.0f, vs = 0.0f;  // scales of the next tile, of the page of this lane's tokens
     bool live = false;
     auto look_up = [&](int t) {
       page[0] = page[1] = -1;
       if (t < t_end) {
         const int tok = (q.tile0 + t) * TT;
-        page[0] = __ldg(table + (tok >> lb));
-        bool wrong = (unsigned)page[0] >= (unsigned)a.c.blocks;
-        if (wrong) page[0] = -1;
-        page[1] = page[0];
-        if (lb == 4) {
-          page[1] = tok + 16 <= reach ? __ldg(table + (tok >> lb) + 1) : 0;
+        bool wrong = false;
+        if (lb > 4 || tok + 16 > seen) {
+          page[0] = __ldg(table + (tok >> lb));
+          wrong = (unsigned)page[0] >= (unsigned)a.c.blocks;
+          if (wrong) page[0] = -1;
+        }
+        if (lb > 4) {
+          page[1] = page[0];
+        } else if (tok + 16 <= reach) {
+          page[1] = __ldg(table + (tok >> lb) + 1);
           if ((unsigned)page[1] >= (unsigned)a.c.blocks) wrong = true, page[1] = -1;
         }
         if (wrong) atomicExch(a.err, DEV_ERR_RANGE);

@@ -815,3 +815,46 @@ def test_attention_precision_goes_by_type_alone(torch, dev, new, spare):
     most = attention_bound("f32", want, *more)
     off, allowed = (got.double() - want).abs(), most + HALF["f16"] * (want.abs() + most) + 2.0 ** -25
     assert bool((off <= allowed).all()), (off / allowed).max().item()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_attention_does_not_depend_on_pages_it_does_not_hold(torch, dev, t):
+    """Pages of no request, page 0 among them, may hold anything: the last 16 tokens of a tile of 32 may have no page."""
+    rng = np.random.default_rng(33)
+    kv, _ = cache(torch, dev, rng, 12, 2, 16, 32)
+    q = torch.from_numpy(rng.normal(0, 1, (3, 4, 32))).cuda().to(dtype(torch, t))
+    table = torch.tensor([[3, 0, 0], [4, 5, 6], [7, -1, -1]], dtype=torch.int32, device="cuda")
+    args = table, ints(torch, [10, 48, 16])
+    want = kv.attention(q, *args)
+    for scale in (math.nan, math.inf):
+        for x in (kv.k_scale, kv.v_scale):
+            x[:3] = scale
+            x[8:] = scale
+        assert bool(torch.equal(kv.attention(q, *args), want))
+    rk.device_check(dev)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("block", [16, 32, 64])
+@pytest.mark.parametrize("window", [1, 16, 20, 100])
+def test_attention_pages_in_front_of_the_window(torch, dev, t, block, window):
+    """Pages that lie wholly in front of every row's window may have left the table: nothing looks them up."""
+    rng = np.random.default_rng(34)
+    lens, new = [300, 141, 47, 16, 33, 128], [1, 3, 1, 1, 2, 1]
+    need = [-(-n // block) for n in lens]
+    kv, _ = cache(torch, dev, rng, sum(need), 2, block, 32)
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(int).tolist()
+    q = torch.from_numpy(rng.normal(0, 1, (starts[-1], 4, 32))).cuda().to(dtype(torch, t))
+    whole, at = np.full((len(lens), max(need)), -1, np.int32), 0
+    for i, n in enumerate(need):
+        whole[i, :n] = range(at, at + n)
+        at += n
+    gone = whole.copy()
+    for i, n in enumerate(lens):
+        first = max(0, n - new[i] + 1 - window)  # the first row's first visible token
+        gone[i, :first // block] = -1
+    rk.device_check(dev)
+    want, got = (kv.attention(q, torch.from_numpy(x).cuda(), ints(torch, lens), q_start=ints(torch, starts), window=window)
+                 for x in (whole, gone))
+    rk.device_check(dev)
+    assert bool(torch.equal(got, want))
