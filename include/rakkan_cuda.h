@@ -555,8 +555,9 @@ int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const voi
  *   out = sum_t softmax_t(scale * q.k_t) v_t
  * over the tokens t up to the query's own position and, when window > 0, the
  * last `window` of those (its own among them); scale 0 is 1/sqrt(head_size).
- * A query that sees no token gives zeros; one with a NaN or infinity gives
- * NaN. Entries of pages that no query of a request sees (in front of its
+ * A query that sees no token gives zeros; one with a NaN or infinity, or that
+ * sees a token of a page with a scale that is not finite, gives NaN. Scales
+ * may have either sign. Entries of pages that no query of a request sees (in front of its
  * windows, behind its length) are not followed. q and out are
  * [tokens][heads][head_size] of `type`, rows q_stride and out_stride elements
  * apart; rows of no request are neither read nor

@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       copy_wait<0>();
       if (rw == 1) __syncwarp();
       else asm volatile("bar.sync %0, %1;" ::"r"(1 + wt), "r"(32 * rw) : "memory");
-      const float cks = ks, cvs = vs;
+      float cks = ks, cvs = vs;
       const bool clive = live;
       load_scales(t + tw);
       copy_tile(t + tw, it ^ 1);
@@ -669,9 +669,12 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
             else sc[s][n][x] = fmaf((float)si[0][n][x], 65536.0f, (float)(256 * si[1][n][x] + si[DIGITS - 1][n][x]));
           }
       }
-      // vs = vf · 2^ve; a scale of zero: weights of zero.
-      const int ex = max(int(f2u(cvs) >> 23) - 127, -126);
-      const float ve = cvs > 0.0f ? (float)ex : -1e30f;
+      // A scale that is not finite makes the scores NaN, where the page is
+      // visible, and leaves the weights of zero elsewhere.
+      if (!(fabsf(cks) < INFINITY && fabsf(cvs) < INFINITY)) cks = u2f(kCanonNaN), cvs = 0.0f;
+      // vs = vf · 2^ve, vf with the sign; a scale of zero: weights of zero.
+      const int ex = max(int(f2u(cvs) >> 23 & 255) - 127, -126);
+      const float ve = cvs != 0.0f ? (float)ex : -1e30f;
       const float vf = cvs * u2f(uint32_t(127 - min(ex, 126)) << 23) * (ex > 126 ? 0.5f : 1.0f);
       const bool whole = __all_sync(0xffffffffu, clive) && tok0 + TT - 1 <= high_min && tok0 > low_max;
 

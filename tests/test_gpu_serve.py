@@ -858,3 +858,47 @@ def test_attention_pages_in_front_of_the_window(torch, dev, t, block, window):
                  for x in (whole, gone))
     rk.device_check(dev)
     assert bool(torch.equal(got, want))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [None, [20, 7]], ids=str)
+def test_attention_scales_below_zero(torch, dev, t, new):
+    """A page's integers times its scale, whatever the scale's sign."""
+    rng = np.random.default_rng(31)
+    kv, _ = cache(torch, dev, rng, 12, 2, 16, 64)
+    kv.k_scale[::3].neg_()
+    kv.v_scale[::2].neg_()
+    lens, starts = [90, 80], [0, 1, 2] if new is None else [0, 20, 27]
+    q = torch.from_numpy(rng.normal(0, 1, (starts[-1], 4, 64))).cuda().to(dtype(torch, t))
+    table = torch.arange(12, dtype=torch.int32, device="cuda").view(2, 6)
+    got = kv.attention(q, table, ints(torch, lens), q_start=None if new is None else ints(torch, starts))
+    want, *more = attention_exact(torch, kv, q, table, lens, starts, 1 / 8, 0)
+    assert bool(((got.double() - want).abs() <= attention_bound(t, want, *more)).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_attention_scales_that_are_not_finite(torch, dev, t, scale, which):
+    """Rows that see a token of such a page give NaN; the others give what they give without it."""
+    rng = np.random.default_rng(32)
+    kv, _ = cache(torch, dev, rng, 12, 1, 16, 32)
+    q = torch.from_numpy(rng.normal(0, 1, (30, 2, 32))).cuda().to(dtype(torch, t))
+    table = torch.tensor([[0, 1, 2, 3], [4, 5, 6, 7]], dtype=torch.int32, device="cuda")
+    args = table, ints(torch, [40, 64]), ints(torch, [0, 20, 30])
+    want = kv.attention(q, *args)
+    getattr(kv, which)[1] = scale  # tokens 16 .. 31 of the first request, whose rows are at 20 .. 39
+    getattr(kv, which)[8:] = scale
+    getattr(kv, which)[3] = scale  # behind the first request's end
+    got = kv.attention(q, *args)
+    assert bool(got[:20].isnan().all())
+    assert bool(torch.equal(got[20:], want[20:]))
+    kv.k_scale[1] = kv.v_scale[1] = 0.01
+    getattr(kv, which)[1] = scale
+    rows = ints(torch, [0, 20, 20])
+    lens = ints(torch, [25, 0])  # rows at 5 .. 24: those up to 15 do not see page 1
+    got = kv.attention(q, table, lens, q_start=rows)
+    getattr(kv, which)[1] = 0.01
+    want = kv.attention(q, table, lens, q_start=rows)
+    assert bool(got[11:20].isnan().all())
+    assert bool(torch.equal(got[:11], want[:11]))
