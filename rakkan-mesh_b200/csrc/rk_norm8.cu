@@ -104,7 +104,8 @@ __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int 
   for (int k = 0; k < K; k++)
     if (at_of(k) < a.cols) w[k].load(static_cast<const T *>(a.weight) + at_of(k));
   // Values within ±127 of their base need no clamp; a thread with a NaN or an
-  // infinity among its h (then its squares' sum is one) or weights does.
+  // infinity among its h (then its squares' sum is one), weights or products
+  // (then its largest is one, and it times the factor of zero a NaN) does.
   bool odd_weights = false;
 #pragma unroll
   for (int k = 0; k < K; k++)
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(K <= 2 ? 1024 : 512) k_norm8(Norm8Args a, int 
       all = fmaxf(all, top[k]);
     }
     if (row + gridDim.x < a.rows) load(row + gridDim.x);
-    const bool odd = odd_weights || !(ss < INFINITY);
+    const bool odd = odd_weights || !(ss < INFINITY) || !(all < INFINITY);
     auto store = [&](int k, float inv) {
       const int at = at_of(k);
       if (at >= a.cols) return;

@@ -902,3 +902,18 @@ def test_attention_scales_that_are_not_finite(torch, dev, t, scale, which):
     want = kv.attention(q, table, lens, q_start=rows)
     assert bool(got[11:20].isnan().all())
     assert bool(torch.equal(got[:11], want[:11]))
+
+
+def test_norm_products_past_float32(torch, dev):
+    """h and weight finite, their product infinite: the group's factor is zero, and so are its integers."""
+    for t, cols, group in (("f32", 64, 32), ("f32", 64, 0), ("f32", 77, 11), ("f32", 66, 2), ("bf16", 256, 64)):
+        x = torch.randn((3, cols), device="cuda")
+        w = torch.ones(cols, device="cuda")
+        x[1, 3], w[3], w[5] = 1e10, 1e30, 1e-3
+        x[1, 5] = -2.0
+        x, w = x.to(dtype(torch, t)), w.to(dtype(torch, t))
+        check_norm(torch, dev, x[::2].contiguous(), w, 1e-5, group)
+        q, s, _ = rk.add_rmsnorm_q8(dev, x, w, 1e-5, group=group)
+        assert bool((q[1, :group or cols] == 0).all()) and s[1, 0] == math.inf
+        if group:
+            check_norm(torch, dev, x[:, group:].contiguous(), w[group:].contiguous(), 1e-5, group)
