@@ -540,11 +540,12 @@ typedef struct {
  * with the same slot the later one stays), and a page is in one such run only
  * (else its contents are unspecified). What a page below its run's first slot
  * holds are earlier tokens, and what lies behind the run is left as it is. For each page and
- * head, with m the largest finite magnitude of the run:
- *   scale = max(the page's scale if it holds earlier tokens, m * fl(1/127)),
- *           zero when below 2^-120;
+ * head, with m the largest finite magnitude of the run and old the page's
+ * scale (if it holds earlier tokens, else 0; NaN as 0):
+ *   scale = max(|old|, m * fl(1/127)), zero when below 2^-120;
  *   new values: clamp(RoundToEven(x * fl(1/scale)), +-127), NaN as 0;
- *   earlier ones, when the scale grew: RoundToEven(q * fl(old / scale)). */
+ *   earlier ones, when scale is not old: RoundToEven(q * fl(old / scale)),
+ *   NaN (of an infinite scale) as 0, 128 as 127. */
 int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const void *k, int64_t k_stride, const void *v,
                   int64_t v_stride, const int32_t *slots, void *stream);
 

@@ -229,9 +229,10 @@ RK_DEV uint32_t quant4(const float *x, float inv, bool odd) {
                       (uint32_t)quant127(x[3], inv));
   return pack_bytes(quant127_bits(x[0], inv), quant127_bits(x[1], inv), quant127_bits(x[2], inv), quant127_bits(x[3], inv));
 }
+// Stored bytes times a ratio within ±1 (-1 makes 128 of -128, which stays 127).
 RK_DEV uint32_t requant4(uint32_t w, float ratio) {
-  return pack_bytes(quant127_bits((float)(int8_t)w, ratio), quant127_bits((float)(int8_t)(w >> 8), ratio),
-                    quant127_bits((float)(int8_t)(w >> 16), ratio), quant127_bits((float)(int8_t)(w >> 24), ratio));
+  const auto again = [&](uint32_t b) { return f2u(__fadd_rn(fminf(__fmul_rn((float)(int8_t)b, ratio), 127.0f), 12582912.0f)); };
+  return pack_bytes(again(w), again(w >> 8), again(w >> 16), again(w >> 24));
 }
 // Bytes [from, to) of a word.
 RK_DEV void store_bytes(int8_t *p, uint32_t w, int from, int to) {
@@ -346,13 +347,14 @@ __global__ void __launch_bounds__(kAppThreads, sizeof(T) == 4 ? 4 : 6) k_kv8_app
       odd = __syncthreads_or(odd);
     }
     m = cta_max(m, sh);
-    float scale = fmaxf(had, __fmul_rn(m, u2f(K_1_127)));
+    float scale = fmaxf(fabsf(had), __fmul_rn(m, u2f(K_1_127)));  // of a NaN and m: m's
     if (scale < u2f(K_TINY)) scale = 0.0f;
     const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
     int8_t *pg = cache + ph * B * hs;
 
     if (had != scale) {  // earlier rows, to the larger scale
-      const float ratio = scale > 0.0f ? __fdiv_rn(had, scale) : 0.0f;
+      float ratio = scale > 0.0f ? __fdiv_rn(had, scale) : 0.0f;
+      if (ratio != ratio) ratio = 0.0f;
       if (!values) {
         for (int e = threadIdx.x; e < first * hs / 4; e += kAppThreads) {
           uint32_t *w = reinterpret_cast<uint32_t *>(pg) + e;

@@ -917,3 +917,27 @@ def test_norm_products_past_float32(torch, dev):
         assert bool((q[1, :group or cols] == 0).all()) and s[1, 0] == math.inf
         if group:
             check_norm(torch, dev, x[:, group:].contiguous(), w[group:].contiguous(), 1e-5, group)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("had,ratio", [(-2.0, -1.0), (-0.001, None), (math.nan, 0.0), (math.inf, 1.0)])
+def test_append_to_pages_of_any_scale(torch, dev, t, had, ratio):
+    """A page's scale counts by its magnitude, as zero if it is NaN; what the page held is rounded to the new one with its sign."""
+    rng = np.random.default_rng(35)
+    kv, host = cache(torch, dev, rng, 2, 2, 16, 32)
+    kv.k_scale.fill_(had)
+    kv.v_scale.fill_(had)
+    x = torch.from_numpy(rng.normal(0, 1, (3, 2, 32))).cuda().to(dtype(torch, t))
+    kv.append(x, x, ints(torch, [5, 6, 7]))
+    m = x.float().abs().amax((0, 2)).cpu().numpy() * np.float32(1 / 127)
+    s = np.maximum(m, np.float32(0 if math.isnan(had) else abs(had)))
+    for scale in (kv.k_scale, kv.v_scale):
+        np.testing.assert_array_equal(scale[0].cpu().numpy(), s)
+        assert bool((scale[1].isnan() if math.isnan(had) else scale[1] == had).all())
+    r = np.float32(had) / s if ratio is None else np.full_like(s, ratio)
+    for got, before in ((kv.k, host[0]), (kv.v.transpose(2, 3), host[1].transpose(0, 1, 3, 2))):
+        np.testing.assert_array_equal(got[0, :, :5].cpu().numpy(), np.rint(before[0, :, :5].astype(np.float32) * r[:, None, None]).astype(np.int8))
+        inv = np.where(np.isinf(s), np.float32(0), np.float32(1) / s)
+        np.testing.assert_array_equal(got[0, :, 5:8].cpu().numpy(), np.rint(x.float().cpu().numpy().transpose(1, 0, 2) * inv[:, None, None]).astype(np.int8))
+        np.testing.assert_array_equal(got[0, :, 8:].cpu().numpy(), before[0, :, 8:])
+        np.testing.assert_array_equal(got[1].cpu().numpy(), before[1])
