@@ -487,14 +487,15 @@ int rk_quantize(rk_device *d, int fmt, const float *w, int64_t n, void *q, float
  * need the alignment of their element type only, unless it says more.
  * Wrong arguments return RK_ERR_ARGS before anything is enqueued. An index
  * read on the device (a page, a slot) that lies outside the cache is never
- * followed: what it names is left out, and the device's error word is set,
- * which rk_device_check reports. */
+ * followed: what it names is left out, and an error word of these operators
+ * is set, which rk_device_check reports and no other call reads. */
 #define RK_ACT_F32 0
 #define RK_ACT_F16 1
 #define RK_ACT_BF16 2
-/* Waits for `stream` and returns RK_OK, or the status of what a kernel on
- * this device has recorded since the word was last read (RK_ERR_ARGS: an
- * index out of range; RK_ERR_TIMEOUT: a bounded wait), clearing it. */
+/* Waits for `stream` and returns RK_OK, or the status of what a kernel of
+ * these operators on this device has recorded since the last check
+ * (RK_ERR_ARGS: an index out of range), clearing it; failing that, of what a
+ * kernel of the other calls has (RK_ERR_TIMEOUT: a bounded wait). */
 int rk_device_check(rk_device *d, void *stream);
 
 /* Block tables, slots and positions from request lengths, on the GPU.

@@ -94,7 +94,10 @@ struct rk_device {
   cudaStream_t st = nullptr;
   DevLock mu;
   int64_t used = 0;
-  int *err_dev = nullptr;  // device-side error word (kernels' bounded waits)
+  // Device-side error words: [0] what kernels of the calls that wait under the
+  // device's mutex record; [1] the flush kernel's sink; [2] what the operators
+  // on the caller's buffers and streams record, which no other call reads.
+  int *err_dev = nullptr;
   // The MulVecs arena (device.go:769-793): input, its Q8_0 form, outputs.
   float *mv_x = nullptr, *mv_out = nullptr, *mv_xs = nullptr;
   int8_t *mv_qx = nullptr;
@@ -115,17 +118,19 @@ static int set_device(rk_device *d) {
   return RK_OK;
 }
 
-// Reads and clears the device error word after a synchronisation.
-static int check_dev_err(rk_device *d) {
+// Reads and clears a device error word after a synchronisation.
+static int check_err_word(int *word) {
   int e = 0;
-  CK(cudaMemcpy(&e, d->err_dev, sizeof e, cudaMemcpyDeviceToHost));
+  CK(cudaMemcpy(&e, word, sizeof e, cudaMemcpyDeviceToHost));
   if (e != 0) {
-    CK(cudaMemset(d->err_dev, 0, sizeof(int)));
+    CK(cudaMemset(word, 0, sizeof(int)));
     if (e == DEV_ERR_RANGE) return fail(RK_ERR_ARGS, "a kernel refused an out-of-range index (device error %d)", e);
     return fail(RK_ERR_TIMEOUT, "a kernel's bounded wait expired (device error %d)", e);
   }
   return RK_OK;
 }
+
+static int check_dev_err(rk_device *d) { return check_err_word(d->err_dev); }
 
 static int sync_dev(rk_device *d) {
   CK(cudaStreamSynchronize(d->st));
@@ -195,8 +200,8 @@ extern "C" int rk_device_open(int index, rk_device **out) {
   if (e == cudaSuccess) e = init_mvmany_attributes();
   if (e == cudaSuccess) e = init_serve_attributes();
   if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&d->st, cudaStreamNonBlocking);
-  if (e == cudaSuccess) e = cudaMalloc(&d->err_dev, 2 * sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(d->err_dev, 0, 2 * sizeof(int));
+  if (e == cudaSuccess) e = cudaMalloc(&d->err_dev, 3 * sizeof(int));
+  if (e == cudaSuccess) e = cudaMemset(d->err_dev, 0, 3 * sizeof(int));
   if (e == cudaSuccess) e = cudaMalloc(&d->mv_x, sizeof(float) * RK_MAX_COLS);
   if (e == cudaSuccess) e = cudaMalloc(&d->mv_qx, RK_MAX_COLS);
   if (e == cudaSuccess) e = cudaMalloc(&d->mv_xs, sizeof(float) * (RK_MAX_COLS / 32));
@@ -3816,7 +3821,7 @@ void internal_device_view(const rk_device *d, int *ordinal, int *sms, void **str
   *ordinal = d->ordinal;
   *sms = d->sms;
   *stream = d->st;
-  *err_word = d->err_dev;
+  *err_word = d->err_dev + 2;
 }
 
 // Counts device memory that a handle holds (rk_device_used).
@@ -3825,9 +3830,11 @@ void internal_device_count(rk_device *d, int64_t bytes) {
   d->used += bytes;
 }
 
+// Reads and clears those operators' word, then (if it was clear) the device's.
 int internal_device_check(rk_device *d) {
   Guard g(d);
-  return check_dev_err(d);
+  const int rc = check_err_word(d->err_dev + 2);
+  return rc ? rc : check_dev_err(d);
 }
 }  // namespace rk
 

@@ -943,3 +943,21 @@ def test_append_to_pages_of_any_scale(torch, dev, t, had, ratio):
         np.testing.assert_array_equal(got[0, :, 5:8].cpu().numpy(), np.rint(x.float().cpu().numpy().transpose(1, 0, 2) * inv[:, None, None]).astype(np.int8))
         np.testing.assert_array_equal(got[0, :, 8:].cpu().numpy(), before[0, :, 8:])
         np.testing.assert_array_equal(got[1].cpu().numpy(), before[1])
+
+
+def test_errors_of_these_operators_are_reported_by_the_check_alone(torch, dev):
+    """A bad slot or page fails no other call on the device, and is not lost to one."""
+    rng = np.random.default_rng(36)
+    kv, _ = cache(torch, dev, rng, 2, 1, 16, 16)
+    q = torch.zeros((1, 1, 16), device="cuda")
+    m = rk.Matrix(dev, 4, 32, rk.FMT_F32, np.ones((4, 32), np.float32))
+    rk.device_check(dev)
+    for bad in (lambda: kv.append(q, q, ints(torch, [99])), lambda: kv.attention(q, ints(torch, [[7]]), ints(torch, [3]))):
+        bad()
+        torch.cuda.synchronize()
+        np.testing.assert_array_equal(m.mulvec(np.ones(32, np.float32)), np.full(4, 32, np.float32))
+        with pytest.raises(rk.RkError) as e:
+            rk.device_check(dev)
+        assert e.value.code == rk.RK_ERR_ARGS
+        rk.device_check(dev)
+    m.free()
