@@ -513,7 +513,10 @@ int rk_device_check(rk_device *d, void *stream);
  * A request is refused when its rows pass max_tokens, its tokens pass
  * max_blocks * block, or the free pages do not suffice for it and those
  * before it: it takes no page, its slots are -1 and its lens is 0, so that
- * the append skips it and the attention gives zeros for its rows.
+ * the append skips it and the attention gives zeros for its rows. Its tokens
+ * stay ctx_lens[i] (not lens[i]), for a later step to take it up again. lens
+ * and info may not be the next step's ctx_lens and free_head as they lie:
+ * buffers that overlap are refused.
  * info: {rows, pages taken, requests refused, head + pages taken}.
  * n <= RK_MAX_REQUESTS; block is 16, 32, 64 or 128. */
 #define RK_MAX_REQUESTS 16384

@@ -103,6 +103,18 @@ extern "C" int rk_page_tables(rk_device *d, int n, int block, const int32_t *ctx
                         (const void *)free_head, (const void *)table, (const void *)lens, (const void *)q_start,
                         (const void *)slots, (const void *)positions, (const void *)info})
     if (!aligned(p, 4)) return bad("page tables: a misaligned buffer");
+  // Every CTA reads the inputs for itself, while others write.
+  const struct { const int32_t *p; int64_t n; bool out; const char *name; } bufs[] = {
+      {ctx_lens, n, false, "ctx_lens"}, {new_lens, n, false, "new_lens"}, {free_pages, n_free, false, "free_pages"},
+      {free_head, free_head ? 1 : 0, false, "free_head"}, {table, (int64_t)n * max_blocks, true, "table"}, {lens, n, true, "lens"},
+      {q_start, (int64_t)n + 1, true, "q_start"}, {slots, max_tokens, true, "slots"}, {positions, max_tokens, true, "positions"},
+      {info, 4, true, "info"}};
+  for (const auto &a : bufs)
+    for (const auto &b : bufs) {
+      const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+      if (&a != &b && b.out && a.n > 0 && b.n > 0 && pa < pb + 4 * (uint64_t)b.n && pb < pa + 4 * (uint64_t)a.n)
+        return bad("page tables: %s and %s overlap", a.name, b.name);
+    }
   OnDevice on(d, stream);
   TablesArgs a{n, block, n_free, max_blocks, max_tokens, ctx_lens, new_lens, free_pages, free_head,
                table, lens, q_start, slots, positions, info};

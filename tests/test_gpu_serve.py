@@ -961,3 +961,75 @@ def test_errors_of_these_operators_are_reported_by_the_check_alone(torch, dev):
         assert e.value.code == rk.RK_ERR_ARGS
         rk.device_check(dev)
     m.free()
+
+
+def test_requests_that_wait_for_a_page(torch, dev):
+    """Three sequences share pages for two: a refused request keeps its context (ctx takes lens where lens is not zero), is
+    given the same token again, and attends to all it holds once another sequence has ended."""
+    n, block, width, kvh, hs = 3, 16, 3, 1, 16
+    rng = np.random.default_rng(37)
+    kv = rk.PagedKV8.new(dev, 5, kvh, block, hs)
+    pages = rk.PageTables(dev, n, width, block, 64)
+    ctx, free, head = ints(torch, [0] * n), ints(torch, [0, 1, 2, 3, 4]), ints(torch, [0])
+    held = [[] for _ in range(n)]  # the keys of each sequence
+
+    def step(new):
+        pages.build(ctx, ints(torch, new), free, head)
+        starts, lens = pages.q_start.tolist(), pages.lens.tolist()
+        x = torch.from_numpy(rng.normal(0, 1, (64, kvh, hs)).astype(np.float32)).cuda()
+        kv.append(x, x, pages.slots)
+        for i in range(n):
+            if lens[i]:
+                held[i] += list(x[starts[i]:starts[i + 1]])
+        out = torch.zeros((64, 2, hs), device="cuda")
+        q = torch.zeros_like(out)  # even weights: the mean of the values
+        kv.attention(q, pages.table, pages.lens, q_start=pages.q_start, out=out)
+        for i in range(n):
+            for j in range(new[i]):
+                got = out[starts[i] + j, 0]
+                if not lens[i]:
+                    assert bool((got == 0).all())
+                    continue
+                seen = torch.stack(held[i])[:len(held[i]) - new[i] + j + 1, 0]
+                # each value rounded to its page's scale, at most once more a growth of it
+                assert bool(((got - seen.mean(0)).abs() <= 4 * 0.5 * 5 / 127).all())
+        ctx.copy_(torch.where(pages.lens > 0, pages.lens, ctx))
+        head.copy_(pages.info[3:4])
+        return lens
+
+    assert step([30, 16, 14]) == [30, 16, 14]          # 2 + 1 + 1 pages
+    assert step([1, 1, 1]) == [31, 17, 15]             # the last page goes to the second
+    assert step([1, 1, 1]) == [32, 18, 16]
+    assert step([1, 1, 1]) == [0, 19, 0]               # no page for the first and the third
+    assert ctx.tolist() == [32, 19, 16] and pages.info.tolist()[2] == 2
+    assert step([1, 1, 1]) == [0, 20, 0]
+    assert ctx.tolist() == [32, 20, 16]
+    ended = pages.table[1, :2].clone()                  # the second ends: its pages are free again
+    free, ctx[1], held[1] = ended, 0, []
+    head.zero_()
+    assert step([1, 0, 1]) == [33, 0, 17]
+    assert pages.table[0].tolist()[2] == ended[0] and pages.table[2].tolist()[1] == ended[1]
+    rk.device_check(dev)
+
+
+def test_tables_of_buffers_side_by_side(torch, dev):
+    """All of a call's buffers, and those between two steps, in one piece of memory."""
+    n, width, rows, block = 3, 4, 9, 16
+    ctx, new, free = [30, 0, 16], [3, 5, 1], [40, 41, 42, 43]
+    sizes = [n, n, len(free), 1, n * width, n, n + 1, rows, rows, 4]
+    at = np.concatenate([[0], np.cumsum(sizes)])
+    arena = torch.full((int(at[-1]) + 1,), -9, dtype=torch.int32, device="cuda")
+    arena[:at[4]] = ints(torch, ctx + new + free + [1])
+    table = np.full((n, width), -9, np.int32)
+    table[0, :2], table[2, :1] = (7, 8), 9
+    arena[at[4]:at[5]] = torch.from_numpy(table).cuda().flatten()
+    p = [arena[int(a):].data_ptr() for a in at[:-1]]
+    torch.cuda.synchronize()  # the call runs on the device's own stream
+    assert rk.lib().rk_page_tables(dev.h, n, block, p[0], p[1], p[2], p[3], len(free), p[4], width, p[5], p[6], p[7], p[8], rows,
+                                   p[9], None) == rk.RK_OK
+    rk.device_check(dev)
+    assert rk.lib().rk_device_check(dev.h, None) == rk.RK_OK
+    want = tables_plain(ctx, new, free, 1, table, block, rows)
+    for i, w in enumerate(want):
+        np.testing.assert_array_equal(arena[at[4 + i]:at[5 + i]].cpu().numpy(), np.array(w, np.int32).flatten())
+    assert arena[-1].item() == -9

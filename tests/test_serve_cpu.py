@@ -139,3 +139,17 @@ def test_w4_refuses():
 
 def test_device_check_refuses_null():
     refused(rk.lib().rk_device_check(None, None), "null")
+
+
+def test_tables_refuse_buffers_that_overlap():
+    """One call's outputs may not be its inputs (the next step's lengths, the free list's head), nor each other."""
+    own = {k: P + 256 * i for i, k in enumerate(("ctx", "new", "free", "head", "table", "lens", "start", "slots", "pos", "info"))}
+    ins, outs = ("ctx", "new", "free", "head"), ("table", "lens", "start", "slots", "pos", "info")
+    for o in outs:
+        for other in ins + outs:
+            if other != o:
+                refused(tables(**{**own, other: own[o]}), "page tables", "overlap")
+    refused(tables(**{**own, "head": own["info"] + 12}), "free_head", "info")
+    refused(tables(**{**own, "ctx": own["lens"] - 8}), "ctx_lens", "lens")
+    refused(tables(**{**own, "lens": own["ctx"] + 8}), "ctx_lens", "lens")
+    refused(tables(**{**own, "free": own["table"] + 4 * 3 * 4 - 4}), "free_pages", "table")
