@@ -576,7 +576,8 @@ int rk_kv8_append(rk_device *d, const rk_kv8 *c, int type, int tokens, const voi
  * the type alone.
  * workspace: rk_kv8_attention_workspace() bytes, 16-byte aligned, used during the
  * call's kernels only; calls that may run at once (on different streams, or
- * captured into graphs that may) need one each. A table of at most
+ * captured into graphs that may) need one each, calls on one stream, of
+ * several threads too, may share one. A table of at most
  * RK_KV8_NO_WORKSPACE tokens (max_blocks * block) needs none. */
 #define RK_KV8_NO_WORKSPACE 512
 int64_t rk_kv8_attention_workspace(rk_device *d, const rk_kv8 *c, int heads);

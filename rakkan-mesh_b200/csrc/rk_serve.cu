@@ -4,6 +4,7 @@
 // aside), so any of them can be captured into a CUDA graph.
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 #include <new>
 
 #include "rk_serve.cuh"
@@ -61,6 +62,10 @@ struct OnDevice {
     return internal_fail(RK_ERR_CUDA, buf);
   }
 };
+
+// Held while a call's kernels that hand a workspace on are enqueued, so that
+// those of two threads on one stream do not mix; by device.
+std::mutex g_pairs[16];
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 size_t act_size(int type) { return type == RK_ACT_F32 ? 4 : 2; }
@@ -178,6 +183,8 @@ extern "C" int rk_kv8_attention(rk_device *d, const rk_kv8 *c, int type, int n, 
   Attn8Args a{*c, n, heads, tokens, max_blocks, window, q, out, q_stride, out_stride, q_start, lens, table, scale,
               workspace, on.err};
   if (scale == 0.0f) a.scale = (float)(1.0 / __builtin_sqrt((double)c->head_size));
+  std::unique_lock<std::mutex> pair(g_pairs[on.ordinal & 15], std::defer_lock);
+  if (need > 0) pair.lock();
   return on.done(on.e == cudaSuccess ? launch_kv8_attention(a, type, on.sms, on.st) : on.e, "kv8 attention");
 }
 

@@ -1033,3 +1033,28 @@ def test_tables_of_buffers_side_by_side(torch, dev):
     for i, w in enumerate(want):
         np.testing.assert_array_equal(arena[at[4 + i]:at[5 + i]].cpu().numpy(), np.array(w, np.int32).flatten())
     assert arena[-1].item() == -9
+
+
+def test_attention_from_threads_of_one_stream(torch, dev):
+    """Two threads that call on the same stream, whose calls share the stream's workspace."""
+    import threading
+    rng = np.random.default_rng(38)
+    kv, _ = cache(torch, dev, rng, 300, 2, 32, 64)
+    table = torch.arange(300, dtype=torch.int32, device="cuda")[None].contiguous()
+    qs = [torch.from_numpy(rng.normal(0, 1, (k, 8, 64)).astype(np.float32)).cuda() for k in (1, 40)]
+    lens, starts = [ints(torch, [9600]), ints(torch, [4000])], [ints(torch, [0, 1]), ints(torch, [0, 40])]
+    want = [kv.attention(q, table, n, q_start=s) for q, n, s in zip(qs, lens, starts)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        for _ in range(200):
+            got[i].append(kv.attention(qs[i], table, lens[i], q_start=starts[i]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 200 and all(bool(torch.equal(g, want[i])) for g in got[i])
