@@ -998,6 +998,8 @@ class PagedKV8:
         shape = q.shape
         tokens, heads = shape[0], shape[1]
         width = heads * self.head_size
+        if table.dim() != 2:
+            _refuse(f"kv8 attention: a table of {table.dim()} dimensions, not 2")
         n, max_blocks = table.shape
         qp, qs = _rows(q, i, q.dtype, "kv8 attention: q", shape, width)
         if out is None:
@@ -1088,6 +1090,8 @@ class W4Matrix:
         """W.(x * x_scales) for each row of x int8 [n][cols], x_scales float32
         [n][cols / x_group]; returns [n][rows] of dtype (float32 by default), or out."""
         t, i = _torch(), self.index
+        if x.dim() != 2 or x_scales.dim() != 2:
+            _refuse(f"w4: vectors of {x.dim()} and scales of {x_scales.dim()} dimensions, not 2")
         n = x.shape[0]
         xp = _tensor(x, i, t.i8, "w4: x", (n, self.cols))
         groups = x_scales.shape[-1]

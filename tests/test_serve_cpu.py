@@ -153,3 +153,35 @@ def test_tables_refuse_buffers_that_overlap():
     refused(tables(**{**own, "ctx": own["lens"] - 8}), "ctx_lens", "lens")
     refused(tables(**{**own, "lens": own["ctx"] + 8}), "ctx_lens", "lens")
     refused(tables(**{**own, "free": own["table"] + 4 * 3 * 4 - 4}), "free_pages", "table")
+
+
+class NoDevice:
+    """A device whose tensors are the host's (get_device() is -1): the binding's own checks come first."""
+    h = None
+
+    class info:
+        index = -1
+
+
+def test_binding_refuses_shapes():
+    """Tensors of a wrong number of dimensions raise RkError like other wrong tensors."""
+    import torch
+    t = torch.zeros
+    kv = rk.PagedKV8(NoDevice, t((2, 2, 16, 32), dtype=torch.int8), t((2, 2, 32, 16), dtype=torch.int8), t((2, 2)), t((2, 2)))
+    m = object.__new__(rk.W4Matrix)
+    m.index, m.rows, m.cols, m.h = -1, 4, 64, None
+    q, i32, x8 = t((1, 4, 32)), dict(dtype=torch.int32), t((1, 64), dtype=torch.int8)
+    pages = rk.PageTables.__new__(rk.PageTables)
+    pages.dev, pages.index, pages.n = NoDevice, -1, 1
+    for call in (lambda: kv.attention(q, t(1, **i32), t(1, **i32)), lambda: kv.attention(q, t((), **i32), t(1, **i32)),
+                 lambda: kv.attention(q, t((1, 1, 1), **i32), t(1, **i32)), lambda: kv.attention(q[0], t((1, 1), **i32), t(1, **i32)),
+                 lambda: kv.append(q[0], q[0], t(1, **i32)), lambda: kv.append(q[:, :2], q[:, :2], t((1, 1), **i32)),
+                 lambda: m.mulvec(x8[0], t((1, 2))), lambda: m.mulvec(x8[0, 0], t((1, 2))), lambda: m.mulvec(x8, t(())),
+                 lambda: m.mulvec(x8, t(2)), lambda: m.mulvec(x8, t((1, 0))), lambda: m.mulvec(x8[None], t((1, 2))),
+                 lambda: rk.add_rmsnorm_q8(NoDevice, q[0, 0], q[0, 0], 1e-5), lambda: rk.add_rmsnorm_q8(NoDevice, q[0], q[0], 1e-5),
+                 lambda: pages.build(t((1, 1), **i32), t(1, **i32), t(1, **i32)),
+                 lambda: rk.W4Matrix(NoDevice, t(4, dtype=torch.uint8), t((4, 1))), lambda: rk.W4Matrix(NoDevice, t((4, 16), dtype=torch.uint8), t(4)),
+                 lambda: rk.PagedKV8(NoDevice, kv.k[0], kv.v, kv.k_scale, kv.v_scale)):
+        with pytest.raises(rk.RkError) as e:
+            call()
+        assert e.value.code == rk.RK_ERR_ARGS
