@@ -856,10 +856,18 @@ def _torch():
         # reads NULL as the device's own, so the legacy stream's handle is passed.
         _t = types.SimpleNamespace(
             torch=torch, stream=lambda index: torch._C._cuda_getCurrentRawStream(index) or 1,
-            capturing=torch.cuda.is_current_stream_capturing,
+            capturing=lambda index: _capturing(torch, index),
             act={torch.float32: ACT_F32, torch.float16: ACT_F16, torch.bfloat16: ACT_BF16},
             f32=torch.float32, i32=torch.int32, i8=torch.int8, u8=torch.uint8)
     return _t
+
+
+def _capturing(torch, index):
+    """Whether the current stream of the device is being captured (torch answers for the current device)."""
+    if torch._C._cuda_getDevice() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
 
 
 _workspaces = {}  # by device and stream
@@ -1020,10 +1028,11 @@ class PagedKV8:
                 self._ws[heads] = need
             # One workspace a stream, whose calls follow one another; in a
             # capture one of the graph's own, which may run beside others.
-            ws = None if t.capturing() else _workspaces.get((i, stream))
+            captured = t.capturing(i)
+            ws = None if captured else _workspaces.get((i, stream))
             if ws is None or ws.numel() < need:
                 ws = t.torch.empty(need, dtype=t.u8, device=q.device)
-                if not t.capturing():
+                if not captured:
                     _workspaces[i, stream] = ws
         rc = _lib.rk_kv8_attention(self.dev.h, self.at, act, n, heads, tokens, qp, qs, sp, lp, tp, max_blocks, scale, window,
                                    op, os_, ws.data_ptr() if need else None, need, stream)

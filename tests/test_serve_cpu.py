@@ -185,3 +185,31 @@ def test_binding_refuses_shapes():
         with pytest.raises(rk.RkError) as e:
             call()
         assert e.value.code == rk.RK_ERR_ARGS
+
+
+def test_capture_is_asked_of_the_operators_device():
+    """Whether a call is being captured goes by the stream of its own device, not of the current one."""
+    from types import SimpleNamespace
+
+    class Fake:
+        def __init__(self, now, capturing):
+            self.now, self.on = now, capturing
+            self._C = SimpleNamespace(_cuda_getDevice=lambda: self.now)
+            self.cuda = SimpleNamespace(is_current_stream_capturing=lambda: self.now in self.on, device=self.device)
+
+        def device(self, index):
+            fake = self
+
+            class Device:
+                def __enter__(self):
+                    self.before, fake.now = fake.now, index
+
+                def __exit__(self, *a):
+                    fake.now = self.before
+            return Device()
+    for now in (0, 1):
+        for on in ((), (0,), (1,), (0, 1)):
+            for index in (0, 1):
+                fake = Fake(now, on)
+                assert rk._capturing(fake, index) == (index in on)
+                assert fake.now == now
