@@ -1058,3 +1058,40 @@ def test_attention_from_threads_of_one_stream(torch, dev):
     torch.cuda.synchronize()
     for i in range(2):
         assert len(got[i]) == 200 and all(bool(torch.equal(g, want[i])) for g in got[i])
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("shape,group", [((5000, 640), 32), ((3001, 1000), 8), ((3001, 1001), 7), ((4001, 77), 0), ((2001, 5120), 128)],
+                         ids=str)
+def test_norm_many_rows(torch, dev, t, shape, group):
+    """More rows than the CTAs that the SMs hold, so that each takes several, and the sum in place."""
+    gen = torch.Generator(device="cuda").manual_seed(39)
+    x = torch.randn(shape, generator=gen, device="cuda").to(dtype(torch, t))
+    w = (1 + 0.2 * torch.randn(shape[1], generator=gen, device="cuda")).to(x.dtype)
+    res = (3 * torch.randn(shape, generator=gen, device="cuda")).to(x.dtype)
+    check_norm(torch, dev, x, w, 1e-5, group, res)
+    want = rk.add_rmsnorm_q8(dev, x, w, 1e-5, group=group, residual=res)
+    for k in range(2):  # the sum over x, over the residual
+        a, b = x.clone(), res.clone()
+        got = rk.add_rmsnorm_q8(dev, a, w, 1e-5, group=group, residual=b, sum_out=b if k else a)
+        assert all(bool(torch.equal(g, v)) for g, v in zip(got, want))
+
+
+@pytest.mark.parametrize("rows,cols,group,xg,n,zeros,st", [
+    (80000, 256, 128, 64, 1, True, "f16"), (80000, 256, 32, 32, 11, False, "bf16"),        # teams take several tiles
+    (120007, 128, 64, 128, 8, True, "f32"), (90000, 96, 32, 96, 16, True, "f16"),
+    (48, 14336, 32, 32, 9, False, "f16"), (48, 14336, 32, 32, 16, True, "f32"),            # vectors that do not fit
+    (40, 14368, 32, 32, 16, True, "f16"), (40, 14368, 32, 14368, 9, False, "f32"),
+    (40, 14400, 64, 64, 15, True, "bf16"), (5000, 8224, 32, 32, 40, True, "f16"),
+    (3000, 14336, 128, 128, 16, True, "f16"), (40000, 4128, 32, 32, 16, True, "f32"),
+    (9000, 14336, 32, 32, 16, True, "f32"), (9000, 14368, 32, 32, 9, False, "f16")], ids=str)
+def test_w4_many_tiles_and_wide_rows(torch, dev, rows, cols, group, xg, n, zeros, st):
+    w4_case(torch, dev, rows, cols, group, xg, n, zeros, st, "f32", extra=1)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hs", [16, 32, 48, 64, 80, 96, 112, 128, 256])
+def test_attention_pieces_of_every_head_size(torch, dev, t, hs):
+    """Enough rows a request for two row tiles a warp, at short tables and over a joined long one."""
+    attention_case(torch, dev, hs, 6, 2, hs, 16, [3, 60, 300], [3, 20, 64], t, spare=2)
+    attention_case(torch, dev, hs + 1, 4, 1, hs, 64, [40, 2500], [7, 33], t, window=700)
