@@ -1008,6 +1008,8 @@ class PagedKV8:
         width = heads * self.head_size
         if table.dim() != 2:
             _refuse(f"kv8 attention: a table of {table.dim()} dimensions, not 2")
+        if not 0 <= window < 1 << 31:  # an integer of the C ABI would wrap
+            _refuse(f"kv8 attention: a window of {window}")
         n, max_blocks = table.shape
         qp, qs = _rows(q, i, q.dtype, "kv8 attention: q", shape, width)
         if out is None:

@@ -213,3 +213,14 @@ def test_capture_is_asked_of_the_operators_device():
                 fake = Fake(now, on)
                 assert rk._capturing(fake, index) == (index in on)
                 assert fake.now == now
+
+
+@pytest.mark.parametrize("window", [-1, -2 ** 32, 2 ** 31, 2 ** 32, 2 ** 32 + 7])
+def test_binding_refuses_windows_past_the_abis_integers(window):
+    """A window that 32 bits do not hold is an error, not another window."""
+    import torch
+    t = torch.zeros
+    kv = rk.PagedKV8(NoDevice, t((2, 2, 16, 32), dtype=torch.int8), t((2, 2, 32, 16), dtype=torch.int8), t((2, 2)), t((2, 2)))
+    with pytest.raises(rk.RkError) as e:
+        kv.attention(t((1, 4, 32)), t((1, 1), dtype=torch.int32), t(1, dtype=torch.int32), window=window)
+    assert e.value.code == rk.RK_ERR_ARGS and "window" in str(e.value)
