@@ -594,7 +594,7 @@ int rk_kv8_attention(rk_device *d, const rk_kv8 *c, int type, int n, int heads, 
  * The quotient y / (max|y| / 127) does not depend on the row's norm, so with
  * u = fl(h * weight) and base = fl(max|u| * fl(1/127)) of a group (zero when
  * below 2^-120), q = clamp(RoundToEven(u * fl(1/base)), +-127), NaN as 0, and
- * scale = base / sqrt(mean(h^2) + eps). Rows of x, residual and sum_out are
+ * scale = base / sqrt(mean(h^2) + eps), squares summed in float32. Rows of x, residual and sum_out are
  * x_stride, r_stride and s_stride elements apart, of type RK_ACT_* as
  * weight; q is [rows][cols], scales [rows][cols / group]. */
 int rk_add_rmsnorm_q8(rk_device *d, int type, int rows, int cols, int group, const void *x, int64_t x_stride,
@@ -616,7 +616,7 @@ int64_t rk_w4_bytes(const rk_w4 *m);
  * [n][cols] (16-byte aligned) with a scale for each x_group columns (a
  * multiple of 32 that divides cols; 0: cols), as rk_add_rmsnorm_q8 makes
  * them. Products are exact integers within a run of columns that shares both
- * scales; the runs are added in float32, and out (rows out_stride elements
+ * scales (128 columns of it at a time); the runs are added in float32, and out (rows out_stride elements
  * apart) is rounded to `type` once. */
 int rk_w4_mulvec(rk_w4 *m, int n, const int8_t *x, const float *x_scales, int x_group, int type, void *out,
                  int64_t out_stride, void *stream);

@@ -67,8 +67,9 @@ constexpr int kA8Tile = 32;  // tokens
 // What a unit's beginning and end cost a CTA, in tiles of one warp (about 5 us
 // against 0.6 us a tile where memory bounds them): a CTA that begins a second
 // unit gets so many fewer. With 6, 9, 12 and 16 one token of the 32 sequences
-// takes 43.1, 43.1, 42.6 and 43.4 us, 8 x 64 rows over up to 2048 tokens 55.5,
-// 54.7, 53.9 and 54.0.
+// takes 43.1, 43.1, 42.6 and 43.4 us, 8 x 64 rows over up to 2048 tokens (one
+// term) 55.5, 54.7, 53.9 and 54.0; heads of 128 in both, and the one value
+// serves the other sizes, where it was not varied.
 constexpr int kA8Begin = 12;
 template <int HS>
 struct A8Shape {

@@ -153,7 +153,8 @@ cudaError_t launch_page_tables(const TablesArgs &a, int sms, cudaStream_t st) {
 // loaded once, into registers; longer ones and rows off 16-byte boundaries are
 // read twice, the second time from L1 or L2. The prompts of 16 sequences (8470
 // tokens, 8 heads of 128, bfloat16) take 21.5 us, 2.4 TB/s, and 32.5 with every
-// run read twice; what is left is each run's chain of load, maximum, store. Values are stored transposed: the
+// run read twice; what is left is each run's chain of load, maximum, store, and
+// 59% of the issue slots. Values are stored transposed: the
 // rounded bytes go through shared memory, from which 4 dimensions of 4 tokens
 // become 4 words, with the tokens in the fast lanes, so that a page row's words
 // are stored side by side. A CTA looks for the runs that begin in its `chunk`

@@ -18,13 +18,15 @@
 // three instructions, and the 16 goes into the vectors' scales. A zero point
 // other than 8 adds (8 − z) · 16 Σ x, with Σ x made once for each segment.
 //
-// Work. One CTA of sixteen warps an SM goes through tiles of 16 rows. KW warps
-// of it (a team) share a tile's columns; each warp keeps its share of the
-// columns from tile to tile, so the vectors and their scales are brought into
-// shared memory once (vectors that do not fit come with each record, from L2,
-// and so do scales that do not).
+// Work. CTAs of sixteen warps, at most one an SM, go through tiles of 16 rows.
+// KW warps of a CTA (a team) share a tile's columns; each warp keeps its share
+// of the columns from tile to tile, so the vectors and their scales are brought
+// into shared memory once (vectors that do not fit come with each record, from
+// L2, and so do scales that do not). Where teams are fewer than the SMs' warps
+// each takes one tile, and whole CTAs of teams leave SMs without work: 112 of
+// 148 have some at 28672x4096, 128 at 4096x14336.
 // The records come through a ring of each warp in shared memory, which runs on
-// over the tiles: no load waits for a tile's end. Sharing a tile's columns over
+// over the tiles of a team: its loads do not wait for a tile's end. Sharing a tile's columns over
 // the CTAs of a cluster was tried for vectors that do not fit and for few rows:
 // the exchange cost 1 to 3 us a tile. (A CTA for each tile took
 // 22.3 us for 28672x4096 by one vector: its beginning and end cost as much as
@@ -32,7 +34,7 @@
 // float32 sums of a tile's shares meet in shared memory, in order, while the
 // warps are at the next tile.
 // 28672x4096 takes 14.4 us by one vector (4.3 TB/s; some 4 us are the launch,
-// the vectors and the last tile), 128256x4096 44.4 us (6.1 TB/s, 0.93 of a plain
+// the vectors and the only tile's end, the rest 112 SMs' streams), 128256x4096 44.4 us (6.1 TB/s, 0.93 of a plain
 // copy's rate), 4096x14336 by 16 vectors in groups of 32 15.8 us.
 #include "rk_act.cuh"
 #include "rk_serve.cuh"
