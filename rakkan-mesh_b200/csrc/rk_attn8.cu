@@ -4,17 +4,6 @@
 
 namespace rk {
 
-RK_DEV float warp_top(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-RK_DEV float warp_total(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // Joins the parts of the unit that crosses into CTA c of the main kernel
 // (c = blockIdx.x + 1). The CTAs of all its crossings share its rows. A row of a
 // few parts is one warp's, a row of many all four's: a warp's lanes read its
@@ -52,10 +41,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int
         const float4 s = *reinterpret_cast<const float4 *>(part_of(i0 + lane * my_step) + 64 * hs + 4 * row);
         m = s.x, M = s.y, l = s.z;
       }
-      const float m1 = fmaxf(mm, warp_top(m)), M1 = fmaxf(MM, warp_top(M));
+      const float m1 = fmaxf(mm, warp_max(m)), M1 = fmaxf(MM, warp_max(M));
       const float ms = m1 == -INFINITY ? 0.0f : m1, Ms = M1 == -INFINITY ? 0.0f : M1;
       const float g = exp2f(M - Ms), old = exp2f(MM - Ms);
-      ll = ll * exp2f(mm - ms) + warp_total(l * exp2f(m - ms));
+      ll = ll * exp2f(mm - ms) + warp_sum(l * exp2f(m - ms));
       mm = m1, MM = M1;
 #pragma unroll
       for (int j = 0; j < J; j++) v[j].x *= old, v[j].y *= old, v[j].z *= old, v[j].w *= old;
@@ -123,7 +112,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_attn8_join(Attn8Args a, int
 }
 
 // The workspace is sized for the most CTAs that any type's kernel has.
-int64_t attn8_workspace(const rk_kv8 &c, int, int sms) {
+int64_t attn8_workspace(const rk_kv8 &c, int sms) {
   const int64_t ctas = (int64_t)sms * a8_ctas(c.head_size, 1, 1);
   return ctas * (int64_t)sizeof(A8Record) + 2 * ctas * a8_part_floats(c.head_size) * 4;
 }

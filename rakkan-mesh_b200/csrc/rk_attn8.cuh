@@ -57,6 +57,7 @@
 #include "rk_act.cuh"
 #include "rk_matvec.cuh"
 #include "rk_serve.cuh"
+#include "rk_warp.cuh"
 
 namespace rk {
 
@@ -97,10 +98,10 @@ __host__ __device__ constexpr int a8_ctas(int hs, int terms, int nt) {
 // (m, M, l), behind the records of all CTAs.
 struct A8Record {
   int first, last;       // CTAs of the unit (first < 0: no unit crosses into this CTA)
-  int req, head, row0;   // request, kv head, first query row
+  int head, row0;        // kv head, first query row
   int rows;              // query rows in the unit
   int q0;                // first row of q of the request
-  int pad;
+  int pad[2];
 };
 __host__ __device__ inline int64_t a8_part_floats(int hs) { return 64LL * (hs + 4); }
 
@@ -137,19 +138,6 @@ RK_DEV void mma16816(float *c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-RK_DEV void mma16832(int *c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// The same from sums of zero.
-RK_DEV void mma16832_first(int *c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
-}
-
 RK_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -172,25 +160,6 @@ RK_DEV uint32_t pack_rest(float a, float b, uint32_t p) {
   return pack_h2(a - __low2float(h), b - __high2float(h));
 }
 
-// Shared memory by 32-bit addresses.
-RK_DEV uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-RK_DEV uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-RK_DEV uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-RK_DEV void copy16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 RK_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 RK_DEV void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -863,12 +832,11 @@ __global__ void __launch_bounds__(kA8Threads, a8_ctas(HS, TERMS, NT)) k_attn8(At
       A8Record rec;
       rec.first = (int)((u0 + kA8Begin) / per);
       rec.last = (int)((u1 - rw) / per);
-      rec.req = req;
       rec.head = head;
       rec.row0 = unit_row0;
       rec.rows = unit_rows;
       rec.q0 = q.q0;
-      rec.pad = 0;
+      rec.pad[0] = rec.pad[1] = 0;
       records[blockIdx.x] = rec;
     }
     at = min(end, u1);

@@ -15,6 +15,7 @@
 // row of 4096 float32 values 3.1 us, most of it the launch.
 #include "rk_act.cuh"
 #include "rk_serve.cuh"
+#include "rk_warp.cuh"
 
 namespace rk {
 
@@ -60,16 +61,6 @@ RK_DEV void norm_store(T *p, const float *v) {
   }
 }
 
-RK_DEV float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-RK_DEV float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
 // 1 / sqrt(mean + eps) within a few units in the last place (the integers do
 // not depend on it).
 RK_DEV float norm_recip(float ss, float inv_cols, float eps) { return rsqrtf(fmaf(ss, inv_cols, eps)); }

@@ -151,7 +151,7 @@ extern "C" int64_t rk_kv8_attention_workspace(rk_device *d, const rk_kv8 *c, int
   int ordinal, sms, *err;
   void *own;
   internal_device_view(d, &ordinal, &sms, &own, &err);
-  return attn8_workspace(*c, heads, sms);
+  return attn8_workspace(*c, sms);
 }
 
 extern "C" int rk_kv8_attention(rk_device *d, const rk_kv8 *c, int type, int n, int heads, int tokens, const void *q,
@@ -176,7 +176,7 @@ extern "C" int rk_kv8_attention(rk_device *d, const rk_kv8 *c, int type, int n, 
       !aligned(table, 4))
     return bad("kv8 attention: a misaligned buffer");
   OnDevice on(d, stream);
-  const int64_t need = (int64_t)max_blocks * c->block <= RK_KV8_NO_WORKSPACE ? 0 : attn8_workspace(*c, heads, on.sms);
+  const int64_t need = (int64_t)max_blocks * c->block <= RK_KV8_NO_WORKSPACE ? 0 : attn8_workspace(*c, on.sms);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned(workspace, 16))))
     return bad("kv8 attention: a workspace of %lld bytes, 16-byte aligned (%lld given)", (long long)need,
                (long long)workspace_bytes);

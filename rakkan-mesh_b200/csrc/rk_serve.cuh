@@ -36,7 +36,7 @@ struct Attn8Args {
   void *ws;
   int *err;
 };
-int64_t attn8_workspace(const rk_kv8 &c, int heads, int sms);
+int64_t attn8_workspace(const rk_kv8 &c, int sms);  // of any number of heads
 cudaError_t launch_kv8_attention(const Attn8Args &a, int type, int sms, cudaStream_t st);
 
 struct Norm8Args {

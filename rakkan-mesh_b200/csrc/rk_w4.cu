@@ -38,6 +38,7 @@
 // copy's rate), 4096x14336 by 16 vectors in groups of 32 15.8 us.
 #include "rk_act.cuh"
 #include "rk_serve.cuh"
+#include "rk_warp.cuh"
 
 namespace rk {
 
@@ -117,40 +118,9 @@ cudaError_t launch_w4_stream(const uint8_t *w, const void *scales, const uint8_t
                   w4_width(group), w4_record(group, s32, zeros != nullptr), reinterpret_cast<uint32_t *>(out), words);
 }
 
-RK_DEV void imma(int *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// The same from sums of zero.
-RK_DEV void imma_first(int *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
-}
-
-// Shared memory by 32-bit addresses.
 RK_DEV uint32_t s_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-RK_DEV uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-RK_DEV uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-RK_DEV uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
 RK_DEV void copy4_s(uint32_t dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-RK_DEV void copy16_s(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // How a product is dealt out, and its shared memory.
 struct W4Plan {
@@ -198,13 +168,13 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
   const bool c_tail_x = SEG < 128 && 128 * (q1 - 1) + 16 * (lane & 7) >= a.cols;  // behind the row's end in its last stretch
   auto copy = [&] {
     if (c_left > 0) {
-      copy16_s(c_to, c_from);
-      copy16_s(c_to + 512, c_from + 512);
-      if (c_tail) copy16_s(c_to + 1024, c_from + 1024);
+      copy16(c_to, c_from);
+      copy16(c_to + 512, c_from + 512);
+      if (c_tail) copy16(c_to + 1024, c_from + 1024);
       if (!XS) {
 #pragma unroll
         for (int i = 0; i < 2 * NT; i++)
-          if ((lane >> 3) + 4 * i < nv && !(c_tile == 1 && c_tail_x)) copy16_s(c_to + c_xto + 512 * i, c_x + (int64_t)4 * i * a.cols);
+          if ((lane >> 3) + 4 * i < nv && !(c_tile == 1 && c_tail_x)) copy16(c_to + c_xto + 512 * i, c_x + (int64_t)4 * i * a.cols);
         c_x += 128;
         if (c_tile == 1) c_x -= 128 * len;
       }
@@ -309,12 +279,12 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4(W4Args a, W4Plan p, int
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           const uint2 xv = lds64((XS ? x_now : now) + xr[n] + x_step[s]);
-          if (s * 32 % SEG == 0) imma_first(sum[n], a0, a1, a2, a3, xv.x, xv.y);
-          else imma(sum[n], a0, a1, a2, a3, xv.x, xv.y);
+          if (s * 32 % SEG == 0) mma16832_first(sum[n], {a0, a1, a2, a3}, xv.x, xv.y);
+          else mma16832(sum[n], {a0, a1, a2, a3}, xv.x, xv.y);
           if constexpr (ZEROS && !ENTRIES) {
             constexpr uint32_t all = 0x10101010u;
-            if (s * 32 % SEG == 0) imma_first(ones[n], all, all, all, all, xv.x, xv.y);
-            else imma(ones[n], all, all, all, all, xv.x, xv.y);
+            if (s * 32 % SEG == 0) mma16832_first(ones[n], {all, all, all, all}, xv.x, xv.y);
+            else mma16832(ones[n], {all, all, all, all}, xv.x, xv.y);
           }
         }
         if ((s + 1) * 32 % SEG == 0) {  // a segment ends

@@ -963,7 +963,7 @@ class PagedKV8:
                      _tensor(k_scale, self.index, t.f32, "kv8: k_scale", (blocks, kv_heads)),
                      _tensor(v_scale, self.index, t.f32, "kv8: v_scale", (blocks, kv_heads)), blocks, block, kv_heads, hs)
         self.at = C.addressof(self.c)
-        self._ws = {}  # workspace bytes by the number of query heads
+        self._ws = None  # bytes of the attention's workspace, the same for any number of query heads
 
     @classmethod
     def new(cls, dev, blocks, kv_heads, block, head_size):
@@ -1022,12 +1022,12 @@ class PagedKV8:
         sp = None if q_start is None else _tensor(q_start, i, t.i32, "kv8 attention: q_start", (n + 1,))
         stream, ws, need = t.stream(i), None, 0
         if max_blocks * self.block > KV8_NO_WORKSPACE:
-            need = self._ws.get(heads)
+            need = self._ws
             if need is None:
                 need = _lib.rk_kv8_attention_workspace(self.dev.h, self.at, heads)
                 if need < 0:
                     _check(need)
-                self._ws[heads] = need
+                self._ws = need
             # One workspace a stream, whose calls follow one another; in a
             # capture one of the graph's own, which may run beside others.
             captured = t.capturing(i)
